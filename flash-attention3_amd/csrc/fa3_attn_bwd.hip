@@ -1,0 +1,605 @@
+// Backward of attention with capped, biased and masked scores.
+//
+// Two job roles in one launch, as in bwd_reg_kernel (fa3_bwd_reg_kernel.h):
+// a dKV job owns 128 keys of a KV head and streams the 64-row query tiles of
+// its query heads that see any of them; a dQ job owns 128 rows (query and
+// query head) and streams the 64-key tiles.  Every output has one writer, so
+// nothing is added atomically and results are reproducible.  P and dS stay
+// in registers as the next product's operand.  A pass over dO and O before it
+// leaves -lse log2 e and -delta per row, padded to whole tiles: a row that
+// sees no key, or is not there, has -infinity in place of the first, which
+// makes its P zero.
+#include "fa3_attn_device.h"
+
+namespace fa3 {
+namespace {
+
+struct AttnBwdArgs {
+    AttnView q, k, v, dout, out, dq, dk, dv;
+    const float* lse;
+    float* softmax_d;
+    float* nlse2;   // [batch * heads_q][sqp]
+    float* ndelta;
+    int* flags;     // [batch * heads_q][sqp / 64]: a row that takes no part
+    AttnMask m;
+    float scale;
+    int heads_q, heads_kv, group, sq, sk, d, sqp;
+    int rows;  // group * sq
+    int kv_tiles, q_tiles, groups;
+    FastDiv div_hkv, div_group, div_groups, div_gpart, div_hq, div_blocks;
+};
+
+template <int D>
+struct BwdCfg {
+    using R = RegCfg<D>;
+    static constexpr int kRangeOff = R::kBytes;
+    static constexpr int kBytes = kRangeOff + 64;
+    static constexpr int kKs = D / 32, kDB = D / 16;
+};
+
+// Workgroup id's job: level < kv_tiles is a dKV job's key tile (first keys
+// first: causal's longest), then come the dQ jobs, last rows first.
+struct BwdJob {
+    int b, hkv, level;
+};
+template <typename Args>
+__device__ __forceinline__ BwdJob bwd_job(const Args& a, int id) {
+    BwdJob j;
+    int grp;
+    attn_job(id, a.groups, a.div_groups, a.div_gpart, j.level, grp);
+    j.b = fdiv(a.div_hkv, grp);
+    j.hkv = grp - j.b * a.heads_kv;
+    return j;
+}
+
+// One workgroup per 64 rows of a query head.
+template <int D, bool kBf16>
+__global__ __launch_bounds__(256) void attn_delta_kernel(AttnBwdArgs a) {
+    constexpr int kLanes = D / 8, kRows = 256 / kLanes;
+    const int blk = blockIdx.x, nb = a.sqp / 64;
+    const int bh = fdiv(a.div_blocks, blk), t = blk - bh * nb;
+    const int b = fdiv(a.div_hq, bh), h = bh - b * a.heads_q;
+    const int c = threadIdx.x % kLanes;
+    bool idle = false;
+#pragma unroll
+    for (int j = 0; j < 64 / kRows; ++j) {
+        const int i = t * 64 + j * kRows + (int)(threadIdx.x / kLanes);
+        const bool there = i < a.sq;
+        const _Float16* x = a.dout.p + b * a.dout.bs + h * a.dout.hs + (there ? i * a.dout.rs : 0);
+        const _Float16* y = a.out.p + b * a.out.bs + h * a.out.hs + (there ? i * a.out.rs : 0);
+        const float l = there ? a.lse[(int64_t)bh * a.sq + i] : kNegInf;
+        const f16x8 u = attn_row8(x, c, a.d, there), v = attn_row8(y, c, a.d, there);
+        float acc = dot8<kBf16>(u, v, 0.f);
+#pragma unroll
+        for (int o = kLanes / 2; o > 0; o >>= 1) acc += __shfl_xor(acc, o, kLanes);
+        const bool none = l == kNegInf;
+        idle |= none;
+        if (none) acc = 0.f;
+        if (c == 0) {
+            a.nlse2[(int64_t)bh * a.sqp + i] = none ? kNegInf : -l * kLog2e;
+            a.ndelta[(int64_t)bh * a.sqp + i] = -acc;
+            if (there && a.softmax_d != nullptr) a.softmax_d[(int64_t)bh * a.sq + i] = acc;
+        }
+    }
+    const int any = __syncthreads_or(idle);
+    if (threadIdx.x == 0) a.flags[blk] = any;
+}
+
+// Bit x of the result as all ones or zeros.
+__device__ __forceinline__ uint32_t bit_mask(uint32_t v, int x) {
+    return (uint32_t)((int32_t)(v << (31 - x)) >> 31);
+}
+// P and dS of one element.  s: raw product, dp: dP - delta, nl: -lse log2 e,
+// far: distance (bias), vis: all ones, or zeros where the element is masked.
+template <bool kCap, bool kBias>
+__device__ __forceinline__ void attn_pds(float s, float dp, float nl, float c, float k1,
+                                         float cap2, bool fine, float slope, float far,
+                                         uint32_t vis, float& p, float& ds) {
+    float x, t = 0.f;
+    if constexpr (kCap) {
+        if (fine) wall();  // (one element at a time, for the registers)
+        t = fine ? attn_tanh_fine(s, k1) : attn_tanh(s, k1);
+        x = __builtin_fmaf(t, cap2, nl);
+    } else {
+        x = __builtin_fmaf(s, c, nl);
+    }
+    if constexpr (kBias) x = __builtin_fmaf(-slope, __builtin_fabsf(far), x);
+    p = fast_exp2(x);
+    p = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, p) & vis);
+    ds = p * dp;
+    if constexpr (kCap) ds *= __builtin_fmaf(-t, t, 1.f);
+}
+
+template <int D, bool kBf16, bool kCap, bool kBias, bool kFine>
+__device__ __forceinline__ void attn_dkv(int b, int hkv, int tile, FA3_LDS char* smem) {
+    typedef AttnBwdArgs Args;
+    using C = BwdCfg<D>;
+    using R = RegCfg<D>;
+    const auto& a = attn_args<Args>();
+    const int lane = opaque_tid() & 63;
+    const int w = __builtin_amdgcn_readfirstlane(opaque_tid() >> 6);
+    const int l16 = lane & 15, g4 = lane >> 4;
+    const int kv = attn_kv(a.m, b, a.sk), off = kv - a.sq;
+    // (keys below it are seen by every query)
+    const int prefix = a.m.causal ? attn_prefix(a.m, b) : 0x7fffffff;
+    const int wg_key = tile * kAttnRows, key0 = wg_key + 32 * w;
+
+    f16x8 kf[2][C::kKs], vf[2][C::kKs];
+    int id[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const int j = key0 + 16 * n + l16;
+        id[n] = -2;
+        if (a.m.doc_k != nullptr && j < kv) id[n] = max(a.m.doc_k[b * a.m.doc_k_bs + j], -1);
+        const bool ok = j < kv && id[n] != -1;
+        const int64_t r = j < kv ? j : 0;
+        const _Float16* k = a.k.p + b * a.k.bs + hkv * a.k.hs + r * a.k.rs;
+        const _Float16* v = a.v.p + b * a.v.bs + hkv * a.v.hs + r * a.v.rs;
+#pragma unroll
+        for (int s = 0; s < C::kKs; ++s) {
+            kf[n][s] = attn_row8(k, p1_chunk<D>(s, g4), a.d, ok);
+            vf[n][s] = attn_row8(v, p1_chunk<D>(s, g4), a.d, ok);
+        }
+    }
+    DocSpan doc{0, 0, 0, 0, false};
+    const bool docs = a.m.doc_k != nullptr;
+    if (docs) doc = doc_span(id, (FA3_LDS int*)(smem + C::kRangeOff), w, lane);
+
+    int begin = 0;
+    if (wg_key >= prefix && wg_key - off > 0) begin = (wg_key - off) >> 6;
+    TileWalk walk(docs ? a.m.range_q + (int64_t)b * a.m.blocks_q : nullptr, begin,
+                  wg_key < kv ? a.sqp / 64 : begin, doc);
+    int t = walk.next(), g = 0;  // the step being computed: query tile and head of the group
+    int ld_t = t, ld_g = 0;      // the step being loaded
+    auto issue = [&](FA3_LDS char* st) {
+        const int ln = opaque_tid() & 63, i0 = ld_t * 64, h = hkv * attn_args<Args>().group + ld_g;
+        int64_t row;  // of the statistics
+        bool whole;
+        {
+            const auto& a = attn_args<Args>();
+            row = ((int64_t)b * a.heads_q + h) * a.sqp + i0;
+            whole = a.d == D && a.flags[row >> 6] == 0;
+        }
+        auto load = [&](FA3_LDS char* tile, const auto& x) {
+            const _Float16* p = x.p + b * x.bs + h * x.hs;
+            if (whole) {
+                attn_load_tile<D>(tile, p, x.rs, i0, w, ln);
+            } else {
+                const auto& a = attn_args<Args>();
+                const float* nl = a.nlse2 + (row - i0);
+                attn_load_tile_edge<D>(tile, p, x.rs, i0, a.sq, a.d, w, ln,
+                                       [&](int i) { return nl[i] != kNegInf; });
+            }
+        };
+        load(st, attn_args<Args>().q);
+        wall();
+        load(st + R::kTileBytes, attn_args<Args>().dout);
+        wall();
+        const auto& a = attn_args<Args>();
+        if (w < 2)
+            __builtin_amdgcn_global_load_lds((const void*)((w == 0 ? a.nlse2 : a.ndelta) + row + ln),
+                                             (FA3_LDS void*)(st + 2 * R::kTileBytes + 256 * w), 4, 0, 0);
+    };
+    f32x4 av[C::kDB][2], ak[C::kDB][2];
+#pragma unroll
+    for (int i = 0; i < C::kDB; ++i) {
+        av[i][0] = av[i][1] = f32x4{};
+        ak[i][0] = ak[i][1] = f32x4{};
+    }
+    const RegReader<D> rd0(lane, 0);
+    const float c = a.m.c;
+
+    auto sub = [&](const FA3_LDS char* st, int r, bool same) {
+        const int i0 = t * 64 + 32 * r;
+        // rows i0 .. i0 + 31 against keys key0 .. key0 + 31
+        if (key0 >= kv || (key0 >= prefix && key0 > i0 + 31 + off)) return;
+        const bool full = key0 + 32 <= kv && same &&
+                          (key0 + 31 <= i0 + off || prefix - 32 >= key0);
+        uint32_t vis = 0xffff;
+        if (!full) {
+            const int l = opaque_tid() & 63;
+            vis = 0;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int j = key0 + 16 * n + (l & 15);
+                // rows (m, e) with 16 m + e >= first see key j
+                const int first = j >= kv ? 64
+                                  : j < prefix ? -64
+                                               : j - off - i0 - 4 * (l >> 4);
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+                    vis |= 16 * (x >> 2) + (x & 3) >= first ? 1u << (8 * n + x) : 0u;
+            }
+            if (walk.ranges != nullptr) {
+                const auto& a = attn_args<Args>();
+                const int* ids = a.m.doc_q + b * a.m.doc_q_bs;
+                uint32_t met = 0;
+                int id[2];  // (read again: not worth two registers over the loop)
+#pragma unroll
+                for (int n = 0; n < 2; ++n)
+                    id[n] = max(a.m.doc_k[b * a.m.doc_k_bs + min(key0 + 16 * n + (l & 15), a.sk - 1)], -1);
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    const int rid =
+                        doc_of(ids[min(i0 + 4 * (l >> 4) + 16 * (x >> 2) + (x & 3), a.sq - 1)]);
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+                        met |= rid == id[n] ? 1u << (8 * n + x) : 0u;
+                }
+                vis &= met;
+            }
+        }
+        RegReader<D> rd = rd0;
+        rd.opaque();
+        const FA3_LDS f32x4* rows = (const FA3_LDS f32x4*)(st + 2 * R::kTileBytes + 128 * r) +
+                                    ((opaque_tid() & 63) >> 4);
+        f32x4 s[2][2], dp[2][2], nl[2];  // [m][n]: rows 16 m + 4 g4 + e, keys 16 n + l16
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            dp[m][0] = dp[m][1] = rows[16 + 4 * m];
+            s[m][0] = s[m][1] = f32x4{};
+        }
+        reg_scores<D, kBf16, AttnAhead<D, kCap>>(rd, st, st + R::kTileBytes, r, kf, vf, s, dp);
+        nl[0] = rows[0];
+        nl[1] = rows[4];
+        float k1 = 0.f, cap2 = 0.f, slope = 0.f;
+        if constexpr (kCap) {
+            const auto& a = attn_args<Args>();
+            k1 = a.m.k1;
+            cap2 = a.m.cap2;
+        }
+        if constexpr (kBias) {
+            const auto& a = attn_args<Args>();
+            slope = a.m.slopes[b * a.m.slopes_bs + hkv * a.group + g] * kLog2e;
+        }
+        float p[2][8], ds[2][8];  // [n][4 m + e]
+        const int ln = opaque_tid() & 63;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            // distance of row (m, e): d0 + 16 m + e
+            wall();
+            const float d0 = kBias ? (float)(i0 + off + 4 * (ln >> 4) - key0 - 16 * n - (ln & 15)) : 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int m = j >> 2, e = j & 3;
+                attn_pds<kCap, kBias>(s[m][n][e], dp[m][n][e], nl[m][e], c, k1, cap2, kFine, slope,
+                                      d0 + (float)(16 * m + e), bit_mask(vis, 8 * n + j), p[n][j],
+                                      ds[n][j]);
+            }
+        }
+        const f16x8 bp[2] = {pack8<kBf16>(p[0]), pack8<kBf16>(p[1])};
+        const f16x8 bs[2] = {pack8<kBf16>(ds[0]), pack8<kBf16>(ds[1])};
+        reg_grads<D, kBf16, true, AttnAhead<D, kCap>>(rd, st + R::kTileBytes, st, r, bp, bs, av, ak);
+    };
+    FA3_LDS char* s0 = smem;
+    FA3_LDS char* s1 = smem + R::kStageBytes;
+    int cls = walk.cls;  // of the tile being computed
+    auto advance = [&]() {
+        if (++ld_g == attn_args<Args>().group) {
+            ld_g = 0;
+            ld_t = walk.next();
+        }
+    };
+    if (t >= 0) issue(s0);
+    auto stage = [&](FA3_LDS char* __restrict__ ld, const FA3_LDS char* __restrict__ st) {
+        wait_vm_lgkm0<0>();
+        barrier();
+        advance();
+        if (ld_t >= 0) issue(ld);
+        if (cls & kTileMeets) {
+            sub(st, 0, cls & kTileSame);
+            sub(st, 1, cls & kTileSame);
+        }
+        t = ld_t;
+        g = ld_g;
+        cls = walk.cls;
+    };
+    while (t >= 0) {
+        stage(s1, s0);
+        if (t < 0) break;
+        stage(s0, s1);
+    }
+    wait_vm_lgkm0<0>();
+    barrier();  // every wave is done with the stages: they take the outputs
+    const auto& z = attn_args<Args>();
+    const BwdJob e = bwd_job(z, blockIdx.x);  // (decoded again: not held over the loop)
+    const int ew = __builtin_amdgcn_readfirstlane(opaque_tid() >> 6);
+    const int ekey = e.level * kAttnRows + 32 * ew;
+    FA3_LDS char* stg = smem + ew * C::kDB * 1024;
+    const float one[2] = {1.f, 1.f}, sc[2] = {z.scale, z.scale};
+    auto store = [&](const f32x4 (&acc)[C::kDB][2], const auto& x, const float (&mul)[2]) {
+        attn_store<D, kBf16>(acc, mul, z.d, stg, [&](int r) -> _Float16* {
+            return ekey + r < z.sk ? x.p + e.b * x.bs + e.hkv * x.hs + (ekey + r) * x.rs : nullptr;
+        });
+    };
+    store(av, z.dv, one);
+    store(ak, z.dk, sc);
+}
+
+template <int D, bool kBf16, bool kCap, bool kBias, bool kFine>
+__device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* smem) {
+    typedef AttnBwdArgs Args;
+    using C = BwdCfg<D>;
+    using R = RegCfg<D>;
+    const auto& a = attn_args<Args>();
+    const int lane = opaque_tid() & 63;
+    const int w = __builtin_amdgcn_readfirstlane(opaque_tid() >> 6);
+    const int l16 = lane & 15, g4 = lane >> 4;
+    const int kv = attn_kv(a.m, b, a.sk), prefix = attn_prefix(a.m, b), off = kv - a.sq;
+    const bool causal = a.m.causal;
+    const int row0 = tile * kAttnRows + 32 * w;
+    const bool any = row0 < a.rows;
+    const int last = min(row0 + 32, a.rows) - 1, wg_last = min((tile + 1) * kAttnRows, a.rows) - 1;
+    const int lim_min = any ? attn_limit(fdiv(a.div_group, row0), off, kv, causal, prefix) : 0x7fffffff;
+    const int lim_max = any ? attn_limit(fdiv(a.div_group, last), off, kv, causal, prefix) : 0;
+    const int wg_max = attn_limit(fdiv(a.div_group, wg_last), off, kv, causal, prefix);
+
+    f16x8 qf[2][C::kKs], df[2][C::kKs];
+    float nl[2], qp[2], slope[2];
+    f32x4 nd[2];
+    int lim[2], id[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const AttnRow r = attn_row(row0 + 16 * n + l16, a.rows, hkv, a.group, a.div_group);
+        const int64_t at = ((int64_t)b * a.heads_q + r.h) * a.sqp + r.i;
+        nl[n] = r.ok ? a.nlse2[at] : kNegInf;
+        const float x = r.ok ? a.ndelta[at] : 0.f;
+        nd[n] = f32x4{x, x, x, x};
+        const bool ok = nl[n] != kNegInf;
+        const _Float16* q = a.q.p + b * a.q.bs + r.h * a.q.hs + r.i * a.q.rs;
+        const _Float16* o = a.dout.p + b * a.dout.bs + r.h * a.dout.hs + r.i * a.dout.rs;
+#pragma unroll
+        for (int s = 0; s < C::kKs; ++s) {
+            qf[n][s] = attn_row8(q, p1_chunk<D>(s, g4), a.d, ok);
+            df[n][s] = attn_row8(o, p1_chunk<D>(s, g4), a.d, ok);
+        }
+        lim[n] = r.ok ? attn_limit(r.i, off, kv, causal, prefix) : 0;
+        id[n] = -2;
+        if (a.m.doc_q != nullptr && r.ok) id[n] = max(a.m.doc_q[b * a.m.doc_q_bs + r.i], -1);
+        qp[n] = 0.f;
+        slope[n] = 0.f;
+        if constexpr (kBias) {
+            qp[n] = (float)(r.i + off);
+            slope[n] = a.m.slopes[b * a.m.slopes_bs + r.h] * kLog2e;
+        }
+    }
+    DocSpan doc{0, 0, 0, 0, false};
+    if (a.m.doc_q != nullptr) doc = doc_span(id, (FA3_LDS int*)(smem + C::kRangeOff), w, lane);
+
+    const _Float16* kp = a.k.p + b * a.k.bs + hkv * a.k.hs;
+    const _Float16* vp = a.v.p + b * a.v.bs + hkv * a.v.hs;
+    const int* ids = a.m.doc_k == nullptr ? nullptr : a.m.doc_k + b * a.m.doc_k_bs;
+    TileWalk walk(ids == nullptr ? nullptr : a.m.range_k + (int64_t)b * a.m.blocks_k, 0,
+                  (wg_max + 63) >> 6, doc);
+    auto issue = [&](FA3_LDS char* st, int t) {
+        const int j0 = t * 64, ln = opaque_tid() & 63;
+        const auto& a = attn_args<Args>();
+        if (j0 + 64 <= kv && a.d == D && !(walk.cls & kTileHidden)) {
+            attn_load_tile<D>(st, kp, a.k.rs, j0, w, ln);
+            attn_load_tile<D>(st + R::kTileBytes, vp, a.v.rs, j0, w, ln);
+        } else {
+            auto seen = [&](int j) { return ids == nullptr || ids[j] >= 0; };
+            attn_load_tile_edge<D>(st, kp, a.k.rs, j0, kv, a.d, w, ln, seen);
+            attn_load_tile_edge<D>(st + R::kTileBytes, vp, a.v.rs, j0, kv, a.d, w, ln, seen);
+        }
+    };
+    f32x4 acc[C::kDB][2];
+#pragma unroll
+    for (int i = 0; i < C::kDB; ++i) acc[i][0] = acc[i][1] = f32x4{};
+    const RegReader<D> rd0(lane, 0);
+    const float c = a.m.c;
+
+    auto sub = [&](const FA3_LDS char* st, int t, int r, bool same) {
+        const int j0 = t * 64 + 32 * r;
+        if (j0 >= lim_max) return;
+        const bool full = j0 + 32 <= lim_min && same;
+        uint32_t vis = 0xffff;
+        if (!full) {
+            const int jl = j0 + 4 * ((opaque_tid() & 63) >> 4);
+            vis = 0;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int k = lim[n] - jl;
+#pragma unroll
+                for (int x = 0; x < 8; ++x)
+                    vis |= 16 * (x >> 2) + (x & 3) < k ? 1u << (8 * n + x) : 0u;
+            }
+            if (ids != nullptr) {
+                const int sk = attn_args<Args>().sk;
+                uint32_t met = 0;
+#pragma unroll
+                for (int x = 0; x < 8; ++x) {
+                    const int kid = doc_of(ids[min(jl + 16 * (x >> 2) + (x & 3), sk - 1)]);
+#pragma unroll
+                    for (int n = 0; n < 2; ++n)
+                        met |= kid == id[n] ? 1u << (8 * n + x) : 0u;
+                }
+                vis &= met;
+            }
+        }
+        RegReader<D> rd = rd0;
+        rd.opaque();
+        f32x4 s[2][2], dp[2][2];  // [m][n]: keys 16 m + 4 g4 + e, rows 16 n + l16
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                s[m][n] = f32x4{};
+                dp[m][n] = nd[n];
+            }
+        reg_scores<D, kBf16, AttnAhead<D, kCap>>(rd, st, st + R::kTileBytes, r, qf, df, s, dp);
+        float k1 = 0.f, cap2 = 0.f;
+        if constexpr (kCap) {
+            const auto& a = attn_args<Args>();
+            k1 = a.m.k1;
+            cap2 = a.m.cap2;
+        }
+        float ds[2][8];
+        const int ln = opaque_tid() & 63;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const float d0 = kBias ? qp[n] - (float)(j0 + 4 * (ln >> 4)) : 0.f;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int m = j >> 2, e = j & 3;
+                float p;
+                attn_pds<kCap, kBias>(s[m][n][e], dp[m][n][e], nl[n], c, k1, cap2, kFine, slope[n],
+                                      d0 - (float)(16 * m + e), bit_mask(vis, 8 * n + j), p, ds[n][j]);
+            }
+        }
+        const f16x8 bs[2] = {pack8<kBf16>(ds[0]), pack8<kBf16>(ds[1])};
+        reg_grads<D, kBf16, false, AttnAhead<D, kCap>>(rd, st, st, r, bs, bs, acc, acc);
+    };
+    FA3_LDS char* s0 = smem;
+    FA3_LDS char* s1 = smem + R::kStageBytes;
+    int t = walk.next();
+    if (t >= 0) issue(s0, t);
+    auto stage = [&](FA3_LDS char* __restrict__ ld, const FA3_LDS char* __restrict__ st) {
+        const int cls = walk.cls;
+        wait_vm_lgkm0<0>();
+        barrier();
+        const int tn = walk.next();
+        if (tn >= 0) issue(ld, tn);
+        if (cls & kTileMeets) {
+            sub(st, t, 0, cls & kTileSame);
+            sub(st, t, 1, cls & kTileSame);
+        }
+        t = tn;
+    };
+    while (t >= 0) {
+        stage(s1, s0);
+        if (t < 0) break;
+        stage(s0, s1);
+    }
+    wait_vm_lgkm0<0>();
+    barrier();
+    const auto& z = attn_args<Args>();
+    const BwdJob e = bwd_job(z, blockIdx.x);
+    const int ew = __builtin_amdgcn_readfirstlane(opaque_tid() >> 6);
+    const int erow = (z.kv_tiles + z.q_tiles - 1 - e.level) * kAttnRows + 32 * ew;
+    const float sc[2] = {z.scale, z.scale};
+    attn_store<D, kBf16>(acc, sc, z.d, smem + ew * C::kDB * 1024, [&](int r) -> _Float16* {
+        const AttnRow x = attn_row(erow + r, z.rows, e.hkv, z.group, z.div_group);
+        return x.ok ? z.dq.p + e.b * z.dq.bs + x.h * z.dq.hs + x.i * z.dq.rs : nullptr;
+    });
+}
+
+// kCap: 0 none, 1 capped, 2 capped with tanh's series for small scores
+template <int D, bool kBf16, int kCap, bool kBias>
+__global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_bwd_kernel(AttnBwdArgs) {
+    __shared__ __attribute__((aligned(1024))) char smem_raw[BwdCfg<D>::kBytes];
+    FA3_LDS char* smem = (FA3_LDS char*)smem_raw;
+    const auto& a = attn_args<AttnBwdArgs>();
+    const BwdJob j = bwd_job(a, blockIdx.x);
+    if (j.level < a.kv_tiles)
+        attn_dkv<D, kBf16, kCap != 0, kBias, kCap == 2>(j.b, j.hkv, j.level, smem);
+    else
+        attn_dq<D, kBf16, kCap != 0, kBias, kCap == 2>(j.b, j.hkv, a.kv_tiles + a.q_tiles - 1 - j.level, smem);
+}
+
+AttnView view(const ShaoboFa3AttnTensor& t) {
+    return AttnView{(_Float16*)t.data, t.batch_stride, t.head_stride, t.row_stride};
+}
+
+}  // namespace
+
+AttnBwdPlan plan_attn_bwd(const AttnProblem& p) {
+    AttnBwdPlan f{};
+    const int64_t rows = (int64_t)p.group * p.sq, groups = (int64_t)p.batch * p.heads_kv;
+    f.kv_tiles = ceil_div(p.sk, kAttnRows);
+    f.q_tiles = ceil_div(rows, kAttnRows);
+    f.sqp = ceil_div(p.sq, 64) * 64;
+    const int64_t jobs = groups * ((int64_t)f.kv_tiles + f.q_tiles);
+    const int64_t blocks = groups * p.group * (f.sqp / 64);
+    size_t at = 0;
+    auto take = [&](size_t n) {
+        const size_t x = at;
+        at += (n + 255) / 256 * 256;
+        return x;
+    };
+    f.nlse2_off = take((size_t)blocks * 64 * 4);
+    f.ndelta_off = take((size_t)blocks * 64 * 4);
+    f.flag_off = take((size_t)blocks * 4);
+    f.range_k_off = take(p.docs ? (size_t)p.batch * ceil_div(p.sk, 64) * sizeof(AttnRange) : 0);
+    f.range_q_off = take(p.docs ? (size_t)p.batch * (f.sqp / 64) * sizeof(AttnRange) : 0);
+    f.total = at;
+    f.ok = rows < (1ll << 30) && jobs < (1ll << 30) && blocks < (1ll << 30);
+    f.jobs = f.ok ? (int)jobs : 0;
+    return f;
+}
+
+hipError_t launch_attn_bwd(const AttnProblem& p, const ShaoboFa3AttnParams& a, AttnMask m,
+                           hipStream_t stream) {
+    const AttnBwdPlan f = plan_attn_bwd(p);
+    if (f.jobs == 0) return hipSuccess;
+    char* ws = (char*)a.workspace;
+    AttnBwdArgs x{};
+    x.q = view(a.q);
+    x.k = view(a.k);
+    x.v = view(a.v);
+    x.out = view(a.out);
+    x.dout = view(a.dout);
+    x.dq = view(a.dq);
+    x.dk = view(a.dk);
+    x.dv = view(a.dv);
+    x.lse = a.softmax_lse;
+    x.softmax_d = a.softmax_d;
+    x.nlse2 = (float*)(ws + f.nlse2_off);
+    x.ndelta = (float*)(ws + f.ndelta_off);
+    x.flags = (int*)(ws + f.flag_off);
+    x.scale = p.scale;
+    x.heads_q = p.heads_q;
+    x.heads_kv = p.heads_kv;
+    x.group = p.group;
+    x.sq = p.sq;
+    x.sk = p.sk;
+    x.d = p.d;
+    x.sqp = f.sqp;
+    x.rows = p.group * p.sq;
+    x.kv_tiles = f.kv_tiles;
+    x.q_tiles = f.q_tiles;
+    x.groups = p.batch * p.heads_kv;
+    x.div_hkv = make_fastdiv(p.heads_kv);
+    x.div_group = make_fastdiv(p.group);
+    x.div_groups = make_fastdiv(x.groups);
+    x.div_gpart = make_fastdiv(x.groups / 8);
+    x.div_hq = make_fastdiv(p.heads_q);
+    x.div_blocks = make_fastdiv(f.sqp / 64);
+    if (p.docs) {
+        AttnRange* rk = (AttnRange*)(ws + f.range_k_off);
+        AttnRange* rq = (AttnRange*)(ws + f.range_q_off);
+        hipError_t e = launch_attn_ranges(m.doc_k, m.doc_k_bs, p.batch, p.sk, rk, stream);
+        if (e == hipSuccess) e = launch_attn_ranges(m.doc_q, m.doc_q_bs, p.batch, p.sq, rq, stream);
+        if (e != hipSuccess) return e;
+        m.range_k = rk;
+        m.range_q = rq;
+        m.blocks_k = ceil_div(p.sk, 64);
+        m.blocks_q = f.sqp / 64;
+    }
+    x.m = m;
+    const int cap = p.softcap > 0.f ? m.cap_fine ? 2 : 1 : 0;
+    const int blocks = x.groups * p.group * (f.sqp / 64);
+    auto pick = [&](auto d, auto bf) {
+        constexpr int kD = decltype(d)::value;
+        constexpr bool kB = decltype(bf)::value;
+        if (blocks > 0)
+            hipLaunchKernelGGL((attn_delta_kernel<kD, kB>), dim3(blocks), dim3(256), 0, stream, x);
+        auto go = [&](auto kernel) {
+            hipLaunchKernelGGL(kernel, dim3(f.jobs), dim3(kRegThreads), 0, stream, x);
+        };
+        auto caps = [&](auto bias) {
+            constexpr bool kBi = decltype(bias)::value;
+            if (cap == 2) go(attn_bwd_kernel<kD, kB, 2, kBi>);
+            else if (cap == 1) go(attn_bwd_kernel<kD, kB, 1, kBi>);
+            else go(attn_bwd_kernel<kD, kB, 0, kBi>);
+        };
+        p.bias ? caps(std::true_type{}) : caps(std::false_type{});
+    };
+    using T = std::true_type;
+    using F = std::false_type;
+    if (p.d > 64) p.bf16 ? pick(std::integral_constant<int, 128>{}, T{}) : pick(std::integral_constant<int, 128>{}, F{});
+    else p.bf16 ? pick(std::integral_constant<int, 64>{}, T{}) : pick(std::integral_constant<int, 64>{}, F{});
+    return hipGetLastError();
+}
+
+}  // namespace fa3

@@ -1,0 +1,88 @@
+// Host-side interface between the attention layer's C entries
+// (fa3_attn_api.cpp) and its kernels.  Nothing here is exported.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stddef.h>
+#include <stdint.h>
+
+#include "fa3_bwd_internal.h"
+#include "shaobo_fa3_attn.h"
+
+namespace fa3 {
+
+// One [batch, heads, rows, head_dim] 16-bit tensor; strides in elements.
+struct AttnView {
+    _Float16* p;
+    int64_t bs, hs, rs;
+};
+
+// Smallest and largest document of 64 consecutive positions, those with a
+// negative one left out: {INT32_MAX, -1} where that leaves none.  Where any
+// was left out (or the block ends behind the sequence) lo is complemented.
+struct AttnRange {
+    int lo, hi;
+};
+
+// Masks and score options as the kernels take them (pointers null: absent).
+struct AttnMask {
+    const int* doc_q;
+    const int* doc_k;
+    int64_t doc_q_bs, doc_k_bs;
+    const AttnRange* range_q;  // [batch][blocks_q], backward only
+    const AttnRange* range_k;  // [batch][blocks_k]
+    int blocks_q, blocks_k;
+    const int* prefix;
+    const int* kv_lens;
+    const float* slopes;
+    int64_t slopes_bs;
+    int causal;
+    // x = log2-domain score: s c, or with a cap cap2 tanh(s / softcap) from
+    // e = exp2(s k1) (see attn_cap)
+    float c, k1, cap2;
+    int cap_fine;  // caps large enough that small scores need tanh's series
+};
+
+// A resolved problem: checked, default scale applied.
+struct AttnProblem {
+    int batch, heads_q, heads_kv, group, sq, sk, d;
+    bool bf16;
+    float scale, softcap;
+    bool bias, docs;
+};
+
+constexpr int kAttnTile = 64;   // keys (or rows) streamed per step
+constexpr int kAttnRows = 128;  // rows (or keys) resident per workgroup
+
+inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+struct AttnFwdPlan {
+    int tiles;   // 128-row tiles of a KV head's group * sq rows
+    int splits;  // parts of the key axis
+    int part;    // 64-key tiles per part
+    int jobs;
+    size_t range_off, po_off, pl_off, total;
+    bool ok;
+};
+AttnFwdPlan plan_attn_fwd(const AttnProblem& p);
+
+struct AttnBwdPlan {
+    int kv_tiles;  // 128-key tiles
+    int q_tiles;   // 128-row tiles of a KV head's group * sq rows
+    int sqp;       // rows of the statistics, padded to whole 64-row blocks
+    int jobs;
+    size_t nlse2_off, ndelta_off, flag_off, range_k_off, range_q_off, total;
+    bool ok;
+};
+AttnBwdPlan plan_attn_bwd(const AttnProblem& p);
+
+hipError_t launch_attn_fwd(const AttnProblem& p, const ShaoboFa3AttnParams& a, AttnMask m,
+                           hipStream_t stream);
+hipError_t launch_attn_bwd(const AttnProblem& p, const ShaoboFa3AttnParams& a, AttnMask m,
+                           hipStream_t stream);
+// AttnRange of every 64-position block of ids [batch][n].
+hipError_t launch_attn_ranges(const int* ids, int64_t bs, int batch, int n, AttnRange* out,
+                              hipStream_t stream);
+hipError_t launch_rotary(const ShaoboFa3RotaryParams& p, hipStream_t stream);
+
+}  // namespace fa3

@@ -198,7 +198,7 @@ __device__ __forceinline__ void reg_load_tile(FA3_LDS char* tile, const _Float16
 
 // s0[m][n] += X0 B0, s1[m][n] += X1 B1 over D, for the 32 streamed rows 32 r
 // .. (blocks m) and the 32 resident columns (blocks n).
-template <int D, bool kBf16>
+template <int D, bool kBf16, typename C = RegCfg<D>>
 __device__ __forceinline__ void reg_scores(const RegReader<D>& rd, const FA3_LDS char* x0,
                                            const FA3_LDS char* x1, int r,
                                            const f16x8 (&b0)[2][D / 32],
@@ -206,7 +206,6 @@ __device__ __forceinline__ void reg_scores(const RegReader<D>& rd, const FA3_LDS
                                            f32x4 (&s1)[2][2]) {
     constexpr int kKs = D / 32, kN = 4 * kKs;
     f16x8 f[kN];
-    using C = RegCfg<D>;
     // Operand i: tile, row block m and k-step.  D 64 takes both row blocks of
     // a k-step in turn and the resident blocks n forth and back, so that
     // consecutive products differ in one operand only (less switching in the
@@ -241,7 +240,7 @@ __device__ __forceinline__ void reg_scores(const RegReader<D>& rd, const FA3_LDS
 
 // g0[db][n] += X0^T B0 (and g1[db][n] += X1^T B1 when kTwo) over the 32
 // streamed rows 32 r ..
-template <int D, bool kBf16, bool kTwo>
+template <int D, bool kBf16, bool kTwo, typename C = RegCfg<D>>
 __device__ __forceinline__ void reg_grads(const RegReader<D>& rd, const FA3_LDS char* x0,
                                           const FA3_LDS char* x1, int r, const f16x8 (&b0)[2],
                                           const f16x8 (&b1)[2], f32x4 (&g0)[D / 16][2],
@@ -255,7 +254,7 @@ __device__ __forceinline__ void reg_grads(const RegReader<D>& rd, const FA3_LDS 
     auto second = [](int i) { return kTwo && (i & 2); };
     auto db_of = [](int i) { return kTwo ? ((i >> 2) << 1) | (i & 1) : i; };
     auto read = [&](int i) { f[i] = rd.tr(second(i) ? x1 : x0, r, db_of(i)); };
-    constexpr int kA = RegCfg<D>::kAheadG;
+    constexpr int kA = C::kAheadG;
 #pragma unroll
     for (int i = 0; i < 2; ++i) read(i);
     wall();

@@ -19,6 +19,8 @@ STATUS = {0: "success", 1: "invalid_value", 2: "unsupported", 3: "not_implemente
           4: "hip_error"}
 SUCCESS, INVALID_VALUE, UNSUPPORTED, NOT_IMPLEMENTED, HIP_ERROR = range(5)
 DTYPE_FP16, DTYPE_BF16, DTYPE_FP8 = range(3)
+DTYPE_FP32 = 3  # (shaobo_fa3_rotary only)
+POSITIONS_INT32, POSITIONS_INT64, POSITIONS_FP32 = range(3)
 LAYOUT_BHSD, LAYOUT_BSHD = range(2)
 AUX_SMAX_SSUM, AUX_LSE = range(2)
 
@@ -37,6 +39,10 @@ EXPORTS = (
     "shaobo_fa3_ext_bwd_v2_no_alloc", "shaobo_fa3_ext_bwd_v2_timed",
     "shaobo_fa3_ext_bwd_v2_stages", "shaobo_fa3_ext_split_status",
     "shaobo_fa3_ext_split_error_count", "shaobo_fa3_ext_bwd_v2_plan",
+    "shaobo_fa3_attn_params_init", "shaobo_fa3_attn_fwd_validate",
+    "shaobo_fa3_attn_bwd_validate", "shaobo_fa3_attn_fwd_workspace_bytes",
+    "shaobo_fa3_attn_bwd_workspace_bytes", "shaobo_fa3_attn_fwd", "shaobo_fa3_attn_bwd",
+    "shaobo_fa3_rotary_params_init", "shaobo_fa3_rotary",
 )
 
 # Size of the static device scratch array behind shaobo_fa3_ext_bwd_v2_no_alloc
@@ -113,6 +119,55 @@ class Plan(ctypes.Structure):
                                       "split_kv", "halved", "split_q", "xcd_parts")]
 
 
+class AttnTensor(ctypes.Structure):
+    """ShaoboFa3AttnTensor (include/shaobo_fa3_attn.h)."""
+    _fields_ = [("data", ctypes.c_void_p), ("batch_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64)]
+
+
+class AttnParams(ctypes.Structure):
+    """ShaoboFa3AttnParams (include/shaobo_fa3_attn.h)."""
+    _fields_ = [("struct_size", ctypes.c_uint32)] + [
+        (n, ctypes.c_int32) for n in ("batch", "seqlen_q", "seqlen_k", "num_heads_q",
+                                      "num_heads_kv", "head_dim", "dtype", "causal",
+                                      "softmax_scale_is_set")] + [
+        ("softmax_scale", ctypes.c_float), ("softcap", ctypes.c_float)] + [
+        (n, AttnTensor) for n in ("q", "k", "v", "out", "dout", "dq", "dk", "dv")] + [
+        ("softmax_lse", ctypes.c_void_p), ("softmax_d", ctypes.c_void_p),
+        ("slopes", ctypes.c_void_p), ("slopes_batch_stride", ctypes.c_int64),
+        ("documents_q", ctypes.c_void_p), ("documents_k", ctypes.c_void_p),
+        ("documents_q_batch_stride", ctypes.c_int64),
+        ("documents_k_batch_stride", ctypes.c_int64),
+        ("prefix_lens", ctypes.c_void_p), ("kv_lens", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class RotaryParams(ctypes.Structure):
+    """ShaoboFa3RotaryParams (include/shaobo_fa3_attn.h)."""
+    _fields_ = [("struct_size", ctypes.c_uint32)] + [
+        (n, ctypes.c_int32) for n in ("batch", "seqlen", "head_dim", "dtype", "axes", "pairs",
+                                      "interleaved", "inverse", "position_type")] + [
+        ("positions", ctypes.c_void_p), ("position_axis_stride", ctypes.c_int64),
+        ("position_batch_stride", ctypes.c_int64), ("position_row_stride", ctypes.c_int64),
+        ("freqs", ctypes.c_void_p), ("tensors", ctypes.c_int32), ("heads", ctypes.c_int32 * 2),
+        ("in_", AttnTensor * 2), ("out", AttnTensor * 2)]
+
+
+def _declare_attn(lib):
+    A, R = ctypes.POINTER(AttnParams), ctypes.POINTER(RotaryParams)
+    for name, args, res in (
+            ("attn_params_init", [A], None), ("attn_fwd_validate", [A], ctypes.c_int),
+            ("attn_bwd_validate", [A], ctypes.c_int),
+            ("attn_fwd_workspace_bytes", [A], ctypes.c_size_t),
+            ("attn_bwd_workspace_bytes", [A], ctypes.c_size_t),
+            ("attn_fwd", [A, ctypes.c_void_p], ctypes.c_int),
+            ("attn_bwd", [A, ctypes.c_void_p], ctypes.c_int),
+            ("rotary_params_init", [R], None),
+            ("rotary", [R, ctypes.c_void_p], ctypes.c_int)):
+        fn = getattr(lib, "shaobo_fa3_" + name)
+        fn.argtypes, fn.restype = args, res
+
+
 def _declare(lib):
     P = ctypes.POINTER(Params)
     vp = ctypes.c_void_p
@@ -178,6 +233,7 @@ def load(path=LIB_PATH):
         lib.shaobo_fa3_ext_split_error_count.restype = ctypes.c_int
         lib.shaobo_fa3_ext_bwd_v2_plan.argtypes = [ctypes.POINTER(Params), ctypes.POINTER(Plan)]
         lib.shaobo_fa3_ext_bwd_v2_plan.restype = ctypes.c_int
+        _declare_attn(lib)
         if path != LIB_PATH:
             return lib
         _LIB = lib

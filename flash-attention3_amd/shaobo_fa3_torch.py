@@ -203,3 +203,169 @@ def attention(q, k, v, causal=True, softmax_scale=None):
     """softmax(scale Q K^T) V with the MI355X FA3 backward (fp16 / bf16 BHSD)."""
     scale = 1.0 / math.sqrt(q.shape[-1]) if softmax_scale is None else softmax_scale
     return _Attention.apply(q, k, v, causal, scale)
+
+
+# ---------------------------------------------------------------------------
+# The attention layer: rotary positions, and attention with capped, biased and
+# masked scores (include/shaobo_fa3_attn.h says what they compute).
+#
+#   torch.ops.shaobo_fa3.rotary(xs, positions, freqs, interleaved, inverse) -> xs
+#   torch.ops.shaobo_fa3.attn_forward(q, k, v, causal, softmax_scale, softcap, slopes,
+#       documents, documents_k, prefix_lens, kv_lens) -> out, lse
+#   torch.ops.shaobo_fa3.attn_backward(dout, q, k, v, out, lse, causal, ...)
+#       -> dq, dk, dv, softmax_d
+#
+# The three are registered by lib/_fa3_torch_attn.so (csrc/fa3_torch_attn.cpp);
+# `rotary` and `score_attention` below add their gradients.
+_ATTN_PATH = os.path.join(os.path.dirname(F.LIB_PATH), "_fa3_torch_attn.so")
+
+
+def _load_attn():
+    """Registers the attention layer's operators; False, with a warning, where
+    their library does not load.  There is no other body: without it the
+    operators do not exist."""
+    if not os.path.exists(_ATTN_PATH):
+        return False
+    try:
+        torch.ops.load_library(_ATTN_PATH)
+    except OSError as e:
+        warnings.warn(f"{_ATTN_PATH} does not load, the attention layer's operators are missing: "
+                      f"{e}", RuntimeWarning, stacklevel=2)
+        return False
+    return True
+
+
+_ATTN = _load_attn()
+
+
+def _need_attn():
+    if not _ATTN:
+        raise RuntimeError(f"the attention layer's operators need {_ATTN_PATH}: "
+                           "make -C flash-attention3_amd torch")
+
+
+if _ATTN:
+    @torch.library.register_fake("shaobo_fa3::attn_forward")
+    def _(q, k, v, causal, softmax_scale=None, softcap=0.0, slopes=None, documents=None,
+          documents_k=None, prefix_lens=None, kv_lens=None):
+        return torch.empty_like(q), q.new_empty(q.shape[:3], dtype=torch.float32)
+
+    @torch.library.register_fake("shaobo_fa3::attn_backward")
+    def _(dout, q, k, v, out, softmax_lse, causal, softmax_scale=None, softcap=0.0, slopes=None,
+          documents=None, documents_k=None, prefix_lens=None, kv_lens=None):
+        return (torch.empty_like(q), torch.empty_like(k), torch.empty_like(v),
+                torch.empty_like(softmax_lse))
+
+    @torch.library.register_fake("shaobo_fa3::rotary")
+    def _(xs, positions, freqs, interleaved=False, inverse=False):
+        return [torch.empty_like(x) for x in xs]
+
+
+def _in_rows(t):
+    """t itself where the operators take its memory as it is, else a copy:
+    gradients arrive in any layout (expanded, transposed, sliced)."""
+    align = 16 // t.element_size()
+    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and \
+            all(s % align == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1):
+        return t
+    return t.contiguous()
+
+
+class _ScoreAttention(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, causal, scale, softcap, slopes, documents, documents_k, prefix_lens,
+                kv_lens):
+        out, lse = torch.ops.shaobo_fa3.attn_forward(q, k, v, causal, scale, softcap, slopes,
+                                                     documents, documents_k, prefix_lens, kv_lens)
+        ctx.save_for_backward(q, k, v, out, lse, slopes, documents, documents_k, prefix_lens,
+                              kv_lens)
+        ctx.options = causal, scale, softcap
+        ctx.mark_non_differentiable(lse)
+        ctx.set_materialize_grads(False)
+        return out, lse
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dout, _):
+        if dout is None:
+            return (None,) * 11
+        q, k, v, out, lse, *mask = ctx.saved_tensors
+        dq, dk, dv, _ = torch.ops.shaobo_fa3.attn_backward(_in_rows(dout), q, k, v, out, lse,
+                                                           *ctx.options, *mask)
+        return (dq, dk, dv) + (None,) * 8
+
+
+def score_attention(q, k, v, *, causal=True, softmax_scale=None, softcap=0.0, slopes=None,
+                    documents=None, documents_k=None, prefix_lens=None, kv_lens=None,
+                    return_lse=False):
+    """Softmax attention whose scores may be capped, biased and masked, with
+    its gradient in q, k and v.
+
+    q [B, Hq, Sq, D], k and v [B, Hkv, Sk, D], fp16 or bf16, Hq a multiple of
+    Hkv, D a multiple of 8 up to 128, rows contiguous and 16-byte aligned (any
+    other strides, so [B, S, H, D] tensors come as transposed views).  The
+    queries are the last Sq of the keys' positions.
+
+    softcap      scores become softcap * tanh(score / softcap); 0: they do not
+    slopes       fp32 [Hq] or [B, Hq]: slope * distance is subtracted
+    documents    int32 [B, Sq]: a query sees the keys of its own document;
+                 negative: padding, sees and is seen by none
+    documents_k  int32 [B, Sk]: the keys' (default: documents)
+    prefix_lens  int32 [B]: keys below are seen by every query (causal only)
+    kv_lens      int32 [B]: keys in use, the rest of k and v is not read
+
+    A query that sees no key gives zeros, and -inf in the log-sum-exp that
+    return_lse=True also returns (fp32 [B, Hq, Sq], without a gradient)."""
+    _need_attn()
+    if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
+        raise ValueError("slopes have no gradient: pass them detached")
+    out, lse = _ScoreAttention.apply(q, k, v, causal, softmax_scale, softcap, slopes, documents,
+                                     documents_k, prefix_lens, kv_lens)
+    return (out, lse) if return_lse else out
+
+
+class _Rotary(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, positions, freqs, interleaved, *xs):
+        ctx.save_for_backward(positions, freqs)
+        ctx.interleaved = interleaved
+        return tuple(torch.ops.shaobo_fa3.rotary(list(xs), positions, freqs, interleaved, False))
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *dys):
+        positions, freqs = ctx.saved_tensors
+        dxs = torch.ops.shaobo_fa3.rotary([_in_rows(d) for d in dys], positions, freqs,
+                                          ctx.interleaved, True)
+        return (None, None, None, *dxs)
+
+
+def rotary(q, k=None, *, positions, freqs, interleaved=False):
+    """q, or (q, k), with each row's first 2 * pairs elements turned by its
+    positions: pair p by sum_a positions[a] * freqs[a, p] radians.
+
+    q [B, Hq, S, D], k [B, Hkv, S, D], fp16, bf16 or fp32, in rows as
+    score_attention takes them (D up to 512); positions int32, int64 or fp32
+    [axes, B, S], any strides; freqs fp32 [axes, pairs] (rotary_freqs makes
+    one), pairs a multiple of 8, axes up to 4.  Pairs are elements (p, pairs +
+    p), or (2 p, 2 p + 1) where interleaved.  Positions and freqs have no
+    gradient."""
+    _need_attn()
+    if torch.is_grad_enabled() and (positions.requires_grad or freqs.requires_grad):
+        raise ValueError("positions and freqs have no gradient: pass them detached")
+    ys = _Rotary.apply(positions, freqs, interleaved, *((q,) if k is None else (q, k)))
+    return ys[0] if k is None else ys
+
+
+def rotary_freqs(sections, theta=10000.0, device=None):
+    """freqs [axes, pairs] of an axis owning sections[a] pairs, one axis after
+    the other, pair p of all turning by theta^(-p / pairs) a step: positions
+    of several axes that agree turn as one axis would."""
+    pairs = sum(sections)
+    inv = theta ** (-torch.arange(pairs, dtype=torch.float64) / pairs)
+    freqs = torch.zeros(len(sections), pairs, dtype=torch.float32)
+    at = 0
+    for a, n in enumerate(sections):
+        freqs[a, at:at + n] = inv[at:at + n].float()
+        at += n
+    return freqs.to(device)

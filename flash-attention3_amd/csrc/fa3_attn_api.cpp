@@ -69,6 +69,7 @@ int check(const ShaoboFa3AttnParams* a, bool backward, AttnProblem* p) {
     p->bf16 = a->dtype == SHAOBO_FA3_DTYPE_BF16;
     p->scale = a->softmax_scale_is_set ? a->softmax_scale : 1.f / std::sqrt((float)a->head_dim);
     p->softcap = a->softcap;
+    p->causal = a->causal != 0;
     p->bias = a->slopes != nullptr;
     p->docs = a->documents_q != nullptr;
     if ((int64_t)p->batch * p->heads_q >= (1 << 30)) return SHAOBO_FA3_STATUS_UNSUPPORTED;

@@ -9,25 +9,13 @@
 // leaves -lse log2 e and -delta per row, padded to whole tiles: a row that
 // sees no key, or is not there, has -infinity in place of the first, which
 // makes its P zero.
+#pragma once
+
 #include "fa3_attn_device.h"
 
 namespace fa3 {
 namespace {
 
-struct AttnBwdArgs {
-    AttnView q, k, v, dout, out, dq, dk, dv;
-    const float* lse;
-    float* softmax_d;
-    float* nlse2;   // [batch * heads_q][sqp]
-    float* ndelta;
-    int* flags;     // [batch * heads_q][sqp / 64]: a row that takes no part
-    AttnMask m;
-    float scale;
-    int heads_q, heads_kv, group, sq, sk, d, sqp;
-    int rows;  // group * sq
-    int kv_tiles, q_tiles, groups;
-    FastDiv div_hkv, div_group, div_groups, div_gpart, div_hq, div_blocks;
-};
 
 template <int D>
 struct BwdCfg {
@@ -37,8 +25,9 @@ struct BwdCfg {
     static constexpr int kKs = D / 32, kDB = D / 16;
 };
 
-// Workgroup id's job: level < kv_tiles is a dKV job's key tile (first keys
-// first: causal's longest), then come the dQ jobs, last rows first.
+// Workgroup id's job: level < kv_tiles * parts is a dKV job's key tile and
+// part (first keys first: causal's longest), then come the dQ jobs, last rows
+// first.
 struct BwdJob {
     int b, hkv, level;
 };
@@ -110,8 +99,10 @@ __device__ __forceinline__ void attn_pds(float s, float dp, float nl, float c, f
     if constexpr (kCap) ds *= __builtin_fmaf(-t, t, 1.f);
 }
 
-template <int D, bool kBf16, bool kCap, bool kBias, bool kFine>
-__device__ __forceinline__ void attn_dkv(int b, int hkv, int tile, FA3_LDS char* smem) {
+// Key tile `tile` (128 / kSplit keys).  kSplit 2: the two waves of a 32-key
+// block take one 32-row half of every stage each, and add up at the end.
+template <int D, bool kBf16, bool kCap, bool kBias, bool kFine, int kSplit>
+__device__ __forceinline__ void attn_dkv(int b, int hkv, int level, FA3_LDS char* smem) {
     typedef AttnBwdArgs Args;
     using C = BwdCfg<D>;
     using R = RegCfg<D>;
@@ -122,7 +113,11 @@ __device__ __forceinline__ void attn_dkv(int b, int hkv, int tile, FA3_LDS char*
     const int kv = attn_kv(a.m, b, a.sk), off = kv - a.sq;
     // (keys below it are seen by every query)
     const int prefix = a.m.causal ? attn_prefix(a.m, b) : 0x7fffffff;
-    const int wg_key = tile * kAttnRows, key0 = wg_key + 32 * w;
+    constexpr int kKb = kRegWaves / kSplit;  // 32-key blocks of the job
+    const int tile = fdiv(a.div_parts, level), part = level - tile * a.parts;
+    const int head_part = fdiv(a.div_rparts, part), row_part = part - head_part * a.row_parts;
+    const int rs = w / kKb;
+    const int wg_key = tile * (32 * kKb), key0 = wg_key + 32 * (w & (kKb - 1));
 
     f16x8 kf[2][C::kKs], vf[2][C::kKs];
     int id[2];
@@ -145,12 +140,17 @@ __device__ __forceinline__ void attn_dkv(int b, int hkv, int tile, FA3_LDS char*
     const bool docs = a.m.doc_k != nullptr;
     if (docs) doc = doc_span(id, (FA3_LDS int*)(smem + C::kRangeOff), w, lane);
 
-    int begin = 0;
+    int begin = 0, end = a.sqp / 64;
     if (wg_key >= prefix && wg_key - off > 0) begin = (wg_key - off) >> 6;
-    TileWalk walk(docs ? a.m.range_q + (int64_t)b * a.m.blocks_q : nullptr, begin,
-                  wg_key < kv ? a.sqp / 64 : begin, doc);
-    int t = walk.next(), g = 0;  // the step being computed: query tile and head of the group
-    int ld_t = t, ld_g = 0;      // the step being loaded
+    if (wg_key >= kv) end = begin;
+    const int len = end - begin;
+    TileWalk walk(docs ? a.m.range_q + (int64_t)b * a.m.blocks_q : nullptr,
+                  begin + len * row_part / a.row_parts, begin + len * (row_part + 1) / a.row_parts,
+                  doc);
+    const int g_first = a.group * head_part / a.head_parts;
+    const int g_end = a.group * (head_part + 1) / a.head_parts;
+    int t = walk.next(), g = g_first;  // the step being computed: query tile and head of the group
+    int ld_t = t, ld_g = g_first;      // the step being loaded
     auto issue = [&](FA3_LDS char* st) {
         const int ln = opaque_tid() & 63, i0 = ld_t * 64, h = hkv * attn_args<Args>().group + ld_g;
         int64_t row;  // of the statistics
@@ -262,6 +262,7 @@ __device__ __forceinline__ void attn_dkv(int b, int hkv, int tile, FA3_LDS char*
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int m = j >> 2, e = j & 3;
+                if (kCap && kSplit == 2 && j == 4) wall();
                 attn_pds<kCap, kBias>(s[m][n][e], dp[m][n][e], nl[m][e], c, k1, cap2, kFine, slope,
                                       d0 + (float)(16 * m + e), bit_mask(vis, 8 * n + j), p[n][j],
                                       ds[n][j]);
@@ -275,8 +276,8 @@ __device__ __forceinline__ void attn_dkv(int b, int hkv, int tile, FA3_LDS char*
     FA3_LDS char* s1 = smem + R::kStageBytes;
     int cls = walk.cls;  // of the tile being computed
     auto advance = [&]() {
-        if (++ld_g == attn_args<Args>().group) {
-            ld_g = 0;
+        if (++ld_g == g_end) {
+            ld_g = g_first;
             ld_t = walk.next();
         }
     };
@@ -287,8 +288,12 @@ __device__ __forceinline__ void attn_dkv(int b, int hkv, int tile, FA3_LDS char*
         advance();
         if (ld_t >= 0) issue(ld);
         if (cls & kTileMeets) {
-            sub(st, 0, cls & kTileSame);
-            sub(st, 1, cls & kTileSame);
+            if constexpr (kSplit == 1) {
+                sub(st, 0, cls & kTileSame);
+                sub(st, 1, cls & kTileSame);
+            } else {
+                sub(st, rs, cls & kTileSame);
+            }
         }
         t = ld_t;
         g = ld_g;
@@ -303,20 +308,54 @@ __device__ __forceinline__ void attn_dkv(int b, int hkv, int tile, FA3_LDS char*
     barrier();  // every wave is done with the stages: they take the outputs
     const auto& z = attn_args<Args>();
     const BwdJob e = bwd_job(z, blockIdx.x);  // (decoded again: not held over the loop)
-    const int ew = __builtin_amdgcn_readfirstlane(opaque_tid() >> 6);
-    const int ekey = e.level * kAttnRows + 32 * ew;
-    FA3_LDS char* stg = smem + ew * C::kDB * 1024;
-    const float one[2] = {1.f, 1.f}, sc[2] = {z.scale, z.scale};
-    auto store = [&](const f32x4 (&acc)[C::kDB][2], const auto& x, const float (&mul)[2]) {
-        attn_store<D, kBf16>(acc, mul, z.d, stg, [&](int r) -> _Float16* {
+    const int etile = fdiv(z.div_parts, e.level), epart = e.level - etile * z.parts;
+    const int ew = __builtin_amdgcn_readfirstlane(opaque_tid() >> 6), ers = ew / kKb;
+    const int ekb = ew & (kKb - 1), ekey = (etile * kKb + ekb) * 32;
+    const int eln = opaque_tid() & 63;
+    auto store = [&](const f32x4 (&acc)[C::kDB][2], const auto& x, float mul, int which,
+                     FA3_LDS char* stg) {
+        if (z.parts > 1) {
+            const int64_t first = ((int64_t)(2 * epart + which) * z.groups + e.b * z.heads_kv + e.hkv) * z.sk;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int j = ekey + 16 * n + (eln & 15);
+                if (j >= z.sk) continue;
+                float* p = z.part + (first + j) * D + 4 * (eln >> 4);
+#pragma unroll
+                for (int i = 0; i < C::kDB; ++i) *(f32x4*)(p + 16 * i) = acc[i][n];
+            }
+            return;
+        }
+        const float m2[2] = {mul, mul};
+        attn_store<D, kBf16>(acc, m2, z.d, stg, [&](int r) -> _Float16* {
             return ekey + r < z.sk ? x.p + e.b * x.bs + e.hkv * x.hs + (ekey + r) * x.rs : nullptr;
         });
     };
-    store(av, z.dv, one);
-    store(ak, z.dk, sc);
+    if constexpr (kSplit == 1) {
+        FA3_LDS char* stg = smem + ew * C::kDB * 1024;
+        store(av, z.dv, 1.f, 0, stg);
+        store(ak, z.dk, z.scale, 1, stg);
+    } else {
+        // the two waves of a key block swap halves: one sums and writes dV, the other dK
+        FA3_LDS char* mine = smem + ew * C::kDB * 2048;
+        FA3_LDS char* other = smem + (ekb + kKb * (1 - ers)) * C::kDB * 2048;
+        if (ers == 0) reg_put<C::kDB>(mine, ak, eln);
+        else reg_put<C::kDB>(mine, av, eln);
+        wait_vm_lgkm0<0>();
+        barrier();
+        if (ers == 0) {
+            reg_add<C::kDB>(other, av, eln);
+            store(av, z.dv, 1.f, 0, other);
+        } else {
+            reg_add<C::kDB>(other, ak, eln);
+            store(ak, z.dk, z.scale, 1, other);
+        }
+    }
 }
 
-template <int D, bool kBf16, bool kCap, bool kBias, bool kFine>
+// Row tile `tile` (128 / kSplit rows).  kSplit 2: the two waves of a 32-row
+// block take one 32-key half of every stage each.
+template <int D, bool kBf16, bool kCap, bool kBias, bool kFine, int kSplit>
 __device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* smem) {
     typedef AttnBwdArgs Args;
     using C = BwdCfg<D>;
@@ -327,9 +366,11 @@ __device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* 
     const int l16 = lane & 15, g4 = lane >> 4;
     const int kv = attn_kv(a.m, b, a.sk), prefix = attn_prefix(a.m, b), off = kv - a.sq;
     const bool causal = a.m.causal;
-    const int row0 = tile * kAttnRows + 32 * w;
+    constexpr int kQb = kRegWaves / kSplit;  // 32-row blocks of the job
+    const int rs = w / kQb;
+    const int row0 = (tile * kQb + (w & (kQb - 1))) * 32;
     const bool any = row0 < a.rows;
-    const int last = min(row0 + 32, a.rows) - 1, wg_last = min((tile + 1) * kAttnRows, a.rows) - 1;
+    const int last = min(row0 + 32, a.rows) - 1, wg_last = min((tile + 1) * (32 * kQb), a.rows) - 1;
     const int lim_min = any ? attn_limit(fdiv(a.div_group, row0), off, kv, causal, prefix) : 0x7fffffff;
     const int lim_max = any ? attn_limit(fdiv(a.div_group, last), off, kv, causal, prefix) : 0;
     const int wg_max = attn_limit(fdiv(a.div_group, wg_last), off, kv, causal, prefix);
@@ -461,8 +502,12 @@ __device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* 
         const int tn = walk.next();
         if (tn >= 0) issue(ld, tn);
         if (cls & kTileMeets) {
-            sub(st, t, 0, cls & kTileSame);
-            sub(st, t, 1, cls & kTileSame);
+            if constexpr (kSplit == 1) {
+                sub(st, t, 0, cls & kTileSame);
+                sub(st, t, 1, cls & kTileSame);
+            } else {
+                sub(st, t, rs, cls & kTileSame);
+            }
         }
         t = tn;
     };
@@ -475,131 +520,96 @@ __device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* 
     barrier();
     const auto& z = attn_args<Args>();
     const BwdJob e = bwd_job(z, blockIdx.x);
-    const int ew = __builtin_amdgcn_readfirstlane(opaque_tid() >> 6);
-    const int erow = (z.kv_tiles + z.q_tiles - 1 - e.level) * kAttnRows + 32 * ew;
+    const int ew = __builtin_amdgcn_readfirstlane(opaque_tid() >> 6), ers = ew / kQb;
+    const int eqb = ew & (kQb - 1), eln = opaque_tid() & 63;
+    const int erow = ((z.kv_tiles * z.parts + z.q_tiles - 1 - e.level) * kQb + eqb) * 32;
     const float sc[2] = {z.scale, z.scale};
-    attn_store<D, kBf16>(acc, sc, z.d, smem + ew * C::kDB * 1024, [&](int r) -> _Float16* {
+    FA3_LDS char* stg = smem + ew * C::kDB * 1024;
+    if constexpr (kSplit == 2) {
+        // the second wave's sums go to the first, which writes
+        FA3_LDS char* slot = smem + eqb * C::kDB * 2048;
+        stg = slot;
+        if (ers == 1) reg_put<C::kDB>(slot, acc, eln);
+        wait_vm_lgkm0<0>();
+        barrier();
+        if (ers == 1) return;
+        reg_add<C::kDB>(slot, acc, eln);
+    }
+    attn_store<D, kBf16>(acc, sc, z.d, stg, [&](int r) -> _Float16* {
         const AttnRow x = attn_row(erow + r, z.rows, e.hkv, z.group, z.div_group);
         return x.ok ? z.dq.p + e.b * z.dq.bs + x.h * z.dq.hs + x.i * z.dq.rs : nullptr;
     });
 }
 
-// kCap: 0 none, 1 capped, 2 capped with tanh's series for small scores
-template <int D, bool kBf16, int kCap, bool kBias>
+// kCap: 0 none, 1 capped, 2 capped with tanh's series for small scores.
+// kSplit: jobs of 128 / kSplit keys or rows.
+template <int D, bool kBf16, int kCap, bool kBias, int kSplit>
 __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_bwd_kernel(AttnBwdArgs) {
     __shared__ __attribute__((aligned(1024))) char smem_raw[BwdCfg<D>::kBytes];
     FA3_LDS char* smem = (FA3_LDS char*)smem_raw;
     const auto& a = attn_args<AttnBwdArgs>();
     const BwdJob j = bwd_job(a, blockIdx.x);
-    if (j.level < a.kv_tiles)
-        attn_dkv<D, kBf16, kCap != 0, kBias, kCap == 2>(j.b, j.hkv, j.level, smem);
+    const int n = a.kv_tiles * a.parts;
+    if (j.level < n)
+        attn_dkv<D, kBf16, kCap != 0, kBias, kCap == 2, kSplit>(j.b, j.hkv, j.level, smem);
     else
-        attn_dq<D, kBf16, kCap != 0, kBias, kCap == 2>(j.b, j.hkv, a.kv_tiles + a.q_tiles - 1 - j.level, smem);
+        attn_dq<D, kBf16, kCap != 0, kBias, kCap == 2, kSplit>(j.b, j.hkv, n + a.q_tiles - 1 - j.level, smem);
 }
 
-AttnView view(const ShaoboFa3AttnTensor& t) {
-    return AttnView{(_Float16*)t.data, t.batch_stride, t.head_stride, t.row_stride};
+// dV and dK from their parts, added in order; 8 columns a thread.
+template <int D, bool kBf16>
+__global__ __launch_bounds__(256) void attn_sum_kernel(AttnBwdArgs a) {
+    constexpr int kLanes = D / 8;
+    const int64_t rows = (int64_t)a.groups * a.sk;
+    const int64_t r = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
+    const int which = blockIdx.y, col = (threadIdx.x % kLanes) * 8;
+    if (r >= rows || col >= a.d) return;
+    float x[8] = {};
+    for (int p = 0; p < a.parts; ++p) {
+        const float* y = a.part + ((int64_t)(2 * p + which) * rows + r) * D + col;
+        const f32x4 lo = *(const f32x4*)y, hi = *(const f32x4*)(y + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            x[e] += lo[e];
+            x[4 + e] += hi[e];
+        }
+    }
+    const int grp = (int)(r / a.sk), j = (int)(r - (int64_t)grp * a.sk);
+    const int b = fdiv(a.div_hkv, grp), hkv = grp - b * a.heads_kv;
+    const AttnView& o = which ? a.dk : a.dv;
+    const float mul = which ? a.scale : 1.f;
+    f16x8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = to16<kBf16>(x[e] * mul);
+    *(f16x8*)(o.p + b * o.bs + hkv * o.hs + j * o.rs + col) = v;
+}
+
+// The kernels of one call: delta, the jobs, and the parts' sum.
+template <int D, bool kBf16>
+void launch_bwd(const AttnBwdArgs& x, const AttnBwdPlan& f, int cap, bool bias, hipStream_t stream) {
+    const int blocks = x.groups * x.group * (x.sqp / 64);
+    if (blocks > 0)
+        hipLaunchKernelGGL((attn_delta_kernel<D, kBf16>), dim3(blocks), dim3(256), 0, stream, x);
+    auto go = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(f.jobs), dim3(kRegThreads), 0, stream, x);
+    };
+    auto splits = [&](auto bi, auto split) {
+        constexpr bool kBi = decltype(bi)::value;
+        constexpr int kS = decltype(split)::value;
+        if (cap == 2) go(attn_bwd_kernel<D, kBf16, 2, kBi, kS>);
+        else if (cap == 1) go(attn_bwd_kernel<D, kBf16, 1, kBi, kS>);
+        else go(attn_bwd_kernel<D, kBf16, 0, kBi, kS>);
+    };
+    auto biases = [&](auto bi) {
+        f.split == 2 ? splits(bi, std::integral_constant<int, 2>{})
+                     : splits(bi, std::integral_constant<int, 1>{});
+    };
+    bias ? biases(std::true_type{}) : biases(std::false_type{});
+    if (x.parts > 1 && x.sk > 0)
+        hipLaunchKernelGGL((attn_sum_kernel<D, kBf16>),
+                           dim3(ceil_div((int64_t)x.groups * x.sk, 2048 / D), 2), dim3(256), 0,
+                           stream, x);
 }
 
 }  // namespace
-
-AttnBwdPlan plan_attn_bwd(const AttnProblem& p) {
-    AttnBwdPlan f{};
-    const int64_t rows = (int64_t)p.group * p.sq, groups = (int64_t)p.batch * p.heads_kv;
-    f.kv_tiles = ceil_div(p.sk, kAttnRows);
-    f.q_tiles = ceil_div(rows, kAttnRows);
-    f.sqp = ceil_div(p.sq, 64) * 64;
-    const int64_t jobs = groups * ((int64_t)f.kv_tiles + f.q_tiles);
-    const int64_t blocks = groups * p.group * (f.sqp / 64);
-    size_t at = 0;
-    auto take = [&](size_t n) {
-        const size_t x = at;
-        at += (n + 255) / 256 * 256;
-        return x;
-    };
-    f.nlse2_off = take((size_t)blocks * 64 * 4);
-    f.ndelta_off = take((size_t)blocks * 64 * 4);
-    f.flag_off = take((size_t)blocks * 4);
-    f.range_k_off = take(p.docs ? (size_t)p.batch * ceil_div(p.sk, 64) * sizeof(AttnRange) : 0);
-    f.range_q_off = take(p.docs ? (size_t)p.batch * (f.sqp / 64) * sizeof(AttnRange) : 0);
-    f.total = at;
-    f.ok = rows < (1ll << 30) && jobs < (1ll << 30) && blocks < (1ll << 30);
-    f.jobs = f.ok ? (int)jobs : 0;
-    return f;
-}
-
-hipError_t launch_attn_bwd(const AttnProblem& p, const ShaoboFa3AttnParams& a, AttnMask m,
-                           hipStream_t stream) {
-    const AttnBwdPlan f = plan_attn_bwd(p);
-    if (f.jobs == 0) return hipSuccess;
-    char* ws = (char*)a.workspace;
-    AttnBwdArgs x{};
-    x.q = view(a.q);
-    x.k = view(a.k);
-    x.v = view(a.v);
-    x.out = view(a.out);
-    x.dout = view(a.dout);
-    x.dq = view(a.dq);
-    x.dk = view(a.dk);
-    x.dv = view(a.dv);
-    x.lse = a.softmax_lse;
-    x.softmax_d = a.softmax_d;
-    x.nlse2 = (float*)(ws + f.nlse2_off);
-    x.ndelta = (float*)(ws + f.ndelta_off);
-    x.flags = (int*)(ws + f.flag_off);
-    x.scale = p.scale;
-    x.heads_q = p.heads_q;
-    x.heads_kv = p.heads_kv;
-    x.group = p.group;
-    x.sq = p.sq;
-    x.sk = p.sk;
-    x.d = p.d;
-    x.sqp = f.sqp;
-    x.rows = p.group * p.sq;
-    x.kv_tiles = f.kv_tiles;
-    x.q_tiles = f.q_tiles;
-    x.groups = p.batch * p.heads_kv;
-    x.div_hkv = make_fastdiv(p.heads_kv);
-    x.div_group = make_fastdiv(p.group);
-    x.div_groups = make_fastdiv(x.groups);
-    x.div_gpart = make_fastdiv(x.groups / 8);
-    x.div_hq = make_fastdiv(p.heads_q);
-    x.div_blocks = make_fastdiv(f.sqp / 64);
-    if (p.docs) {
-        AttnRange* rk = (AttnRange*)(ws + f.range_k_off);
-        AttnRange* rq = (AttnRange*)(ws + f.range_q_off);
-        hipError_t e = launch_attn_ranges(m.doc_k, m.doc_k_bs, p.batch, p.sk, rk, stream);
-        if (e == hipSuccess) e = launch_attn_ranges(m.doc_q, m.doc_q_bs, p.batch, p.sq, rq, stream);
-        if (e != hipSuccess) return e;
-        m.range_k = rk;
-        m.range_q = rq;
-        m.blocks_k = ceil_div(p.sk, 64);
-        m.blocks_q = f.sqp / 64;
-    }
-    x.m = m;
-    const int cap = p.softcap > 0.f ? m.cap_fine ? 2 : 1 : 0;
-    const int blocks = x.groups * p.group * (f.sqp / 64);
-    auto pick = [&](auto d, auto bf) {
-        constexpr int kD = decltype(d)::value;
-        constexpr bool kB = decltype(bf)::value;
-        if (blocks > 0)
-            hipLaunchKernelGGL((attn_delta_kernel<kD, kB>), dim3(blocks), dim3(256), 0, stream, x);
-        auto go = [&](auto kernel) {
-            hipLaunchKernelGGL(kernel, dim3(f.jobs), dim3(kRegThreads), 0, stream, x);
-        };
-        auto caps = [&](auto bias) {
-            constexpr bool kBi = decltype(bias)::value;
-            if (cap == 2) go(attn_bwd_kernel<kD, kB, 2, kBi>);
-            else if (cap == 1) go(attn_bwd_kernel<kD, kB, 1, kBi>);
-            else go(attn_bwd_kernel<kD, kB, 0, kBi>);
-        };
-        p.bias ? caps(std::true_type{}) : caps(std::false_type{});
-    };
-    using T = std::true_type;
-    using F = std::false_type;
-    if (p.d > 64) p.bf16 ? pick(std::integral_constant<int, 128>{}, T{}) : pick(std::integral_constant<int, 128>{}, F{});
-    else p.bf16 ? pick(std::integral_constant<int, 64>{}, T{}) : pick(std::integral_constant<int, 64>{}, F{});
-    return hipGetLastError();
-}
-
 }  // namespace fa3

@@ -194,8 +194,8 @@ __device__ __forceinline__ f16x8 attn_row8(const _Float16* row, int c, int d, bo
 // options leave fewer registers for them at D 128.
 template <int D, bool kCap>
 struct AttnAhead : RegCfg<D> {
-    static constexpr int kAhead0 = D == 128 && kCap ? 3 : 2;
-    static constexpr int kAhead1 = 2;
+    static constexpr int kAhead0 = 2;
+    static constexpr int kAhead1 = D == 128 && kCap ? 1 : 2;
     static constexpr int kAheadG = D == 128 ? 4 : 2;
 };
 

@@ -48,7 +48,7 @@ struct AttnProblem {
     int batch, heads_q, heads_kv, group, sq, sk, d;
     bool bf16;
     float scale, softcap;
-    bool bias, docs;
+    bool causal, bias, docs;
 };
 
 constexpr int kAttnTile = 64;   // keys (or rows) streamed per step
@@ -67,14 +67,41 @@ struct AttnFwdPlan {
 AttnFwdPlan plan_attn_fwd(const AttnProblem& p);
 
 struct AttnBwdPlan {
-    int kv_tiles;  // 128-key tiles
-    int q_tiles;   // 128-row tiles of a KV head's group * sq rows
+    int split;     // jobs of 128 / split keys or rows
+    int kv_tiles;  // key tiles
+    int q_tiles;   // row tiles of a KV head's group * sq rows
+    int head_parts, row_parts;  // dKV jobs per key tile: their product
     int sqp;       // rows of the statistics, padded to whole 64-row blocks
     int jobs;
-    size_t nlse2_off, ndelta_off, flag_off, range_k_off, range_q_off, total;
+    size_t nlse2_off, ndelta_off, flag_off, range_k_off, range_q_off, part_off, total;
     bool ok;
 };
 AttnBwdPlan plan_attn_bwd(const AttnProblem& p);
+
+struct AttnBwdArgs {
+    AttnView q, k, v, dout, out, dq, dk, dv;
+    const float* lse;
+    float* softmax_d;
+    float* nlse2;   // [batch * heads_q][sqp]
+    float* ndelta;
+    int* flags;     // [batch * heads_q][sqp / 64]: a row that takes no part
+    AttnMask m;
+    float scale;
+    int heads_q, heads_kv, group, sq, sk, d, sqp;
+    int rows;  // group * sq
+    int kv_tiles, q_tiles, groups;
+    // dKV jobs per key tile: head_parts ranges of the group's heads times
+    // row_parts ranges of the query tiles.  More than one: their fp32 sums go
+    // to part [head_parts * row_parts][dV, dK][groups][sk][D] and attn_sum_kernel
+    // adds them in order.
+    int head_parts, row_parts, parts;
+    float* part;
+    FastDiv div_hkv, div_group, div_groups, div_gpart, div_hq, div_blocks, div_parts, div_rparts;
+};
+void launch_attn_bwd_d64_fp16(const AttnBwdArgs&, const AttnBwdPlan&, int cap, bool bias, hipStream_t);
+void launch_attn_bwd_d64_bf16(const AttnBwdArgs&, const AttnBwdPlan&, int cap, bool bias, hipStream_t);
+void launch_attn_bwd_d128_fp16(const AttnBwdArgs&, const AttnBwdPlan&, int cap, bool bias, hipStream_t);
+void launch_attn_bwd_d128_bf16(const AttnBwdArgs&, const AttnBwdPlan&, int cap, bool bias, hipStream_t);
 
 hipError_t launch_attn_fwd(const AttnProblem& p, const ShaoboFa3AttnParams& a, AttnMask m,
                            hipStream_t stream);

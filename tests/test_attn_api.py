@@ -166,6 +166,19 @@ def test_workspace_grows_with_what_it_holds(lib):
     assert need(True) >= rows * 8 + rows // 64 * 4
 
 
+def test_backward_cuts_few_heads_into_parts(lib):
+    """One KV head for many query heads: dK and dV are summed from parts, two
+    fp32 tensors each; many KV heads: they are not."""
+    def need(**kw):
+        p = params(lib, **kw)
+        return lib.shaobo_fa3_attn_bwd_workspace_bytes(ctypes.byref(p))
+
+    few = need(batch=1, seqlen_q=4096, seqlen_k=4096, num_heads_q=8, num_heads_kv=1)
+    assert few >= 2 * 2 * 4096 * 128 * 4
+    many = need(batch=4, seqlen_q=4096, seqlen_k=4096, num_heads_q=32, num_heads_kv=32)
+    assert many < 4 * 32 * 4096 * 8 + 4 * 32 * 64 * 4 + 3 * 256 + 1
+
+
 def rotary_params(lib, **kw):
     p = F.RotaryParams()
     lib.shaobo_fa3_rotary_params_init(ctypes.byref(p))

@@ -179,6 +179,25 @@ def test_long_key_axis(T, case):
     run_both(*make(case))
 
 
+# Backwards cut in every way: whole and halved jobs, parts over the heads and
+# over the query tiles, the parts' masks and last tiles.
+CUTS = [
+    dict(B=1, Hq=8, Hkv=1, Sq=700, D=128), dict(B=1, Hq=6, Hkv=1, Sq=333, D=64, docs=70.0, dtype=HF),
+    dict(B=1, Hq=3, Hkv=1, Sq=500, D=128, softcap=20.0, prefix=[100]), dict(B=1, Hq=1, Hkv=1, Sq=1500, D=64),
+    dict(B=1, Hq=5, Hkv=5, Sq=800, D=128, causal=False, slopes=1), dict(B=8, Hq=8, Hkv=8, Sq=290, D=128),
+    dict(B=8, Hq=16, Hkv=8, Sq=200, D=64, dtype=HF, softcap=200.0), dict(B=8, Hq=32, Hkv=8, Sq=130, D=128, bshd=True),
+    dict(B=2, Hq=16, Hkv=2, Sq=100, Sk=900, D=96), dict(B=2, Hq=4, Hkv=2, Sq=900, Sk=70, D=128, causal=False),
+    dict(B=1, Hq=12, Hkv=2, Sq=260, D=128, kv=[100]), dict(B=12, Hq=24, Hkv=12, Sq=140, D=128, docs=50.0, slopes=2),
+]
+
+
+@pytest.mark.parametrize("case", CUTS, ids=lambda c: "-".join(
+    f"{k}{str(v).replace('torch.', '')}" for k, v in c.items()))
+def test_backward_cuts(T, case):
+    print("[case]", case, flush=True)
+    run_both(*make(case))
+
+
 @pytest.mark.parametrize("Sq,Sk,causal", [(0, 5, True), (5, 0, True), (0, 0, False), (7, 0, False)])
 def test_no_queries_or_no_keys(T, Sq, Sk, causal):
     print("[case] empty", Sq, Sk, flush=True)

@@ -20,7 +20,9 @@ namespace {
 template <int D>
 struct BwdCfg {
     using R = RegCfg<D>;
-    static constexpr int kRangeOff = R::kBytes;
+    // two tiles, the rows' statistics, the documents of 64 rows or keys
+    static constexpr int kStageBytes = R::kStageBytes + 256, kIdsOff = R::kStageBytes;
+    static constexpr int kRangeOff = 2 * kStageBytes;
     static constexpr int kBytes = kRangeOff + 64;
     static constexpr int kKs = D / 32, kDB = D / 16;
 };
@@ -179,6 +181,8 @@ __device__ __forceinline__ void attn_dkv(int b, int hkv, int level, FA3_LDS char
         if (w < 2)
             __builtin_amdgcn_global_load_lds((const void*)((w == 0 ? a.nlse2 : a.ndelta) + row + ln),
                                              (FA3_LDS void*)(st + 2 * R::kTileBytes + 256 * w), 4, 0, 0);
+        else if (w == 2 && a.m.doc_q != nullptr)
+            attn_load_ids(st + C::kIdsOff, a.m.doc_q + b * a.m.doc_q_bs, i0, a.sq, ln);
     };
     f32x4 av[C::kDB][2], ak[C::kDB][2];
 #pragma unroll
@@ -212,19 +216,20 @@ __device__ __forceinline__ void attn_dkv(int b, int hkv, int level, FA3_LDS char
             }
             if (walk.ranges != nullptr) {
                 const auto& a = attn_args<Args>();
-                const int* ids = a.m.doc_q + b * a.m.doc_q_bs;
                 uint32_t met = 0;
                 int id[2];  // (read again: not worth two registers over the loop)
 #pragma unroll
                 for (int n = 0; n < 2; ++n)
                     id[n] = max(a.m.doc_k[b * a.m.doc_k_bs + min(key0 + 16 * n + (l & 15), a.sk - 1)], -1);
+                const FA3_LDS i32x4* ids = (const FA3_LDS i32x4*)(st + C::kIdsOff + 128 * r) + (l >> 4);
 #pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    const int rid =
-                        doc_of(ids[min(i0 + 4 * (l >> 4) + 16 * (x >> 2) + (x & 3), a.sq - 1)]);
+                for (int m = 0; m < 2; ++m) {
+                    const i32x4 x = ids[4 * m];
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
-                        met |= rid == id[n] ? 1u << (8 * n + x) : 0u;
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+                            met |= doc_of(x[e]) == id[n] ? 1u << (8 * n + 4 * m + e) : 0u;
                 }
                 vis &= met;
             }
@@ -273,7 +278,7 @@ __device__ __forceinline__ void attn_dkv(int b, int hkv, int level, FA3_LDS char
         reg_grads<D, kBf16, true, AttnAhead<D, kCap>>(rd, st + R::kTileBytes, st, r, bp, bs, av, ak);
     };
     FA3_LDS char* s0 = smem;
-    FA3_LDS char* s1 = smem + R::kStageBytes;
+    FA3_LDS char* s1 = smem + C::kStageBytes;
     int cls = walk.cls;  // of the tile being computed
     auto advance = [&]() {
         if (++ld_g == g_end) {
@@ -423,6 +428,7 @@ __device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* 
             attn_load_tile_edge<D>(st, kp, a.k.rs, j0, kv, a.d, w, ln, seen);
             attn_load_tile_edge<D>(st + R::kTileBytes, vp, a.v.rs, j0, kv, a.d, w, ln, seen);
         }
+        if (ids != nullptr && w == 0) attn_load_ids(st + C::kIdsOff, ids, j0, a.sk, ln);
     };
     f32x4 acc[C::kDB][2];
 #pragma unroll
@@ -446,14 +452,17 @@ __device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* 
                     vis |= 16 * (x >> 2) + (x & 3) < k ? 1u << (8 * n + x) : 0u;
             }
             if (ids != nullptr) {
-                const int sk = attn_args<Args>().sk;
                 uint32_t met = 0;
+                const FA3_LDS i32x4* kids = (const FA3_LDS i32x4*)(st + C::kIdsOff + 128 * r) +
+                                            ((opaque_tid() & 63) >> 4);
 #pragma unroll
-                for (int x = 0; x < 8; ++x) {
-                    const int kid = doc_of(ids[min(jl + 16 * (x >> 2) + (x & 3), sk - 1)]);
+                for (int m = 0; m < 2; ++m) {
+                    const i32x4 x = kids[4 * m];
 #pragma unroll
-                    for (int n = 0; n < 2; ++n)
-                        met |= kid == id[n] ? 1u << (8 * n + x) : 0u;
+                    for (int e = 0; e < 4; ++e)
+#pragma unroll
+                        for (int n = 0; n < 2; ++n)
+                            met |= doc_of(x[e]) == id[n] ? 1u << (8 * n + 4 * m + e) : 0u;
                 }
                 vis &= met;
             }
@@ -492,7 +501,7 @@ __device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* 
         reg_grads<D, kBf16, false, AttnAhead<D, kCap>>(rd, st, st, r, bs, bs, acc, acc);
     };
     FA3_LDS char* s0 = smem;
-    FA3_LDS char* s1 = smem + R::kStageBytes;
+    FA3_LDS char* s1 = smem + C::kStageBytes;
     int t = walk.next();
     if (t >= 0) issue(s0, t);
     auto stage = [&](FA3_LDS char* __restrict__ ld, const FA3_LDS char* __restrict__ st) {

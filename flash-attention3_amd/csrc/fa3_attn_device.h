@@ -9,6 +9,7 @@ namespace fa3 {
 namespace {
 
 typedef int i32x2 __attribute__((ext_vector_type(2)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
 
 constexpr float kNegInf = -__builtin_inff();
 
@@ -137,11 +138,12 @@ struct TileWalk {
         }
         const int k = __builtin_ctzll(live);
         live &= live - 1;
-        // (read once more, uniformly: held per lane, the ranges would cost
-        // two vector registers over the whole loop)
-        const i32x2 r = *(const i32x2*)(ranges + base + k);
-        const int x = __builtin_amdgcn_readfirstlane(r[0]);
-        const int hi = __builtin_amdgcn_readfirstlane(r[1]), lo = x < 0 ? ~x : x;
+        // (read once more, through the scalar cache: held per lane, the ranges
+        // would cost two vector registers over the whole loop, and a vector
+        // load here is waited for before the next tile's loads go out)
+        typedef __attribute__((address_space(4))) const i32x2 KRange;
+        const i32x2 r = *(KRange*)(uintptr_t)(ranges + base + k);
+        const int x = r[0], hi = r[1], lo = x < 0 ? ~x : x;
         cls = (hi >= doc.lo && lo <= doc.hi ? kTileMeets : 0) |
               (x >= 0 && !doc.pad && lo == hi && doc.lo == doc.hi && lo == doc.lo ? kTileSame : 0) |
               (x < 0 ? kTileHidden : 0);
@@ -182,6 +184,14 @@ __device__ __forceinline__ void attn_load_tile_edge(FA3_LDS char* tile, const _F
         __builtin_amdgcn_global_load_lds((const void*)p,
                                          (FA3_LDS void*)(tile + (w * kLd + j) * 1024), 16, 0, 0);
     }
+}
+
+// The documents of 64 positions from i0 on (n in all) to 256 bytes of LDS, by
+// one wave.
+__device__ __forceinline__ void attn_load_ids(FA3_LDS char* to, const int* ids, int i0, int n,
+                                              int lane) {
+    __builtin_amdgcn_global_load_lds((const void*)(ids + min(i0 + lane, n - 1)), (FA3_LDS void*)to,
+                                     4, 0, 0);
 }
 
 // 8 elements 8 c .. of a row (d of them are there), or zeros

@@ -29,101 +29,70 @@ struct AttnFwdArgs {
 template <int D>
 struct FwdCfg {
     static constexpr int kTileBytes = 64 * D * 2;
-    static constexpr int kStageBytes = 2 * kTileBytes;
+    static constexpr int kStageBytes = 2 * kTileBytes + 256;  // K, V, the keys' documents
     static constexpr int kRangeOff = 2 * kStageBytes;  // the waves' document ranges
     static constexpr int kBytes = kRangeOff + 64;
     static constexpr int kKs = D / 32, kDB = D / 16;
 };
 
+// A wave's 32 rows: what they see, and their running softmax and output.
 template <int D, bool kBf16, bool kCap, bool kBias>
-__global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(AttnFwdArgs) {
+struct FwdRows {
     typedef AttnFwdArgs Args;
-    const auto& a = attn_args<Args>();
-    using C = FwdCfg<D>;
-    __shared__ __attribute__((aligned(1024))) char smem_raw[C::kBytes];
-    FA3_LDS char* smem = (FA3_LDS char*)smem_raw;
-    const int lane = threadIdx.x & 63;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int l16 = lane & 15, g4 = lane >> 4;
-
-    int level, grp;
-    attn_job(blockIdx.x, a.groups, a.div_groups, a.div_gpart, level, grp);
-    const int b = fdiv(a.div_hkv, grp), hkv = grp - b * a.heads_kv;
-    const int tl = fdiv(a.div_splits, level);
-    const int split = level - tl * a.splits, tile = a.tiles - 1 - tl;
-    const int kv = attn_kv(a.m, b, a.sk), prefix = attn_prefix(a.m, b), off = kv - a.sq;
-
-    // this wave's rows, and what they see
-    const int row0 = tile * kAttnRows + 32 * w;
-    const bool any = row0 < a.rows;
-    const int last = min(row0 + 32, a.rows) - 1, wg_last = min((tile + 1) * kAttnRows, a.rows) - 1;
-    const int lim_min = any ? attn_limit(fdiv(a.div_group, row0), off, kv, a.m.causal, prefix) : 0x7fffffff;
-    const int lim_max = any ? attn_limit(fdiv(a.div_group, last), off, kv, a.m.causal, prefix) : 0;
-    const int wg_max = attn_limit(fdiv(a.div_group, wg_last), off, kv, a.m.causal, prefix);
-    f16x8 qf[2][C::kKs];
+    static constexpr int kKs = D / 32, kDB = D / 16;
+    static constexpr bool kLog2 = kCap || kBias;  // scores leave their product in the log2 domain
+    f16x8 qf[2][kKs];
     int lim[2], id[2];
     float qp[2], slope[2];
+    f32x4 o[kDB][2];  // columns 16 db + 4 g4 + e of rows 16 n + l16
+    float mx[2], sum[2];
+    int lim_min, lim_max;  // over the rows
+
+    // Rows row0 .. row0 + 31 of KV head hkv in batch entry b.
+    template <typename A>
+    __device__ __forceinline__ void init(const A& a, int row0, int b, int hkv, int kv, int prefix,
+                                         int off, int lane) {
+        const int l16 = lane & 15, g4 = lane >> 4;
+        const bool any = row0 < a.rows;
+        const int last = min(row0 + 32, a.rows) - 1;
+        lim_min = any ? attn_limit(fdiv(a.div_group, row0), off, kv, a.m.causal, prefix) : 0x7fffffff;
+        lim_max = any ? attn_limit(fdiv(a.div_group, last), off, kv, a.m.causal, prefix) : 0;
 #pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const AttnRow r = attn_row(row0 + 16 * n + l16, a.rows, hkv, a.group, a.div_group);
-        id[n] = -2;
-        // (documents: -1 for every negative one, -2 for rows that are not there)
-        if (a.m.doc_q != nullptr && r.ok) id[n] = max(a.m.doc_q[b * a.m.doc_q_bs + r.i], -1);
-        const bool ok = r.ok && a.scored && id[n] != -1;
-        const _Float16* q = a.q.p + b * a.q.bs + r.h * a.q.hs + r.i * a.q.rs;
+        for (int n = 0; n < 2; ++n) {
+            const AttnRow r = attn_row(row0 + 16 * n + l16, a.rows, hkv, a.group, a.div_group);
+            id[n] = -2;
+            // (documents: -1 for every negative one, -2 for rows that are not there)
+            if (a.m.doc_q != nullptr && r.ok) id[n] = max(a.m.doc_q[b * a.m.doc_q_bs + r.i], -1);
+            const bool ok = r.ok && a.scored && id[n] != -1;
+            const _Float16* q = a.q.p + b * a.q.bs + r.h * a.q.hs + r.i * a.q.rs;
 #pragma unroll
-        for (int s = 0; s < C::kKs; ++s) {
-            // (a scale below zero turns Q's signs)
-            qf[n][s] = attn_flip(attn_row8(q, p1_chunk<D>(s, g4), a.d, ok), a.flip);
+            for (int s = 0; s < kKs; ++s)  // (a scale below zero turns Q's signs)
+                qf[n][s] = attn_flip(attn_row8(q, p1_chunk<D>(s, g4), a.d, ok), a.flip);
+            lim[n] = r.ok ? attn_limit(r.i, off, kv, a.m.causal, prefix) : 0;
+            qp[n] = 0.f;
+            slope[n] = 0.f;
+            if constexpr (kBias) {
+                qp[n] = (float)(r.i + off);
+                slope[n] = a.m.slopes[b * a.m.slopes_bs + r.h] * kLog2e;
+            }
+            mx[n] = kNegInf;
+            sum[n] = 0.f;
         }
-        lim[n] = r.ok ? attn_limit(r.i, off, kv, a.m.causal, prefix) : 0;
-        qp[n] = 0.f;
-        slope[n] = 0.f;
-        if constexpr (kBias) {
-            qp[n] = (float)(r.i + off);
-            slope[n] = a.m.slopes[b * a.m.slopes_bs + r.h] * kLog2e;
-        }
+#pragma unroll
+        for (int i = 0; i < kDB; ++i) o[i][0] = o[i][1] = f32x4{};
     }
-    DocSpan doc{0, 0, 0, 0, false};
-    if (a.m.doc_q != nullptr) doc = doc_span(id, (FA3_LDS int*)(smem + C::kRangeOff), w, lane);
 
-    const _Float16* kp = a.k.p + b * a.k.bs + hkv * a.k.hs;
-    const _Float16* vp = a.v.p + b * a.v.bs + hkv * a.v.hs;
-    const int* ids = a.m.doc_k == nullptr ? nullptr : a.m.doc_k + b * a.m.doc_k_bs;
-    const int begin = split * a.part;
-    TileWalk walk(ids == nullptr ? nullptr : a.m.range_k + (int64_t)b * a.m.blocks_k, begin,
-                  min(begin + a.part, (wg_max + 63) >> 6), doc);
-    auto issue = [&](FA3_LDS char* st, int t) {
-        const int j0 = t * 64, lane = opaque_tid() & 63;
-        const auto& a = attn_args<Args>();
-        if (j0 + 64 <= kv && a.d == D && !(walk.cls & kTileHidden)) {
-            attn_load_tile<D>(st, kp, a.k.rs, j0, w, lane);
-            attn_load_tile<D>(st + C::kTileBytes, vp, a.v.rs, j0, w, lane);
-        } else {
-            auto seen = [&](int j) { return ids == nullptr || ids[j] >= 0; };
-            attn_load_tile_edge<D>(st, kp, a.k.rs, j0, kv, a.d, w, lane, seen);
-            attn_load_tile_edge<D>(st + C::kTileBytes, vp, a.v.rs, j0, kv, a.d, w, lane, seen);
-        }
-    };
-
-    f32x4 o[C::kDB][2];
-#pragma unroll
-    for (int i = 0; i < C::kDB; ++i) o[i][0] = o[i][1] = f32x4{};
-    float mx[2] = {kNegInf, kNegInf}, sum[2] = {0.f, 0.f};
-    const RegReader<D> rd0(lane, 0);
-    constexpr bool kLog2 = kCap || kBias;  // scores leave their product in the log2 domain
-    const float c = a.m.c;
-
-    auto compute = [&](const FA3_LDS char* st, int t, int cls) {
-        const int j0 = t * 64;
-        if (j0 >= lim_max) return;
-        if (!(cls & kTileMeets)) return;
-        const bool full = j0 + 64 <= lim_min && (cls & kTileSame);
+    // Keys j0 .. j0 + 16 M - 1, which are rows 16 m0 .. of the tiles tk and tv.
+    // full: every row sees every one of them.  ids: their documents in LDS, or null.
+    template <int M>
+    __device__ __forceinline__ void step(const RegReader<D>& rd0, const FA3_LDS char* tk,
+                                         const FA3_LDS char* tv, int m0, int j0, bool full,
+                                         const FA3_LDS char* ids, float c) {
         RegReader<D> rd = rd0;
         rd.opaque();
-        f32x4 s[4][2];  // [m][n]: keys 16 m + 4 g4 + e, rows 16 n + l16
+        f32x4 s[M][2];  // [m][n]: keys 16 m + 4 g4 + e, rows 16 n + l16
 #pragma unroll
-        for (int m = 0; m < 4; ++m) s[m][0] = s[m][1] = f32x4{};
+        for (int m = 0; m < M; ++m) s[m][0] = s[m][1] = f32x4{};
         // (the bias-free, cap-free score is masked in its product's seed: its
         // scale is positive, and nothing that can be masked is infinite)
         auto mask = [&]() {
@@ -133,32 +102,32 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(
             for (int n = 0; n < 2; ++n) {
                 const int k = lim[n] - jl;
 #pragma unroll
-                for (int m = 0; m < 4; ++m)
+                for (int m = 0; m < M; ++m)
 #pragma unroll
                     for (int e = 0; e < 4; ++e)
                         s[m][n][e] = 16 * m + e < k ? s[m][n][e] : kNegInf;
             }
             if (ids != nullptr) {
-                const int sk = attn_args<Args>().sk;
+                const FA3_LDS i32x4* kids = (const FA3_LDS i32x4*)ids + (ln >> 4);
 #pragma unroll
-                for (int m = 0; m < 4; ++m)
+                for (int m = 0; m < M; ++m) {
+                    const i32x4 kid = kids[4 * m];
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const int kid = doc_of(ids[min(jl + 16 * m + e, sk - 1)]);
+                    for (int e = 0; e < 4; ++e)
 #pragma unroll
                         for (int n = 0; n < 2; ++n)
-                            s[m][n][e] = kid == id[n] ? s[m][n][e] : kNegInf;
-                    }
+                            s[m][n][e] = doc_of(kid[e]) == id[n] ? s[m][n][e] : kNegInf;
+                }
             }
         };
         if (!kLog2 && !full) mask();
-        attn_scores<D, kBf16, 4, 4>(rd, st, 0, qf, s);
+        attn_scores<D, kBf16, M, 4>(rd, tk, m0, qf, s);
         if constexpr (kCap) {
             const auto& a = attn_args<Args>();
             const float k1 = a.m.k1, cap2 = a.m.cap2;
             if (a.m.cap_fine) {
 #pragma unroll
-                for (int m = 0; m < 4; ++m)
+                for (int m = 0; m < M; ++m)
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -166,7 +135,7 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(
                             s[m][n][e] = attn_tanh_fine(s[m][n][e], k1) * cap2;
             } else {
 #pragma unroll
-                for (int m = 0; m < 4; ++m)
+                for (int m = 0; m < M; ++m)
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -175,11 +144,12 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(
             }
         }
         if constexpr (kBias) {
+            const int g4 = (opaque_tid() & 63) >> 4;
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const float d0 = qp[n] - (float)(j0 + 4 * g4);
 #pragma unroll
-                for (int m = 0; m < 4; ++m)
+                for (int m = 0; m < M; ++m)
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const float x = kCap ? s[m][n][e] : s[m][n][e] * c;
@@ -195,7 +165,7 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(
         for (int n = 0; n < 2; ++n) {
             float x = mx[n];
 #pragma unroll
-            for (int m = 0; m < 4; ++m)
+            for (int m = 0; m < M; ++m)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x = __builtin_fmaxf(x, s[m][n][e]);
             mn[n] = max_groups(x);
@@ -211,11 +181,11 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(
                 mx[n] = mn[n];
                 sum[n] *= f;
 #pragma unroll
-                for (int i = 0; i < C::kDB; ++i) o[i][n] *= f;
+                for (int i = 0; i < kDB; ++i) o[i][n] *= f;
             }
         }
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {
+        for (int r = 0; r < M / 2; ++r) {
             f16x8 bp[2];
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
@@ -228,10 +198,161 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(
                 }
                 bp[n] = pack8<kBf16>(p);
             }
-            reg_grads<D, kBf16, false>(rd, st + C::kTileBytes, st + C::kTileBytes, r, bp, bp, o, o);
+            reg_grads<D, kBf16, false>(rd, tv, tv, m0 / 2 + r, bp, bp, o, o);
         }
-    };
+    }
 
+    // The four waves' (kSplit: of the same rows, over different keys) softmaxes
+    // meet: afterwards the wave with rs 0 holds the whole.  x: 2 KiB, slots:
+    // D / 16 * 2 KiB + 512 a wave of rs > 0.
+    template <int kSplit>
+    __device__ __forceinline__ void meet(FA3_LDS float* x, FA3_LDS char* slots, int w, int qb,
+                                         int rs, float c) {
+        constexpr int kQb = kRegWaves / kSplit, kSlot = kDB * 2048 + 512;
+        const int ln = opaque_tid() & 63;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) x[(2 * w + n) * 64 + ln] = mx[n];
+        wait_vm_lgkm0<0>();
+        barrier();
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            float top = kNegInf;
+#pragma unroll
+            for (int k = 0; k < kSplit; ++k)
+                top = __builtin_fmaxf(top, x[(2 * (qb + kQb * k) + n) * 64 + ln]);
+            const float mu = top == kNegInf ? 0.f : top;
+            const float f = fast_exp2(kLog2 ? mx[n] - mu : (mx[n] - mu) * c);
+            mx[n] = top;
+            sum[n] *= f;
+#pragma unroll
+            for (int i = 0; i < kDB; ++i) o[i][n] *= f;
+        }
+        if (rs > 0) {
+            FA3_LDS char* slot = slots + (qb + kQb * (rs - 1)) * kSlot;
+            reg_put<kDB>(slot, o, ln);
+            FA3_LDS float* l = (FA3_LDS float*)(slot + kDB * 2048);
+            l[ln] = sum[0];
+            l[64 + ln] = sum[1];
+        }
+        wait_vm_lgkm0<0>();
+        barrier();
+        if (rs > 0) return;
+#pragma unroll
+        for (int k = 0; k < kSplit - 1; ++k) {
+            FA3_LDS char* slot = slots + (qb + kQb * k) * kSlot;
+            reg_add<kDB>(slot, o, ln);
+            FA3_LDS float* l = (FA3_LDS float*)(slot + kDB * 2048);
+            sum[0] += l[ln];
+            sum[1] += l[64 + ln];
+        }
+    }
+
+    // The rows' outputs and log-sum-exps, or (splits > 1) their part of both;
+    // stg: D / 16 KiB of the wave's own.
+    __device__ __forceinline__ void finish(int row0, int b, int hkv, int grp, int split,
+                                           FA3_LDS char* stg) {
+        const auto& z = attn_args<Args>();
+        const int ln = opaque_tid() & 63, l16 = ln & 15, g4 = ln >> 4;
+        float inv[2], lse2[2];
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const float l = sum_groups(sum[n]);
+            const bool none = mx[n] == kNegInf;
+            inv[n] = none ? 0.f : 1.f / l;
+            if (none) {  // (its Q may have been NaN)
+#pragma unroll
+                for (int i = 0; i < kDB; ++i) o[i][n] = f32x4{};
+            }
+            lse2[n] = none ? kNegInf : (kLog2 ? mx[n] : mx[n] * z.m.c) + __builtin_amdgcn_logf(l);
+        }
+        if (z.splits > 1) {
+            const int64_t base = ((int64_t)split * z.groups + grp) * z.rows;
+#pragma unroll
+            for (int n = 0; n < 2; ++n) {
+                const int r = row0 + 16 * n + l16;
+                if (r >= z.rows) continue;
+                if (g4 == 0) z.part_l[base + r] = lse2[n];
+                float* p = z.part_o + (base + r) * D + 4 * g4;
+#pragma unroll
+                for (int i = 0; i < kDB; ++i) *(f32x4*)(p + 16 * i) = o[i][n] * inv[n];
+            }
+            return;
+        }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const AttnRow r = attn_row(row0 + 16 * n + l16, z.rows, hkv, z.group, z.div_group);
+            if (g4 == 0 && r.ok)
+                z.lse[((int64_t)b * z.heads_q + r.h) * z.sq + r.i] = lse2[n] * 0.69314718055994531f;
+        }
+        attn_store<D, kBf16>(o, inv, z.d, stg, [&](int r) -> _Float16* {
+            const AttnRow x = attn_row(row0 + r, z.rows, hkv, z.group, z.div_group);
+            return x.ok ? z.out.p + b * z.out.bs + x.h * z.out.hs + x.i * z.out.rs : nullptr;
+        });
+    }
+};
+
+// A workgroup's job: levels are row tiles (last rows first, causal's longest)
+// times parts of the key axis.
+struct FwdJob {
+    int b, hkv, grp, tile, split;
+};
+template <typename A>
+__device__ __forceinline__ FwdJob fwd_job(const A& a, int id) {
+    FwdJob j;
+    int level;
+    attn_job(id, a.groups, a.div_groups, a.div_gpart, level, j.grp);
+    j.b = fdiv(a.div_hkv, j.grp);
+    j.hkv = j.grp - j.b * a.heads_kv;
+    const int tl = fdiv(a.div_splits, level);
+    j.split = level - tl * a.splits;
+    j.tile = a.tiles - 1 - tl;
+    return j;
+}
+
+// 128 / kSplit rows a workgroup.  kSplit 2: the two waves of a 32-row block
+// take one 32-key half of every stage each.
+template <int D, bool kBf16, bool kCap, bool kBias, int kSplit>
+__global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(AttnFwdArgs) {
+    typedef AttnFwdArgs Args;
+    const auto& a = attn_args<Args>();
+    using C = FwdCfg<D>;
+    constexpr int kQb = kRegWaves / kSplit;  // 32-row blocks of the job
+    __shared__ __attribute__((aligned(1024))) char smem_raw[C::kBytes];
+    FA3_LDS char* smem = (FA3_LDS char*)smem_raw;
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int qb = w & (kQb - 1), rs = w / kQb;
+    const FwdJob job = fwd_job(a, blockIdx.x);
+    const int b = job.b, hkv = job.hkv;
+    const int kv = attn_kv(a.m, b, a.sk), prefix = attn_prefix(a.m, b), off = kv - a.sq;
+    FwdRows<D, kBf16, kCap, kBias> rows;
+    rows.init(a, (job.tile * kQb + qb) * 32, b, hkv, kv, prefix, off, lane);
+    const int wg_last = min((job.tile + 1) * (32 * kQb), a.rows) - 1;
+    const int wg_max = attn_limit(fdiv(a.div_group, wg_last), off, kv, a.m.causal, prefix);
+    DocSpan doc{0, 0, 0, 0, false};
+    if (a.m.doc_q != nullptr) doc = doc_span(rows.id, (FA3_LDS int*)(smem + C::kRangeOff), w, lane);
+
+    const _Float16* kp = a.k.p + b * a.k.bs + hkv * a.k.hs;
+    const _Float16* vp = a.v.p + b * a.v.bs + hkv * a.v.hs;
+    const int* ids = a.m.doc_k == nullptr ? nullptr : a.m.doc_k + b * a.m.doc_k_bs;
+    const int begin = job.split * a.part;
+    TileWalk walk(ids == nullptr ? nullptr : a.m.range_k + (int64_t)b * a.m.blocks_k, begin,
+                  min(begin + a.part, (wg_max + 63) >> 6), doc);
+    auto issue = [&](FA3_LDS char* st, int t) {
+        const int j0 = t * 64, lane = opaque_tid() & 63;
+        const auto& a = attn_args<Args>();
+        if (j0 + 64 <= kv && a.d == D && !(walk.cls & kTileHidden)) {
+            attn_load_tile<D>(st, kp, a.k.rs, j0, w, lane);
+            attn_load_tile<D>(st + C::kTileBytes, vp, a.v.rs, j0, w, lane);
+        } else {
+            auto seen = [&](int j) { return ids == nullptr || ids[j] >= 0; };
+            attn_load_tile_edge<D>(st, kp, a.k.rs, j0, kv, a.d, w, lane, seen);
+            attn_load_tile_edge<D>(st + C::kTileBytes, vp, a.v.rs, j0, kv, a.d, w, lane, seen);
+        }
+        if (ids != nullptr && w == 0) attn_load_ids(st + 2 * C::kTileBytes, ids, j0, a.sk, lane);
+    };
+    const RegReader<D> rd(lane, 0);
+    const float c = a.m.c;
     FA3_LDS char* s0 = smem;
     FA3_LDS char* s1 = smem + C::kStageBytes;
     int t = walk.next();
@@ -242,7 +363,15 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(
         barrier();
         const int tn = walk.next();
         if (tn >= 0) issue(ld, tn);
-        compute(st, t, cls);
+        if (cls & kTileMeets) {
+            constexpr int kKeys = 64 / kSplit;
+            const int j0 = t * 64 + kKeys * rs;
+            if (j0 < rows.lim_max)
+                rows.template step<4 / kSplit>(rd, st, st + C::kTileBytes, kKeys / 16 * rs, j0,
+                                               j0 + kKeys <= rows.lim_min && (cls & kTileSame),
+                                               ids == nullptr ? nullptr : st + 2 * C::kTileBytes + 4 * kKeys * rs,
+                                               c);
+        }
         t = tn;
     };
     while (t >= 0) {
@@ -250,81 +379,165 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(
         if (t < 0) break;
         stage(s0, s1);
     }
-
-    const auto& z = attn_args<Args>();
-    float inv[2], lse2[2];
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const float l = sum_groups(sum[n]);
-        const bool none = mx[n] == kNegInf;
-        inv[n] = none ? 0.f : 1.f / l;
-        if (none) {  // (its Q may have been NaN)
-#pragma unroll
-            for (int i = 0; i < C::kDB; ++i) o[i][n] = f32x4{};
-        }
-        lse2[n] = none ? kNegInf : (kLog2 ? mx[n] : mx[n] * c) + __builtin_amdgcn_logf(l);
-    }
-    if (z.splits > 1) {
-        const int64_t base = ((int64_t)split * z.groups + grp) * z.rows;
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const int r = row0 + 16 * n + l16;
-            if (r >= z.rows) continue;
-            if (g4 == 0) z.part_l[base + r] = lse2[n];
-            float* p = z.part_o + (base + r) * D + 4 * g4;
-#pragma unroll
-            for (int i = 0; i < C::kDB; ++i) *(f32x4*)(p + 16 * i) = o[i][n] * inv[n];
-        }
-        return;
-    }
     wait_vm_lgkm0<0>();
     barrier();  // every wave is done with the stages: they take the outputs
-#pragma unroll
-    for (int n = 0; n < 2; ++n) {
-        const AttnRow r = attn_row(row0 + 16 * n + l16, z.rows, hkv, z.group, z.div_group);
-        if (g4 == 0 && r.ok)
-            z.lse[((int64_t)b * z.heads_q + r.h) * z.sq + r.i] = lse2[n] * 0.69314718055994531f;
+    const FwdJob e = fwd_job(attn_args<Args>(), blockIdx.x);  // (decoded again: not held over the loop)
+    const int ew = __builtin_amdgcn_readfirstlane(opaque_tid() >> 6), eqb = ew & (kQb - 1);
+    if constexpr (kSplit > 1) {
+        rows.template meet<kSplit>((FA3_LDS float*)smem, smem + 2048, ew, eqb, ew / kQb, c);
+        if (ew / kQb > 0) return;
     }
-    attn_store<D, kBf16>(o, inv, z.d, smem + w * C::kDB * 1024, [&](int r) -> _Float16* {
-        const AttnRow x = attn_row(row0 + r, z.rows, hkv, z.group, z.div_group);
-        return x.ok ? z.out.p + b * z.out.bs + x.h * z.out.hs + x.i * z.out.rs : nullptr;
-    });
+    // (of the meeting, this wave reads only what it has read: its own block's slots)
+    rows.finish((e.tile * kQb + eqb) * 32, e.b, e.hkv, e.grp, e.split,
+                kSplit > 1 ? smem + 2048 + eqb * (C::kDB * 2048 + 512) : smem + ew * C::kDB * 1024);
+}
+
+// Few rows (32 at most of a KV head: single tokens), no documents: a
+// workgroup's four waves all hold them and take every fourth 32-key block
+// each, through two LDS stages of their own -- no barrier until they meet.
+// Bound by reading the cache.
+template <int D>
+struct TokenCfg {
+    static constexpr int kBlock = 32 * D * 2;   // 32 rows of K or V
+    static constexpr int kStage = 2 * kBlock;
+    static constexpr int kBytes = kRegWaves * 2 * kStage;
+    static constexpr int kLd = kBlock / 1024;   // loads per wave, block and tensor
+    static_assert(2048 + 3 * (D / 16 * 2048 + 512) <= kBytes, "the meeting fits the stages");
+};
+
+template <int D, bool kBf16, bool kCap, bool kBias>
+__global__ __launch_bounds__(kRegThreads, D == 64 ? 2 : 1) void attn_token_kernel(AttnFwdArgs) {
+    typedef AttnFwdArgs Args;
+    const auto& a = attn_args<Args>();
+    using C = TokenCfg<D>;
+    __shared__ __attribute__((aligned(1024))) char smem_raw[C::kBytes];
+    FA3_LDS char* smem = (FA3_LDS char*)smem_raw;
+    const int lane = threadIdx.x & 63;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const FwdJob job = fwd_job(a, blockIdx.x);
+    const int b = job.b, hkv = job.hkv;
+    const int kv = attn_kv(a.m, b, a.sk), prefix = attn_prefix(a.m, b), off = kv - a.sq;
+    const _Float16* kp = a.k.p + b * a.k.bs + hkv * a.k.hs;
+    const _Float16* vp = a.v.p + b * a.v.bs + hkv * a.v.hs;
+    // this wave's x-th block is keys 32 (first + 4 x) ..
+    const int lim = attn_limit(a.sq - 1, off, kv, a.m.causal, prefix);
+    const int first = 2 * job.split * a.part + w;
+    const int end = min(2 * (job.split + 1) * a.part, (lim + 31) >> 5);
+    const int n = end > first ? (end - first + 3) >> 2 : 0;
+    auto load = [&](FA3_LDS char* st, const _Float16* src, int64_t rs, int j0, bool whole, int d) {
+        constexpr int kRows = 512 / D, kC = D / 8;
+        const int ln = opaque_tid() & 63, row = ln / kC;
+        const uint32_t cc = ((uint32_t)(ln % kC) ^ reg_swz<D>(row)) & (kC - 1);
+        const char* p = (const char*)(src + (int64_t)(j0 + row) * rs);
+        auto put = [&](int j, const char* x) {
+            __builtin_amdgcn_global_load_lds((const void*)x, (FA3_LDS void*)(st + j * 1024), 16, 0, 0);
+        };
+        auto chunk = [&](int j) { return (cc ^ reg_swz<D>(kRows * j)) & (kC - 1); };
+        if (whole) {
+#pragma unroll
+            for (int j = 0; j < C::kLd; ++j) put(j, p + (int64_t)(kRows * j) * rs * 2 + chunk(j) * 16);
+        } else {
+#pragma unroll
+            for (int j = 0; j < C::kLd; ++j) {
+                const bool ok = j0 + kRows * j + row < kv && (int)chunk(j) * 8 < d;
+                put(j, ok ? p + (int64_t)(kRows * j) * rs * 2 + chunk(j) * 16 : (const char*)attn_zeros);
+            }
+        }
+    };
+    // one stage: always 2 kLd loads, which the waits below count
+    auto issue = [&](FA3_LDS char* st, int x) {
+        const auto& a = attn_args<Args>();
+        const int j0 = 32 * (first + 4 * x);
+        const bool whole = j0 + 32 <= kv && a.d == D;
+        load(st, kp, a.k.rs, j0, whole, a.d);
+        load(st + C::kBlock, vp, a.v.rs, j0, whole, a.d);
+    };
+    FA3_LDS char* s0 = smem + w * 2 * C::kStage;
+    FA3_LDS char* s1 = s0 + C::kStage;
+    if (n > 0) issue(s0, 0);
+    FwdRows<D, kBf16, kCap, kBias> rows;
+    rows.init(a, 0, b, hkv, kv, prefix, off, lane);
+    const RegReader<D> rd(lane, 0);
+    const float c = a.m.c;
+    int x = 0;
+    auto stage = [&](FA3_LDS char* __restrict__ ld, const FA3_LDS char* __restrict__ st) {
+        wait_vm_lgkm0<63>();  // (the block read from ld before is done with)
+        wall();
+        if (x + 1 < n) {
+            issue(ld, x + 1);
+            wall();
+            wait_vm_lgkm0<2 * C::kLd>();
+        } else {
+            wait_vm_lgkm0<0>();
+        }
+        __atomic_signal_fence(__ATOMIC_SEQ_CST);
+        wall();
+        const int j0 = 32 * (first + 4 * x);
+        rows.template step<2>(rd, st, st + C::kBlock, 0, j0, j0 + 32 <= rows.lim_min, nullptr, c);
+        ++x;
+    };
+    while (x < n) {
+        stage(s1, s0);
+        if (x >= n) break;
+        stage(s0, s1);
+    }
+    wait_vm_lgkm0<0>();
+    barrier();
+    const FwdJob e = fwd_job(attn_args<Args>(), blockIdx.x);
+    const int ew = __builtin_amdgcn_readfirstlane(opaque_tid() >> 6);
+    rows.template meet<4>((FA3_LDS float*)smem, smem + 2048, ew, 0, ew, c);
+    if (ew > 0) return;
+    rows.finish(0, e.b, e.hkv, e.grp, e.split, smem + 2048);
 }
 
 // Joins the parts of a split key axis: with w_s = exp2(l_s - max l), out =
-// sum w_s o_s / sum w_s.  16 lanes (D 128; 8 for D 64) take a row, 8 columns
-// each; bound by reading the parts.
-template <int D, bool kBf16>
+// sum w_s o_s / sum w_s.  D / 8 lanes hold a row, 8 columns each.  kWays
+// groups of them take every kWays-th part of it, whose sums meet at the end:
+// many parts are few rows, which leave only latency to win (32 parts, 32 rows:
+// 18 us with one way, 8 with four at D 128), and few parts are many rows,
+// which fill the chip (2 parts, 8 044 rows: 14 us with one way, 21 with four).
+template <int D, bool kBf16, int kWays>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnFwdArgs a) {
-    constexpr int kLanes = D / 8;
+    constexpr int kLanes = D / 8, kRow = kLanes * kWays;
+    const int lane = threadIdx.x & (kRow - 1);
     const int64_t total = (int64_t)a.groups * a.rows;
-    const int64_t rg = (int64_t)blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes;
-    const int col = (threadIdx.x % kLanes) * 8;
+    const int64_t rg = (int64_t)blockIdx.x * (256 / kRow) + (int)(threadIdx.x / kRow);
     if (rg >= total) return;
     float top = kNegInf;
-    for (int s = 0; s < a.splits; ++s) top = __builtin_fmaxf(top, a.part_l[s * total + rg]);
+    for (int s = lane; s < a.splits; s += kRow) top = __builtin_fmaxf(top, a.part_l[s * total + rg]);
+#pragma unroll
+    for (int o = kRow / 2; o > 0; o >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o));
+    const int col = (lane % kLanes) * 8;
     float z = 0.f, acc[8] = {};
-    for (int s = 0; s < a.splits; ++s) {
+#pragma unroll 4
+    for (int s = lane / kLanes; s < a.splits; s += kWays) {
         const float l = a.part_l[s * total + rg];
-        if (l == kNegInf) continue;  // (nothing seen there)
-        const float f = fast_exp2(l - top);
-        z += f;
         const float* p = a.part_o + (s * total + rg) * D + col;
         const f32x4 x = *(const f32x4*)p, y = *(const f32x4*)(p + 4);
+        // (a part that saw nothing has no output to weigh: it may hold anything)
+        const bool none = l == kNegInf;
+        const float f = none ? 0.f : fast_exp2(l - top);
+        z += f;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-            acc[e] = __builtin_fmaf(f, x[e], acc[e]);
-            acc[4 + e] = __builtin_fmaf(f, y[e], acc[4 + e]);
+            acc[e] = __builtin_fmaf(f, none ? 0.f : x[e], acc[e]);
+            acc[4 + e] = __builtin_fmaf(f, none ? 0.f : y[e], acc[4 + e]);
         }
+    }
+#pragma unroll
+    for (int o = kRow / 2; o >= kLanes; o >>= 1) {
+        z += __shfl_xor(z, o);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] += __shfl_xor(acc[e], o);
     }
     const int grp = (int)(rg / a.rows), r = (int)(rg - (int64_t)grp * a.rows);
     const int b = fdiv(a.div_hkv, grp), hkv = grp - b * a.heads_kv;
     const AttnRow x = attn_row(r, a.rows, hkv, a.group, a.div_group);
     const float inv = z > 0.f ? 1.f / z : 0.f;
-    if (col == 0)
+    if (lane == 0)
         a.lse[((int64_t)b * a.heads_q + x.h) * a.sq + x.i] =
             z > 0.f ? (top + __builtin_amdgcn_logf(z)) * 0.69314718055994531f : kNegInf;
-    if (col >= a.d) return;
+    if (lane >= kLanes || col >= a.d) return;
     f16x8 v;
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = to16<kBf16>(acc[e] * inv);
@@ -367,20 +580,18 @@ AttnFwdPlan plan_attn_fwd(const AttnProblem& p) {
     AttnFwdPlan f{};
     const int64_t rows = (int64_t)p.group * p.sq, groups = (int64_t)p.batch * p.heads_kv;
     const int D = p.d > 64 ? 128 : 64;
-    f.tiles = ceil_div(rows, kAttnRows);
     const int n_t = ceil_div(p.sk, 64);
+    f.token = rows <= 32 && !p.docs;
+    f.split = !f.token && groups * ceil_div(rows, kAttnRows) < 512 ? 2 : 1;
+    f.tiles = f.token ? 1 : ceil_div(rows, kAttnRows / f.split);
     f.splits = 1;
     f.part = n_t;
     const int64_t jobs = groups * f.tiles;
-    // Fewer workgroups than two per CU: the key axis is cut, into parts of at
-    // least four tiles.
-    if (jobs > 0 && jobs < 512 && n_t >= 8) {
-        const int want = (int)(512 / jobs), most = n_t / 4;
-        const int s = want < most ? want : most;
-        if (s > 1) {
-            f.part = ceil_div(n_t, s);
-            f.splits = ceil_div(n_t, f.part);
-        }
+    const int fill = f.token && D == 128 ? 256 : 512, least = f.token ? 4 : 8;
+    if (jobs > 0 && 2 * jobs <= fill && n_t >= 2 * least) {
+        const int want = (int)(fill / jobs), most = n_t / least;
+        f.part = ceil_div(n_t, want < most ? want : most);
+        f.splits = ceil_div(n_t, f.part);
     }
     size_t at = 0;
     auto take = [&](size_t n) {
@@ -394,8 +605,9 @@ AttnFwdPlan plan_attn_fwd(const AttnProblem& p) {
         f.pl_off = take((size_t)f.splits * groups * rows * 4);
     }
     f.total = at;
-    f.ok = rows < (1ll << 30) && jobs * f.splits < (1ll << 30);
-    f.jobs = f.ok ? (int)(jobs * f.splits) : 0;
+    const int64_t all = groups * f.tiles * f.splits;
+    f.ok = rows < (1ll << 30) && all < (1ll << 30);
+    f.jobs = f.ok ? (int)all : 0;
     return f;
 }
 
@@ -451,12 +663,25 @@ hipError_t launch_attn_fwd(const AttnProblem& p, const ShaoboFa3AttnParams& a, A
         auto go = [&](auto kernel) {
             hipLaunchKernelGGL(kernel, dim3(f.jobs), dim3(kRegThreads), 0, stream, x);
         };
-        if (cap) bias ? go(attn_fwd_kernel<kD, kB, true, true>) : go(attn_fwd_kernel<kD, kB, true, false>);
-        else bias ? go(attn_fwd_kernel<kD, kB, false, true>) : go(attn_fwd_kernel<kD, kB, false, false>);
+        auto join = [&](auto ways) {
+            constexpr int kW = decltype(ways)::value;
+            hipLaunchKernelGGL((attn_join_kernel<kD, kB, kW>),
+                               dim3(ceil_div((int64_t)x.groups * x.rows, 2048 / (kD * kW))),
+                               dim3(256), 0, stream, x);
+        };
+        auto kinds = [&](auto cz, auto bi) {
+            constexpr bool kC = decltype(cz)::value, kBi = decltype(bi)::value;
+            if (f.token) go(attn_token_kernel<kD, kB, kC, kBi>);
+            else if (f.split == 2) go(attn_fwd_kernel<kD, kB, kC, kBi, 2>);
+            else go(attn_fwd_kernel<kD, kB, kC, kBi, 1>);
+        };
+        using T = std::true_type;
+        using F = std::false_type;
+        if (cap) bias ? kinds(T{}, T{}) : kinds(T{}, F{});
+        else bias ? kinds(F{}, T{}) : kinds(F{}, F{});
         if (f.splits > 1)
-            hipLaunchKernelGGL((attn_join_kernel<kD, kB>),
-                               dim3(ceil_div((int64_t)x.groups * x.rows, 2048 / kD)), dim3(256), 0,
-                               stream, x);
+            f.splits >= 8 ? join(std::integral_constant<int, 512 / kD>{})
+                          : join(std::integral_constant<int, 1>{});
     };
     using T = std::true_type;
     using F = std::false_type;

@@ -57,7 +57,9 @@ constexpr int kAttnRows = 128;  // rows (or keys) resident per workgroup
 inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 struct AttnFwdPlan {
-    int tiles;   // 128-row tiles of a KV head's group * sq rows
+    bool token;  // the kernel for few rows
+    int split;   // otherwise: workgroups of 128 / split rows
+    int tiles;   // row tiles of a KV head's group * sq rows
     int splits;  // parts of the key axis
     int part;    // 64-key tiles per part
     int jobs;

@@ -36,17 +36,32 @@ struct FwdCfg {
 };
 
 // A wave's 32 rows: what they see, and their running softmax and output.
+//
+// The vector units bound the tile loop, so an element's score stays as it
+// leaves its products as long as it can: the log2-domain score is
+//   x = al raw + be[n],  al > 0
+// with al, be the tile's -- raw the dot product (al = c), with a distance bias
+// linear over the tile the product seeded by the bias's slope (be its value
+// at the tile's first key), capped -1 / (exp(2 s / softcap) + 1) (al = 2 cap2,
+// be = cap2).  Maxima are taken over raw, and p = exp2(al raw + (be - mx)) is
+// one fma and the exponential.
+//
+// mx need not be the maximum: sums and outputs are rescaled only where a
+// tile's maximum exceeds it by 2^kLazy, so p and the sums stay below 2^8 times
+// their usual size, far inside fp16's and fp32's ranges.  With the exact
+// maximum some row of the 32 rescales all of them in nearly every early tile.
 template <int D, bool kBf16, bool kCap, bool kBias>
 struct FwdRows {
     typedef AttnFwdArgs Args;
     static constexpr int kKs = D / 32, kDB = D / 16;
-    static constexpr bool kLog2 = kCap || kBias;  // scores leave their product in the log2 domain
+    static constexpr float kLazy = 8.f;
     f16x8 qf[2][kKs];
     int lim[2], id[2];
     float qp[2], slope[2];
     f32x4 o[kDB][2];  // columns 16 db + 4 g4 + e of rows 16 n + l16
     float mx[2], sum[2];
     int lim_min, lim_max;  // over the rows
+    int q_first, q_last;   // places of the first and last row among the keys
 
     // Rows row0 .. row0 + 31 of KV head hkv in batch entry b.
     template <typename A>
@@ -54,9 +69,12 @@ struct FwdRows {
                                          int off, int lane) {
         const int l16 = lane & 15, g4 = lane >> 4;
         const bool any = row0 < a.rows;
-        const int last = min(row0 + 32, a.rows) - 1;
-        lim_min = any ? attn_limit(fdiv(a.div_group, row0), off, kv, a.m.causal, prefix) : 0x7fffffff;
-        lim_max = any ? attn_limit(fdiv(a.div_group, last), off, kv, a.m.causal, prefix) : 0;
+        const int first = fdiv(a.div_group, any ? row0 : 0);
+        const int last = fdiv(a.div_group, any ? min(row0 + 32, a.rows) - 1 : 0);
+        lim_min = any ? attn_limit(first, off, kv, a.m.causal, prefix) : 0x7fffffff;
+        lim_max = any ? attn_limit(last, off, kv, a.m.causal, prefix) : 0;
+        q_first = first + off;
+        q_last = last + off;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             const AttnRow r = attn_row(row0 + 16 * n + l16, a.rows, hkv, a.group, a.div_group);
@@ -83,29 +101,50 @@ struct FwdRows {
     }
 
     // Keys j0 .. j0 + 16 M - 1, which are rows 16 m0 .. of the tiles tk and tv.
-    // full: every row sees every one of them.  ids: their documents in LDS, or null.
+    // ids: their documents in LDS, or null where all rows are of theirs.
     template <int M>
     __device__ __forceinline__ void step(const RegReader<D>& rd0, const FA3_LDS char* tk,
-                                         const FA3_LDS char* tv, int m0, int j0, bool full,
+                                         const FA3_LDS char* tv, int m0, int j0,
                                          const FA3_LDS char* ids, float c) {
         RegReader<D> rd = rd0;
         rd.opaque();
+        const bool limited = j0 + 16 * M > lim_min;
         f32x4 s[M][2];  // [m][n]: keys 16 m + 4 g4 + e, rows 16 n + l16
-#pragma unroll
-        for (int m = 0; m < M; ++m) s[m][0] = s[m][1] = f32x4{};
-        // (the bias-free, cap-free score is masked in its product's seed: its
-        // scale is positive, and nothing that can be masked is infinite)
-        auto mask = [&]() {
-            const int ln = opaque_tid() & 63;
-            const int jl = j0 + 4 * (ln >> 4);
+        float al = c, be[2] = {0.f, 0.f};
+        bool linear = false;  // every row of the wave on one side of every key
+        if constexpr (kBias && !kCap) {
+            const bool past = q_first >= j0 + 16 * M - 1;
+            linear = (past || q_last <= j0) && c > 1e-30f;
+            const float j = (float)(j0 + 4 * ((opaque_tid() & 63) >> 4));
+            const float inv = linear ? __builtin_amdgcn_rcpf(past ? c : -c) : 0.f;
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-                const int k = lim[n] - jl;
+                const float seed = slope[n] * inv;
+                if (linear) be[n] = -slope[n] * __builtin_fabsf(qp[n] - j);
 #pragma unroll
                 for (int m = 0; m < M; ++m)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        s[m][n][e] = 16 * m + e < k ? s[m][n][e] : kNegInf;
+                    for (int e = 0; e < 4; ++e) s[m][n][e] = seed * (float)(16 * m + e);
+            }
+        } else {
+#pragma unroll
+            for (int m = 0; m < M; ++m) s[m][0] = s[m][1] = f32x4{};
+        }
+        // (a score without a cap is masked in its product's seed: al is
+        // positive, and nothing that can be masked is infinite)
+        auto mask = [&]() {
+            const int ln = opaque_tid() & 63;
+            if (limited) {
+                const int jl = j0 + 4 * (ln >> 4);
+#pragma unroll
+                for (int n = 0; n < 2; ++n) {
+                    const int k = lim[n] - jl;
+#pragma unroll
+                    for (int m = 0; m < M; ++m)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            s[m][n][e] = 16 * m + e < k ? s[m][n][e] : kNegInf;
+                }
             }
             if (ids != nullptr) {
                 const FA3_LDS i32x4* kids = (const FA3_LDS i32x4*)ids + (ln >> 4);
@@ -120,12 +159,13 @@ struct FwdRows {
                 }
             }
         };
-        if (!kLog2 && !full) mask();
+        if (!kCap && !(kBias && !linear)) mask();
         attn_scores<D, kBf16, M, 4>(rd, tk, m0, qf, s);
         if constexpr (kCap) {
             const auto& a = attn_args<Args>();
             const float k1 = a.m.k1, cap2 = a.m.cap2;
             if (a.m.cap_fine) {
+                al = 1.f;
 #pragma unroll
                 for (int m = 0; m < M; ++m)
 #pragma unroll
@@ -134,56 +174,62 @@ struct FwdRows {
                         for (int e = 0; e < 4; ++e)
                             s[m][n][e] = attn_tanh_fine(s[m][n][e], k1) * cap2;
             } else {
+                al = 2.f * cap2;
+                be[0] = be[1] = cap2;
 #pragma unroll
                 for (int m = 0; m < M; ++m)
 #pragma unroll
                     for (int n = 0; n < 2; ++n)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            s[m][n][e] = attn_tanh(s[m][n][e], k1) * cap2;
+                            s[m][n][e] = __builtin_amdgcn_rcpf(-1.f - fast_exp2(s[m][n][e] * k1));
             }
         }
         if constexpr (kBias) {
-            const int g4 = (opaque_tid() & 63) >> 4;
+            if (!linear) {
+                const float j = (float)(j0 + 4 * ((opaque_tid() & 63) >> 4));
 #pragma unroll
-            for (int n = 0; n < 2; ++n) {
-                const float d0 = qp[n] - (float)(j0 + 4 * g4);
+                for (int n = 0; n < 2; ++n) {
+                    // (uncapped: the seed taken off again with the bias)
+                    const float d0 = qp[n] - j, b0 = be[n];
 #pragma unroll
-                for (int m = 0; m < M; ++m)
+                    for (int m = 0; m < M; ++m)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        const float x = kCap ? s[m][n][e] : s[m][n][e] * c;
-                        s[m][n][e] = __builtin_fmaf(-slope[n], __builtin_fabsf(d0 - (float)(16 * m + e)), x);
-                    }
+                        for (int e = 0; e < 4; ++e)
+                            s[m][n][e] = __builtin_fmaf(-slope[n], __builtin_fabsf(d0 - (float)(16 * m + e)),
+                                                        __builtin_fmaf(s[m][n][e], al, b0));
+                    be[n] = 0.f;
+                }
+                al = 1.f;
             }
         }
-        if (kLog2 && !full) mask();
-        float mu[2];
+        if (kCap || (kBias && !linear)) mask();
+        float top[2];
         bool up = false;
-        float mn[2];
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            float x = mx[n];
+            float x = s[0][n][0];
 #pragma unroll
             for (int m = 0; m < M; ++m)
 #pragma unroll
                 for (int e = 0; e < 4; ++e) x = __builtin_fmaxf(x, s[m][n][e]);
-            mn[n] = max_groups(x);
-            up |= mn[n] > mx[n];
-            mu[n] = mn[n] == kNegInf ? 0.f : mn[n];
-            if (!kLog2) mu[n] *= c;
+            top[n] = max_groups(__builtin_fmaf(al, x, be[n]));
+            up |= top[n] > mx[n] + kLazy;
         }
         if (__ballot(up)) {
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
-                // (mx -inf: exp2(-inf) = 0; both -inf: mu 0, the same)
-                const float f = fast_exp2(kLog2 ? mx[n] - mu[n] : __builtin_fmaf(mx[n], c, -mu[n]));
-                mx[n] = mn[n];
+                const float m = __builtin_fmaxf(mx[n], top[n]);
+                // (mx -inf: nothing seen before, 0 times its zeros)
+                const float f = mx[n] == kNegInf ? 0.f : fast_exp2(mx[n] - m);
+                mx[n] = m;
                 sum[n] *= f;
 #pragma unroll
                 for (int i = 0; i < kDB; ++i) o[i][n] *= f;
             }
         }
+#pragma unroll
+        for (int n = 0; n < 2; ++n) be[n] -= mx[n] == kNegInf ? 0.f : mx[n];
 #pragma unroll
         for (int r = 0; r < M / 2; ++r) {
             f16x8 bp[2];
@@ -192,8 +238,7 @@ struct FwdRows {
                 float p[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const float x = s[2 * r + (j >> 2)][n][j & 3];
-                    p[j] = fast_exp2(kLog2 ? x - mu[n] : __builtin_fmaf(x, c, -mu[n]));
+                    p[j] = fast_exp2(__builtin_fmaf(s[2 * r + (j >> 2)][n][j & 3], al, be[n]));
                     sum[n] += p[j];
                 }
                 bp[n] = pack8<kBf16>(p);
@@ -207,7 +252,7 @@ struct FwdRows {
     // D / 16 * 2 KiB + 512 a wave of rs > 0.
     template <int kSplit>
     __device__ __forceinline__ void meet(FA3_LDS float* x, FA3_LDS char* slots, int w, int qb,
-                                         int rs, float c) {
+                                         int rs) {
         constexpr int kQb = kRegWaves / kSplit, kSlot = kDB * 2048 + 512;
         const int ln = opaque_tid() & 63;
 #pragma unroll
@@ -221,7 +266,7 @@ struct FwdRows {
             for (int k = 0; k < kSplit; ++k)
                 top = __builtin_fmaxf(top, x[(2 * (qb + kQb * k) + n) * 64 + ln]);
             const float mu = top == kNegInf ? 0.f : top;
-            const float f = fast_exp2(kLog2 ? mx[n] - mu : (mx[n] - mu) * c);
+            const float f = fast_exp2(mx[n] - mu);
             mx[n] = top;
             sum[n] *= f;
 #pragma unroll
@@ -263,7 +308,7 @@ struct FwdRows {
 #pragma unroll
                 for (int i = 0; i < kDB; ++i) o[i][n] = f32x4{};
             }
-            lse2[n] = none ? kNegInf : (kLog2 ? mx[n] : mx[n] * z.m.c) + __builtin_amdgcn_logf(l);
+            lse2[n] = none ? kNegInf : mx[n] + __builtin_amdgcn_logf(l);
         }
         if (z.splits > 1) {
             const int64_t base = ((int64_t)split * z.groups + grp) * z.rows;
@@ -367,10 +412,9 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(
             constexpr int kKeys = 64 / kSplit;
             const int j0 = t * 64 + kKeys * rs;
             if (j0 < rows.lim_max)
-                rows.template step<4 / kSplit>(rd, st, st + C::kTileBytes, kKeys / 16 * rs, j0,
-                                               j0 + kKeys <= rows.lim_min && (cls & kTileSame),
-                                               ids == nullptr ? nullptr : st + 2 * C::kTileBytes + 4 * kKeys * rs,
-                                               c);
+                rows.template step<4 / kSplit>(
+                    rd, st, st + C::kTileBytes, kKeys / 16 * rs, j0,
+                    cls & kTileSame ? nullptr : st + 2 * C::kTileBytes + 4 * kKeys * rs, c);
         }
         t = tn;
     };
@@ -384,7 +428,7 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(
     const FwdJob e = fwd_job(attn_args<Args>(), blockIdx.x);  // (decoded again: not held over the loop)
     const int ew = __builtin_amdgcn_readfirstlane(opaque_tid() >> 6), eqb = ew & (kQb - 1);
     if constexpr (kSplit > 1) {
-        rows.template meet<kSplit>((FA3_LDS float*)smem, smem + 2048, ew, eqb, ew / kQb, c);
+        rows.template meet<kSplit>((FA3_LDS float*)smem, smem + 2048, ew, eqb, ew / kQb);
         if (ew / kQb > 0) return;
     }
     // (of the meeting, this wave reads only what it has read: its own block's slots)
@@ -473,7 +517,7 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 2 : 1) void attn_token_kerne
         __atomic_signal_fence(__ATOMIC_SEQ_CST);
         wall();
         const int j0 = 32 * (first + 4 * x);
-        rows.template step<2>(rd, st, st + C::kBlock, 0, j0, j0 + 32 <= rows.lim_min, nullptr, c);
+        rows.template step<2>(rd, st, st + C::kBlock, 0, j0, nullptr, c);
         ++x;
     };
     while (x < n) {
@@ -485,7 +529,7 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 2 : 1) void attn_token_kerne
     barrier();
     const FwdJob e = fwd_job(attn_args<Args>(), blockIdx.x);
     const int ew = __builtin_amdgcn_readfirstlane(opaque_tid() >> 6);
-    rows.template meet<4>((FA3_LDS float*)smem, smem + 2048, ew, 0, ew, c);
+    rows.template meet<4>((FA3_LDS float*)smem, smem + 2048, ew, 0, ew);
     if (ew > 0) return;
     rows.finish(0, e.b, e.hkv, e.grp, e.split, smem + 2048);
 }
@@ -638,10 +682,9 @@ hipError_t launch_attn_fwd(const AttnProblem& p, const ShaoboFa3AttnParams& a, A
     x.div_gpart = make_fastdiv(x.groups / 8);
     x.div_splits = make_fastdiv(f.splits);
     const bool cap = p.softcap > 0.f, bias = p.bias;
-    // The running maximum is taken over raw products where nothing else
-    // enters the score: its scale must be positive.
+    // Maxima are taken over raw products: their scale must be positive.
     x.scored = 1;
-    if (!cap && !bias) {
+    if (!cap) {
         if (m.c < 0.f) x.flip = 0x80008000u;
         x.scored = m.c != 0.f;
         m.c = m.c == 0.f ? 1.f : m.c < 0.f ? -m.c : m.c;

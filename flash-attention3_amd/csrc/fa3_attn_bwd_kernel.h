@@ -148,7 +148,7 @@ __device__ __forceinline__ void attn_dkv(int b, int hkv, int level, FA3_LDS char
     const int len = end - begin;
     TileWalk walk(docs ? a.m.range_q + (int64_t)b * a.m.blocks_q : nullptr,
                   begin + len * row_part / a.row_parts, begin + len * (row_part + 1) / a.row_parts,
-                  doc);
+                  doc, end);
     const int g_first = a.group * head_part / a.head_parts;
     const int g_end = a.group * (head_part + 1) / a.head_parts;
     int t = walk.next(), g = g_first;  // the step being computed: query tile and head of the group
@@ -416,7 +416,7 @@ __device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* 
     const _Float16* vp = a.v.p + b * a.v.bs + hkv * a.v.hs;
     const int* ids = a.m.doc_k == nullptr ? nullptr : a.m.doc_k + b * a.m.doc_k_bs;
     TileWalk walk(ids == nullptr ? nullptr : a.m.range_k + (int64_t)b * a.m.blocks_k, 0,
-                  (wg_max + 63) >> 6, doc);
+                  (wg_max + 63) >> 6, doc, 1 << 30);
     auto issue = [&](FA3_LDS char* st, int t) {
         const int j0 = t * 64, ln = opaque_tid() & 63;
         const auto& a = attn_args<Args>();

@@ -109,19 +109,29 @@ constexpr int kTileMeets = 1;   // the tile's documents can meet this wave's
 constexpr int kTileSame = 2;    // both have one document, the same
 constexpr int kTileHidden = 4;  // the tile has positions of no document
 struct TileWalk {
-    const AttnRange* ranges;  // of this batch entry; null: every tile
+    const AttnRange* ranges;  // of this batch entry; null: every tile, from `near` down, then up
     int at, end;              // next tile (ranges: next tile to look up)
+    int begin, up;
     int base;
     uint64_t live;            // of the tiles base .. base + 63
     DocSpan doc;
     int cls;                  // kTile* of the tile last returned
 
-    __device__ __forceinline__ TileWalk(const AttnRange* r, int begin, int end_, const DocSpan& d)
-        : ranges(r), at(begin), end(end_), base(begin), live(0), doc(d),
-          cls(kTileMeets | kTileSame) {}
+    __device__ __forceinline__ TileWalk(const AttnRange* r, int begin_, int end_, const DocSpan& d,
+                                        int near)
+        : ranges(r), at(begin_), end(end_), begin(begin_), base(begin_), live(0), doc(d),
+          cls(kTileMeets | kTileSame) {
+        near = near < end_ - 1 ? near : end_ - 1;
+        if (ranges == nullptr && near >= begin_) at = near;
+        if (ranges == nullptr && begin_ >= end_) at = -1;
+        up = near >= begin_ ? near + 1 : begin_ + 1;
+    }
     // the next tile, or -1
     __device__ __forceinline__ int next() {
-        if (ranges == nullptr) return at < end ? at++ : -1;
+        if (ranges == nullptr) {
+            if (at >= begin) return at--;
+            return up < end ? up++ : -1;
+        }
         while (live == 0) {
             if (at >= end) return -1;
             base = at;

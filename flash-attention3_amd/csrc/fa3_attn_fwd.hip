@@ -55,6 +55,10 @@ struct FwdRows {
     typedef AttnFwdArgs Args;
     static constexpr int kKs = D / 32, kDB = D / 16;
     static constexpr float kLazy = 8.f;
+    // A tile whose every p is below 2^-64 of its row's largest is left: 2^30
+    // keys of them, the longest axis, add less than 2^-34, fp32's half step
+    // being 2^-25.  (Looked for only with a distance bias, which makes them.)
+    static constexpr float kNone = 64.f;
     f16x8 qf[2][kKs];
     int lim[2], id[2];
     float qp[2], slope[2];
@@ -205,17 +209,20 @@ struct FwdRows {
         }
         if (kCap || (kBias && !linear)) mask();
         float top[2];
-        bool up = false;
+        bool up = false, some = false;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             float x = s[0][n][0];
 #pragma unroll
             for (int m = 0; m < M; ++m)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) x = __builtin_fmaxf(x, s[m][n][e]);
+                for (int e = 0; e < 4; ++e)  // (v_maximum3: no canonicalising before it)
+                    x = __builtin_elementwise_maximum(x, s[m][n][e]);
             top[n] = max_groups(__builtin_fmaf(al, x, be[n]));
             up |= top[n] > mx[n] + kLazy;
+            some |= top[n] > mx[n] - kNone;
         }
+        if (kBias && !__ballot(some)) return;
         if (__ballot(up)) {
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
@@ -381,8 +388,11 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(
     const _Float16* vp = a.v.p + b * a.v.bs + hkv * a.v.hs;
     const int* ids = a.m.doc_k == nullptr ? nullptr : a.m.doc_k + b * a.m.doc_k_bs;
     const int begin = job.split * a.part;
+    // (the workgroup's own place among the keys: with a distance bias the
+    // nearest tiles first, which leave little to rescale and much to skip)
+    const int rows_at = fdiv(a.div_group, wg_last) + off;
     TileWalk walk(ids == nullptr ? nullptr : a.m.range_k + (int64_t)b * a.m.blocks_k, begin,
-                  min(begin + a.part, (wg_max + 63) >> 6), doc);
+                  min(begin + a.part, (wg_max + 63) >> 6), doc, rows_at >> 6);
     auto issue = [&](FA3_LDS char* st, int t) {
         const int j0 = t * 64, lane = opaque_tid() & 63;
         const auto& a = attn_args<Args>();

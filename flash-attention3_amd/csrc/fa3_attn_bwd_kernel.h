@@ -37,7 +37,7 @@ template <typename Args>
 __device__ __forceinline__ BwdJob bwd_job(const Args& a, int id) {
     BwdJob j;
     int grp;
-    attn_job(id, a.groups, a.div_groups, a.div_gpart, j.level, grp);
+    attn_job(id, a.groups, a.by_group, a.div_groups, a.div_gpart, a.div_levels, a.levels, j.level, grp);
     j.b = fdiv(a.div_hkv, grp);
     j.hkv = grp - j.b * a.heads_kv;
     return j;

@@ -328,17 +328,26 @@ __device__ __forceinline__ void attn_store(const f32x4 (*acc)[2], const float (&
     }
 }
 
-// Jobs are numbered [level][group]; XCD x runs the workgroups with id % 8 ==
-// x.  With a multiple of 8 groups ((batch, KV head) pairs) an XCD takes whole
-// groups, so that a group's keys stay in one L2; either way the first levels
-// start first.
+// Workgroup id's job.  XCD x runs the workgroups with id % 8 == x.  With a
+// multiple of 8 groups ((batch, KV head) pairs) an XCD takes every eighth one
+// whole, so that its keys stay in one L2: level by level over its groups, so
+// that the longest jobs start first, or (by_group, for jobs of one length) one
+// group after the other.  Otherwise jobs go level by level over all groups.
 template <typename Div>
-__device__ __forceinline__ void attn_job(int id, int groups, const Div& div_groups,
-                                         const Div& div_part, int& level, int& group) {
+__device__ __forceinline__ void attn_job(int id, int groups, bool by_group, const Div& div_groups,
+                                         const Div& div_part, const Div& div_levels, int levels,
+                                         int& level, int& group) {
     if (groups % 8 == 0) {
         const int part = groups / 8, pos = id / 8;
-        level = fdiv(div_part, pos);
-        group = (id % 8) * part + pos - level * part;
+        int g;
+        if (by_group) {
+            g = fdiv(div_levels, pos);
+            level = pos - g * levels;
+        } else {
+            level = fdiv(div_part, pos);
+            g = pos - level * part;
+        }
+        group = id % 8 + 8 * g;
     } else {
         level = fdiv(div_groups, id);
         group = id - level * groups;

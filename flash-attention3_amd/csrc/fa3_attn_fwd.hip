@@ -23,7 +23,8 @@ struct AttnFwdArgs {
     int tiles, splits, part, groups;
     uint32_t flip;  // XORed into Q's 16-bit pairs
     int scored;     // 0: a scale of zero, Q is taken as zeros
-    FastDiv div_hkv, div_group, div_groups, div_gpart, div_splits;
+    int levels, by_group;
+    FastDiv div_hkv, div_group, div_groups, div_gpart, div_splits, div_levels;
 };
 
 template <int D>
@@ -352,7 +353,7 @@ template <typename A>
 __device__ __forceinline__ FwdJob fwd_job(const A& a, int id) {
     FwdJob j;
     int level;
-    attn_job(id, a.groups, a.div_groups, a.div_gpart, level, j.grp);
+    attn_job(id, a.groups, a.by_group, a.div_groups, a.div_gpart, a.div_levels, a.levels, level, j.grp);
     j.b = fdiv(a.div_hkv, j.grp);
     j.hkv = j.grp - j.b * a.heads_kv;
     const int tl = fdiv(a.div_splits, level);
@@ -691,6 +692,14 @@ hipError_t launch_attn_fwd(const AttnProblem& p, const ShaoboFa3AttnParams& a, A
     x.div_groups = make_fastdiv(x.groups);
     x.div_gpart = make_fastdiv(x.groups / 8);
     x.div_splits = make_fastdiv(f.splits);
+    x.levels = f.tiles * f.splits;
+    x.div_levels = make_fastdiv(x.levels);
+    // Causal jobs differ in length by their place: longest first (B4 H16 S2048
+    // D128 88 us against 128 group after group).  Full ones do not, and with
+    // documents the place says little: a group's keys in one L2 count for more
+    // (B2 H16 S8192 D64 with bias 668 -> 551, B2 Hq32 Hkv8 S4096 with
+    // documents 250 -> 199).
+    x.by_group = !p.causal || p.docs;
     const bool cap = p.softcap > 0.f, bias = p.bias;
     // Maxima are taken over raw products: their scale must be positive.
     x.scored = 1;

@@ -121,22 +121,12 @@ __device__ __forceinline__ void attn_dkv(int b, int hkv, int level, FA3_LDS char
     const int rs = w / kKb;
     const int wg_key = tile * (32 * kKb), key0 = wg_key + 32 * (w & (kKb - 1));
 
-    f16x8 kf[2][C::kKs], vf[2][C::kKs];
     int id[2];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
         const int j = key0 + 16 * n + l16;
         id[n] = -2;
         if (a.m.doc_k != nullptr && j < kv) id[n] = max(a.m.doc_k[b * a.m.doc_k_bs + j], -1);
-        const bool ok = j < kv && id[n] != -1;
-        const int64_t r = j < kv ? j : 0;
-        const _Float16* k = a.k.p + b * a.k.bs + hkv * a.k.hs + r * a.k.rs;
-        const _Float16* v = a.v.p + b * a.v.bs + hkv * a.v.hs + r * a.v.rs;
-#pragma unroll
-        for (int s = 0; s < C::kKs; ++s) {
-            kf[n][s] = attn_row8(k, p1_chunk<D>(s, g4), a.d, ok);
-            vf[n][s] = attn_row8(v, p1_chunk<D>(s, g4), a.d, ok);
-        }
     }
     DocSpan doc{0, 0, 0, 0, false};
     const bool docs = a.m.doc_k != nullptr;
@@ -151,8 +141,24 @@ __device__ __forceinline__ void attn_dkv(int b, int hkv, int level, FA3_LDS char
                   doc, end);
     const int g_first = a.group * head_part / a.head_parts;
     const int g_end = a.group * (head_part + 1) / a.head_parts;
-    int t = walk.next(), g = g_first;  // the step being computed: query tile and head of the group
-    int ld_t = t, ld_g = g_first;      // the step being loaded
+    // The step being computed -- query tile and head of the group -- and the
+    // one to load.  The next one is looked up before the barrier, so that its
+    // words are there when its loads go out.
+    int t, g, cls;
+    int ld_t = walk.next(), ld_g = g_first, ld_idle = 0;
+    auto lookup = [&]() {
+        if (ld_t < 0) return;
+        const auto& a = attn_args<Args>();
+        const int h = hkv * a.group + ld_g;
+        ld_idle = scalar_load(a.flags + (((int64_t)b * a.heads_q + h) * (a.sqp >> 6) + ld_t));
+    };
+    auto take = [&]() {
+        t = ld_t;
+        g = ld_g;
+        cls = walk.cls;
+    };
+    lookup();
+    take();
     auto issue = [&](FA3_LDS char* st) {
         const int ln = opaque_tid() & 63, i0 = ld_t * 64, h = hkv * attn_args<Args>().group + ld_g;
         int64_t row;  // of the statistics
@@ -160,7 +166,7 @@ __device__ __forceinline__ void attn_dkv(int b, int hkv, int level, FA3_LDS char
         {
             const auto& a = attn_args<Args>();
             row = ((int64_t)b * a.heads_q + h) * a.sqp + i0;
-            whole = a.d == D && a.flags[row >> 6] == 0;
+            whole = a.d == D && ld_idle == 0;
         }
         auto load = [&](FA3_LDS char* tile, const auto& x) {
             const _Float16* p = x.p + b * x.bs + h * x.hs;
@@ -184,6 +190,23 @@ __device__ __forceinline__ void attn_dkv(int b, int hkv, int level, FA3_LDS char
         else if (w == 2 && a.m.doc_q != nullptr)
             attn_load_ids(st + C::kIdsOff, a.m.doc_q + b * a.m.doc_q_bs, i0, a.sq, ln);
     };
+    FA3_LDS char* s0 = smem;
+    FA3_LDS char* s1 = smem + C::kStageBytes;
+    if (t >= 0) issue(s0);
+    f16x8 kf[2][C::kKs], vf[2][C::kKs];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const int j = key0 + 16 * n + l16;
+        const bool ok = j < kv && id[n] != -1;
+        const int64_t r = j < kv ? j : 0;
+        const _Float16* k = a.k.p + b * a.k.bs + hkv * a.k.hs + r * a.k.rs;
+        const _Float16* v = a.v.p + b * a.v.bs + hkv * a.v.hs + r * a.v.rs;
+#pragma unroll
+        for (int s = 0; s < C::kKs; ++s) {
+            kf[n][s] = attn_row8(k, p1_chunk<D>(s, g4), a.d, ok);
+            vf[n][s] = attn_row8(v, p1_chunk<D>(s, g4), a.d, ok);
+        }
+    }
     f32x4 av[C::kDB][2], ak[C::kDB][2];
 #pragma unroll
     for (int i = 0; i < C::kDB; ++i) {
@@ -244,18 +267,19 @@ __device__ __forceinline__ void attn_dkv(int b, int hkv, int level, FA3_LDS char
             dp[m][0] = dp[m][1] = rows[16 + 4 * m];
             s[m][0] = s[m][1] = f32x4{};
         }
-        reg_scores<D, kBf16, AttnAhead<D, kCap>>(rd, st, st + R::kTileBytes, r, kf, vf, s, dp);
+        reg_scores<D, kBf16, AttnAhead<D, D == 128 ? kCap || kBias : kFine>>(rd, st, st + R::kTileBytes, r, kf, vf, s, dp);
         nl[0] = rows[0];
         nl[1] = rows[4];
-        float k1 = 0.f, cap2 = 0.f, slope = 0.f;
+        float slope = 0.f;
+        if constexpr (kBias) {
+            const auto& a = attn_args<Args>();
+            slope = scalar_load(a.m.slopes + (b * a.m.slopes_bs + hkv * a.group + g)) * kLog2e;
+        }
+        float k1 = 0.f, cap2 = 0.f;
         if constexpr (kCap) {
             const auto& a = attn_args<Args>();
             k1 = a.m.k1;
             cap2 = a.m.cap2;
-        }
-        if constexpr (kBias) {
-            const auto& a = attn_args<Args>();
-            slope = a.m.slopes[b * a.m.slopes_bs + hkv * a.group + g] * kLog2e;
         }
         float p[2][8], ds[2][8];  // [n][4 m + e]
         const int ln = opaque_tid() & 63;
@@ -275,22 +299,16 @@ __device__ __forceinline__ void attn_dkv(int b, int hkv, int level, FA3_LDS char
         }
         const f16x8 bp[2] = {pack8<kBf16>(p[0]), pack8<kBf16>(p[1])};
         const f16x8 bs[2] = {pack8<kBf16>(ds[0]), pack8<kBf16>(ds[1])};
-        reg_grads<D, kBf16, true, AttnAhead<D, kCap>>(rd, st + R::kTileBytes, st, r, bp, bs, av, ak);
+        reg_grads<D, kBf16, true, AttnAhead<D, D == 128 ? kCap || kBias : kFine>>(rd, st + R::kTileBytes, st, r, bp, bs, av, ak);
     };
-    FA3_LDS char* s0 = smem;
-    FA3_LDS char* s1 = smem + C::kStageBytes;
-    int cls = walk.cls;  // of the tile being computed
-    auto advance = [&]() {
+    auto stage = [&](FA3_LDS char* __restrict__ ld, const FA3_LDS char* __restrict__ st) {
         if (++ld_g == g_end) {
             ld_g = g_first;
             ld_t = walk.next();
         }
-    };
-    if (t >= 0) issue(s0);
-    auto stage = [&](FA3_LDS char* __restrict__ ld, const FA3_LDS char* __restrict__ st) {
+        lookup();
         wait_vm_lgkm0<0>();
         barrier();
-        advance();
         if (ld_t >= 0) issue(ld);
         if (cls & kTileMeets) {
             if constexpr (kSplit == 1) {
@@ -300,9 +318,7 @@ __device__ __forceinline__ void attn_dkv(int b, int hkv, int level, FA3_LDS char
                 sub(st, rs, cls & kTileSame);
             }
         }
-        t = ld_t;
-        g = ld_g;
-        cls = walk.cls;
+        take();
     };
     while (t >= 0) {
         stage(s1, s0);
@@ -380,34 +396,13 @@ __device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* 
     const int lim_max = any ? attn_limit(fdiv(a.div_group, last), off, kv, causal, prefix) : 0;
     const int wg_max = attn_limit(fdiv(a.div_group, wg_last), off, kv, causal, prefix);
 
-    f16x8 qf[2][C::kKs], df[2][C::kKs];
-    float nl[2], qp[2], slope[2];
-    f32x4 nd[2];
     int lim[2], id[2];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
         const AttnRow r = attn_row(row0 + 16 * n + l16, a.rows, hkv, a.group, a.div_group);
-        const int64_t at = ((int64_t)b * a.heads_q + r.h) * a.sqp + r.i;
-        nl[n] = r.ok ? a.nlse2[at] : kNegInf;
-        const float x = r.ok ? a.ndelta[at] : 0.f;
-        nd[n] = f32x4{x, x, x, x};
-        const bool ok = nl[n] != kNegInf;
-        const _Float16* q = a.q.p + b * a.q.bs + r.h * a.q.hs + r.i * a.q.rs;
-        const _Float16* o = a.dout.p + b * a.dout.bs + r.h * a.dout.hs + r.i * a.dout.rs;
-#pragma unroll
-        for (int s = 0; s < C::kKs; ++s) {
-            qf[n][s] = attn_row8(q, p1_chunk<D>(s, g4), a.d, ok);
-            df[n][s] = attn_row8(o, p1_chunk<D>(s, g4), a.d, ok);
-        }
         lim[n] = r.ok ? attn_limit(r.i, off, kv, causal, prefix) : 0;
         id[n] = -2;
         if (a.m.doc_q != nullptr && r.ok) id[n] = max(a.m.doc_q[b * a.m.doc_q_bs + r.i], -1);
-        qp[n] = 0.f;
-        slope[n] = 0.f;
-        if constexpr (kBias) {
-            qp[n] = (float)(r.i + off);
-            slope[n] = a.m.slopes[b * a.m.slopes_bs + r.h] * kLog2e;
-        }
     }
     DocSpan doc{0, 0, 0, 0, false};
     if (a.m.doc_q != nullptr) doc = doc_span(id, (FA3_LDS int*)(smem + C::kRangeOff), w, lane);
@@ -430,6 +425,35 @@ __device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* 
         }
         if (ids != nullptr && w == 0) attn_load_ids(st + C::kIdsOff, ids, j0, a.sk, ln);
     };
+    FA3_LDS char* s0 = smem;
+    FA3_LDS char* s1 = smem + C::kStageBytes;
+    int t = walk.next();
+    if (t >= 0) issue(s0, t);
+    f16x8 qf[2][C::kKs], df[2][C::kKs];
+    float nl[2], qp[2], slope[2];
+    f32x4 nd[2];
+#pragma unroll
+    for (int n = 0; n < 2; ++n) {
+        const AttnRow r = attn_row(row0 + 16 * n + l16, a.rows, hkv, a.group, a.div_group);
+        const int64_t at = ((int64_t)b * a.heads_q + r.h) * a.sqp + r.i;
+        nl[n] = r.ok ? a.nlse2[at] : kNegInf;
+        const float x = r.ok ? a.ndelta[at] : 0.f;
+        nd[n] = f32x4{x, x, x, x};
+        const bool ok = nl[n] != kNegInf;
+        const _Float16* q = a.q.p + b * a.q.bs + r.h * a.q.hs + r.i * a.q.rs;
+        const _Float16* o = a.dout.p + b * a.dout.bs + r.h * a.dout.hs + r.i * a.dout.rs;
+#pragma unroll
+        for (int s = 0; s < C::kKs; ++s) {
+            qf[n][s] = attn_row8(q, p1_chunk<D>(s, g4), a.d, ok);
+            df[n][s] = attn_row8(o, p1_chunk<D>(s, g4), a.d, ok);
+        }
+        qp[n] = 0.f;
+        slope[n] = 0.f;
+        if constexpr (kBias) {
+            qp[n] = (float)(r.i + off);
+            slope[n] = a.m.slopes[b * a.m.slopes_bs + r.h] * kLog2e;
+        }
+    }
     f32x4 acc[C::kDB][2];
 #pragma unroll
     for (int i = 0; i < C::kDB; ++i) acc[i][0] = acc[i][1] = f32x4{};
@@ -477,7 +501,7 @@ __device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* 
                 s[m][n] = f32x4{};
                 dp[m][n] = nd[n];
             }
-        reg_scores<D, kBf16, AttnAhead<D, kCap>>(rd, st, st + R::kTileBytes, r, qf, df, s, dp);
+        reg_scores<D, kBf16, AttnAhead<D, D == 128 ? kCap || kBias : kFine>>(rd, st, st + R::kTileBytes, r, qf, df, s, dp);
         float k1 = 0.f, cap2 = 0.f;
         if constexpr (kCap) {
             const auto& a = attn_args<Args>();
@@ -498,17 +522,12 @@ __device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* 
             }
         }
         const f16x8 bs[2] = {pack8<kBf16>(ds[0]), pack8<kBf16>(ds[1])};
-        reg_grads<D, kBf16, false, AttnAhead<D, kCap>>(rd, st, st, r, bs, bs, acc, acc);
+        reg_grads<D, kBf16, false, AttnAhead<D, D == 128 ? kCap || kBias : kFine>>(rd, st, st, r, bs, bs, acc, acc);
     };
-    FA3_LDS char* s0 = smem;
-    FA3_LDS char* s1 = smem + C::kStageBytes;
-    int t = walk.next();
-    if (t >= 0) issue(s0, t);
     auto stage = [&](FA3_LDS char* __restrict__ ld, const FA3_LDS char* __restrict__ st) {
-        const int cls = walk.cls;
+        const int cls = walk.cls, tn = walk.next();
         wait_vm_lgkm0<0>();
         barrier();
-        const int tn = walk.next();
         if (tn >= 0) issue(ld, tn);
         if (cls & kTileMeets) {
             if constexpr (kSplit == 1) {

@@ -102,6 +102,14 @@ __device__ __forceinline__ DocSpan doc_span(const int (&id)[2], FA3_LDS int* x, 
     return s;
 }
 
+// A word that no kernel running now writes, at an address that is the same in
+// all lanes, through the scalar cache.
+template <typename T>
+__device__ __forceinline__ T scalar_load(const T* p) {
+    typedef __attribute__((address_space(4))) const T K;
+    return *(K*)(uintptr_t)p;
+}
+
 // The tiles' walk: 64-position tiles t of [begin, end), those left out whose
 // documents cannot meet the workgroup's.  All lanes of all waves of a
 // workgroup step alike: a wave looks at the ranges of 64 tiles at a time.
@@ -151,8 +159,7 @@ struct TileWalk {
         // (read once more, through the scalar cache: held per lane, the ranges
         // would cost two vector registers over the whole loop, and a vector
         // load here is waited for before the next tile's loads go out)
-        typedef __attribute__((address_space(4))) const i32x2 KRange;
-        const i32x2 r = *(KRange*)(uintptr_t)(ranges + base + k);
+        const i32x2 r = scalar_load((const i32x2*)(ranges + base + k));
         const int x = r[0], hi = r[1], lo = x < 0 ? ~x : x;
         cls = (hi >= doc.lo && lo <= doc.hi ? kTileMeets : 0) |
               (x >= 0 && !doc.pad && lo == hi && doc.lo == doc.hi && lo == doc.lo ? kTileSame : 0) |
@@ -212,10 +219,10 @@ __device__ __forceinline__ f16x8 attn_row8(const _Float16* row, int c, int d, bo
 
 // Operands on their way in the backward's products (RegCfg): masks and score
 // options leave fewer registers for them at D 128.
-template <int D, bool kCap>
+template <int D, bool kScored>
 struct AttnAhead : RegCfg<D> {
     static constexpr int kAhead0 = 2;
-    static constexpr int kAhead1 = D == 128 && kCap ? 1 : 2;
+    static constexpr int kAhead1 = kScored ? 1 : 2;
     static constexpr int kAheadG = D == 128 ? 4 : 2;
 };
 
@@ -287,13 +294,13 @@ __device__ __forceinline__ int attn_limit(int i, int off, int kv, int causal, in
 template <typename M>
 __device__ __forceinline__ int attn_kv(const M& m, int b, int sk) {
     if (m.kv_lens == nullptr) return sk;
-    const int kv = __builtin_amdgcn_readfirstlane(m.kv_lens[b]);
+    const int kv = scalar_load(m.kv_lens + b);
     return kv < 0 ? 0 : kv < sk ? kv : sk;
 }
 template <typename M>
 __device__ __forceinline__ int attn_prefix(const M& m, int b) {
     if (m.prefix == nullptr) return 0;
-    const int n = __builtin_amdgcn_readfirstlane(m.prefix[b]);
+    const int n = scalar_load(m.prefix + b);
     return n > 0 ? n : 0;
 }
 

@@ -72,7 +72,7 @@ struct FwdRows {
     template <typename A>
     __device__ __forceinline__ void init(const A& a, int row0, int b, int hkv, int kv, int prefix,
                                          int off, int lane) {
-        const int l16 = lane & 15, g4 = lane >> 4;
+        const int l16 = lane & 15;
         const bool any = row0 < a.rows;
         const int first = fdiv(a.div_group, any ? row0 : 0);
         const int last = fdiv(a.div_group, any ? min(row0 + 32, a.rows) - 1 : 0);
@@ -83,15 +83,24 @@ struct FwdRows {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             const AttnRow r = attn_row(row0 + 16 * n + l16, a.rows, hkv, a.group, a.div_group);
+            lim[n] = r.ok ? attn_limit(r.i, off, kv, a.m.causal, prefix) : 0;
             id[n] = -2;
             // (documents: -1 for every negative one, -2 for rows that are not there)
             if (a.m.doc_q != nullptr && r.ok) id[n] = max(a.m.doc_q[b * a.m.doc_q_bs + r.i], -1);
+        }
+    }
+    // Their Q, after the first tile's loads have gone out.
+    template <typename A>
+    __device__ __forceinline__ void load(const A& a, int row0, int b, int hkv, int off, int lane) {
+        const int l16 = lane & 15, g4 = lane >> 4;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const AttnRow r = attn_row(row0 + 16 * n + l16, a.rows, hkv, a.group, a.div_group);
             const bool ok = r.ok && a.scored && id[n] != -1;
             const _Float16* q = a.q.p + b * a.q.bs + r.h * a.q.hs + r.i * a.q.rs;
 #pragma unroll
             for (int s = 0; s < kKs; ++s)  // (a scale below zero turns Q's signs)
                 qf[n][s] = attn_flip(attn_row8(q, p1_chunk<D>(s, g4), a.d, ok), a.flip);
-            lim[n] = r.ok ? attn_limit(r.i, off, kv, a.m.causal, prefix) : 0;
             qp[n] = 0.f;
             slope[n] = 0.f;
             if constexpr (kBias) {
@@ -413,11 +422,11 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(
     FA3_LDS char* s1 = smem + C::kStageBytes;
     int t = walk.next();
     if (t >= 0) issue(s0, t);
+    rows.load(a, (job.tile * kQb + qb) * 32, b, hkv, off, lane);
     auto stage = [&](FA3_LDS char* __restrict__ ld, const FA3_LDS char* __restrict__ st) {
-        const int cls = walk.cls;
+        const int cls = walk.cls, tn = walk.next();
         wait_vm_lgkm0<0>();
         barrier();
-        const int tn = walk.next();
         if (tn >= 0) issue(ld, tn);
         if (cls & kTileMeets) {
             constexpr int kKeys = 64 / kSplit;
@@ -512,6 +521,7 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 2 : 1) void attn_token_kerne
     if (n > 0) issue(s0, 0);
     FwdRows<D, kBf16, kCap, kBias> rows;
     rows.init(a, 0, b, hkv, kv, prefix, off, lane);
+    rows.load(a, 0, b, hkv, off, lane);
     const RegReader<D> rd(lane, 0);
     const float c = a.m.c;
     int x = 0;

@@ -1,8 +1,8 @@
 // Rotary positions on several axes for one or two tensors (q and k).
 //
 // A workgroup takes kTokens tokens (or one): it forms their cosines and sines
-// once, in LDS, and turns every head's row with them, 2 x 8 elements a
-// thread at a time.  Bound by HBM: x read once, written once.  Angles are
+// once, in LDS, and turns every head's row with them, 16 bytes (or 16 and
+// their partners') a thread at a time.  Bound by HBM: x read once, written once.  Angles are
 // sum_a positions[a] freqs[a][p] in fp64, reduced to [-1/2, 1/2] turns there:
 // at a million positions an fp32 product would be off by 0.06 radians.
 #include "fa3_attn_internal.h"
@@ -27,46 +27,43 @@ struct RotaryArgs {
     int64_t p_as, p_bs, p_rs;
     const float* freqs;
     int seqlen, total;  // batch * seqlen
-    int axes, pairs, units, inverse;  // units: 16-element pieces turned, and 8-element ones copied
+    int axes, pairs, inverse;
+    int units;  // of a row: 16-byte pieces turned (with their partners, where those lie apart) or copied
     int tokens;
     FastDiv div_seq, div_pairs, div_units, div_tokens;
 };
 
 constexpr int kRotaryThreads = 256;
 
+struct Half {};
+struct Bf {};
 template <typename T>
-struct Chunk {  // 8 elements
+struct Chunk {  // 16 bytes
+    static constexpr int kN = 8;
     f16x8 v;
 };
 template <>
 struct Chunk<float> {
-    f32x4 lo, hi;
+    static constexpr int kN = 4;
+    f32x4 v;
 };
-struct Half {};
-struct Bf {};
 
 template <typename T>
-__device__ __forceinline__ void to_f32(const Chunk<T>& c, float (&x)[8]) {
+__device__ __forceinline__ void to_f32(const Chunk<T>& c, float (&x)[Chunk<T>::kN]) {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if constexpr (std::is_same<T, float>::value) x[i] = i < 4 ? c.lo[i] : c.hi[i - 4];
-        else if constexpr (std::is_same<T, Bf>::value) x[i] = (float)__builtin_bit_cast(__bf16, (_Float16)c.v[i]);
+    for (int i = 0; i < Chunk<T>::kN; ++i) {
+        if constexpr (std::is_same<T, Bf>::value) x[i] = (float)__builtin_bit_cast(__bf16, (_Float16)c.v[i]);
         else x[i] = (float)c.v[i];
     }
 }
 template <typename T>
-__device__ __forceinline__ Chunk<T> from_f32(const float (&x)[8]) {
+__device__ __forceinline__ Chunk<T> from_f32(const float (&x)[Chunk<T>::kN]) {
     Chunk<T> c;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        if constexpr (std::is_same<T, float>::value) {
-            if (i < 4) c.lo[i] = x[i];
-            else c.hi[i - 4] = x[i];
-        } else if constexpr (std::is_same<T, Bf>::value) {
-            c.v[i] = __builtin_bit_cast(_Float16, (__bf16)x[i]);
-        } else {
-            c.v[i] = (_Float16)x[i];
-        }
+    for (int i = 0; i < Chunk<T>::kN; ++i) {
+        if constexpr (std::is_same<T, float>::value) c.v[i] = x[i];
+        else if constexpr (std::is_same<T, Bf>::value) c.v[i] = __builtin_bit_cast(_Float16, (__bf16)x[i]);
+        else c.v[i] = (_Float16)x[i];
     }
     return c;
 }
@@ -95,8 +92,8 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a, in
         turn[i] = make_float2(cs, a.inverse ? -sn : sn);
     }
     __syncthreads();
-    constexpr int kSize = std::is_same<T, float>::value ? 4 : 2;
-    const int turned = a.pairs / 8;
+    constexpr int kN = Chunk<T>::kN;
+    const int turned = (kInterleaved ? 2 : 1) * a.pairs / kN;
     for (int k = 0; k < a.tensors; ++k) {
         const RotaryView& v = a.x[k];
         const int total = n * v.heads * a.units;
@@ -114,35 +111,33 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a, in
             const char* in = v.in + b * v.ib + h * v.ih + s * v.ir;
             char* out = v.out + b * v.ob + h * v.oh + s * v.orow;
             if (u >= turned) {
-                const int e = (2 * a.pairs + 8 * (u - turned)) * kSize;
+                const int e = 2 * a.pairs * (16 / kN) + 16 * (u - turned);
                 *(Chunk<T>*)(out + e) = *(const Chunk<T>*)(in + e);
                 continue;
             }
-            const int lo = (kInterleaved ? 16 * u : 8 * u) * kSize;
-            const int hi = (kInterleaved ? 16 * u + 8 : a.pairs + 8 * u) * kSize;
-            float x[8], y[8], r[8], q[8];
-            to_f32(*(const Chunk<T>*)(in + lo), x);
-            to_f32(*(const Chunk<T>*)(in + hi), y);
-            const float2* cs = turn + t * a.pairs + 8 * u;
+            const float2* cs = turn + t * a.pairs + (kInterleaved ? kN / 2 : kN) * u;
+            float x[kN], r[kN];
+            to_f32(*(const Chunk<T>*)(in + 16 * u), x);
             if constexpr (kInterleaved) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const float2 c = cs[j], d = cs[4 + j];
+                for (int j = 0; j < kN / 2; ++j) {
+                    const float2 c = cs[j];
                     r[2 * j] = x[2 * j] * c.x - x[2 * j + 1] * c.y;
                     r[2 * j + 1] = x[2 * j + 1] * c.x + x[2 * j] * c.y;
-                    q[2 * j] = y[2 * j] * d.x - y[2 * j + 1] * d.y;
-                    q[2 * j + 1] = y[2 * j + 1] * d.x + y[2 * j] * d.y;
                 }
             } else {
+                const int far = a.pairs * (16 / kN);
+                float y[kN], q[kN];
+                to_f32(*(const Chunk<T>*)(in + far + 16 * u), y);
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
+                for (int j = 0; j < kN; ++j) {
                     const float2 c = cs[j];
                     r[j] = x[j] * c.x - y[j] * c.y;
                     q[j] = y[j] * c.x + x[j] * c.y;
                 }
+                *(Chunk<T>*)(out + far + 16 * u) = from_f32<T>(q);
             }
-            *(Chunk<T>*)(out + lo) = from_f32<T>(r);
-            *(Chunk<T>*)(out + hi) = from_f32<T>(q);
+            *(Chunk<T>*)(out + 16 * u) = from_f32<T>(r);
         }
     }
 }
@@ -177,9 +172,16 @@ hipError_t launch_rotary(const ShaoboFa3RotaryParams& p, hipStream_t stream) {
     a.total = p.batch * p.seqlen;
     a.axes = p.axes;
     a.pairs = p.pairs;
-    a.units = p.pairs / 8 + (p.head_dim - 2 * p.pairs) / 8;
+    const int n = 16 / size;
+    a.units = ((p.interleaved ? 2 : 1) * p.pairs + p.head_dim - 2 * p.pairs) / n;
     a.inverse = p.inverse;
-    a.tokens = a.total >= 8192 ? 8 : a.total >= 1024 ? 2 : 1;
+    // As many tokens as keep a workgroup's threads busy a few times over, and
+    // workgroups enough for the chip.
+    int heads = 0;
+    for (int k = 0; k < p.tensors; ++k) heads += p.heads[k];
+    a.tokens = 1;
+    while (a.tokens < 8 && a.tokens * heads * a.units < 2048 && a.total / (2 * a.tokens) >= 1024)
+        a.tokens *= 2;
     a.div_seq = make_fastdiv(p.seqlen);
     a.div_pairs = make_fastdiv(p.pairs);
     a.div_units = make_fastdiv(a.units);

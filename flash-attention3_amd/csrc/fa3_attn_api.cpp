@@ -23,6 +23,8 @@ constexpr float kCapFine = 100.f;
 // jobs count in 32 bits (their products are checked by the plans).
 constexpr int32_t kMaxLen = 1 << 30;
 constexpr int32_t kMaxHeads = 1 << 16;
+// Scales and caps are held where their products with log2 e stay in fp32.
+constexpr float kMaxScore = 1e30f;
 
 bool strides_ok(const ShaoboFa3AttnTensor& t, int elements) {
     return t.batch_stride % elements == 0 && t.head_stride % elements == 0 &&
@@ -42,9 +44,9 @@ int check(const ShaoboFa3AttnParams* a, bool backward, AttnProblem* p) {
     if ((a->causal != 0 && a->causal != 1) ||
         (a->softmax_scale_is_set != 0 && a->softmax_scale_is_set != 1))
         return SHAOBO_FA3_STATUS_INVALID_VALUE;
-    if (a->softmax_scale_is_set && !std::isfinite(a->softmax_scale))
+    if (a->softmax_scale_is_set && !(std::fabs(a->softmax_scale) <= kMaxScore))
         return SHAOBO_FA3_STATUS_INVALID_VALUE;
-    if (!std::isfinite(a->softcap) || a->softcap < 0.f) return SHAOBO_FA3_STATUS_INVALID_VALUE;
+    if (!(a->softcap >= 0.f && a->softcap <= kMaxScore)) return SHAOBO_FA3_STATUS_INVALID_VALUE;
     if ((a->documents_q == nullptr) != (a->documents_k == nullptr))
         return SHAOBO_FA3_STATUS_INVALID_VALUE;
     if (a->prefix_lens != nullptr && !a->causal) return SHAOBO_FA3_STATUS_INVALID_VALUE;
@@ -72,7 +74,7 @@ int check(const ShaoboFa3AttnParams* a, bool backward, AttnProblem* p) {
     p->causal = a->causal != 0;
     p->bias = a->slopes != nullptr;
     p->docs = a->documents_q != nullptr;
-    if ((int64_t)p->batch * p->heads_q >= (1 << 30)) return SHAOBO_FA3_STATUS_UNSUPPORTED;
+    if ((int64_t)p->batch * p->heads_q >= fa3::kMaxGrid) return SHAOBO_FA3_STATUS_UNSUPPORTED;
     const bool fits = backward ? fa3::plan_attn_bwd(*p).ok : fa3::plan_attn_fwd(*p).ok;
     return fits ? SHAOBO_FA3_STATUS_SUCCESS : SHAOBO_FA3_STATUS_UNSUPPORTED;
 }
@@ -90,7 +92,9 @@ AttnMask mask_of(const ShaoboFa3AttnParams& a, const AttnProblem& p) {
     m.causal = a.causal;
     m.c = p.scale * kLog2E;
     if (p.softcap > 0.f) {
-        m.k1 = 2.f * p.scale / p.softcap * kLog2E;
+        // (a tiny cap: the largest fp32, so that a score of zero stays one)
+        const double k1 = 2.0 * p.scale / p.softcap * kLog2E;
+        m.k1 = (float)std::fmin(std::fmax(k1, -3e38), 3e38);
         m.cap2 = p.softcap * kLog2E;
         m.cap_fine = p.softcap > kCapFine;
     }
@@ -187,16 +191,13 @@ int shaobo_fa3_rotary(const ShaoboFa3RotaryParams* params, void* stream) {
         2 * p->pairs > p->head_dim || p->axes > 4)
         return SHAOBO_FA3_STATUS_UNSUPPORTED;
     const int align = p->dtype == SHAOBO_FA3_DTYPE_FP32 ? 4 : 8;
-    int heads = 0;
     for (int k = 0; k < p->tensors; ++k) {
         if (p->heads[k] <= 0) return SHAOBO_FA3_STATUS_INVALID_VALUE;
         if (p->heads[k] > kMaxHeads || !strides_ok(p->in[k], align) ||
             !strides_ok(p->out[k], align))
             return SHAOBO_FA3_STATUS_UNSUPPORTED;
-        heads += p->heads[k];
     }
-    (void)heads;
-    if ((int64_t)p->batch * p->seqlen > kMaxLen) return SHAOBO_FA3_STATUS_UNSUPPORTED;
+    if ((int64_t)p->batch * p->seqlen >= fa3::kMaxGrid) return SHAOBO_FA3_STATUS_UNSUPPORTED;
     if (p->batch == 0 || p->seqlen == 0) return SHAOBO_FA3_STATUS_SUCCESS;
     bool ok = p->positions != nullptr && p->freqs != nullptr;
     for (int k = 0; k < p->tensors; ++k) ok = ok && tensor_ok(p->in[k]) && tensor_ok(p->out[k]);

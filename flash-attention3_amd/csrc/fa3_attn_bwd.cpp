@@ -77,7 +77,8 @@ AttnBwdPlan plan_attn_bwd(const AttnProblem& p) {
     f.range_q_off = take(p.docs ? (size_t)p.batch * q_steps * sizeof(AttnRange) : 0);
     f.part_off = take(parts > 1 ? (size_t)2 * parts * groups * p.sk * D * 4 : 0);
     f.total = at;
-    f.ok = rows < (1ll << 30) && jobs < (1ll << 30) && blocks < (1ll << 30);
+    f.ok = rows < (1ll << 30) && jobs < kMaxGrid && blocks < kMaxGrid &&
+           groups * p.sk / 4 < kMaxGrid;
     f.jobs = f.ok ? (int)jobs : 0;
     return f;
 }

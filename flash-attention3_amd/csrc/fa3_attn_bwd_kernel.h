@@ -430,7 +430,8 @@ __device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* 
     int t = walk.next();
     if (t >= 0) issue(s0, t);
     f16x8 qf[2][C::kKs], df[2][C::kKs];
-    float nl[2], qp[2], slope[2];
+    float nl[2], slope[2];
+    int qp[2];
     f32x4 nd[2];
 #pragma unroll
     for (int n = 0; n < 2; ++n) {
@@ -447,10 +448,10 @@ __device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* 
             qf[n][s] = attn_row8(q, p1_chunk<D>(s, g4), a.d, ok);
             df[n][s] = attn_row8(o, p1_chunk<D>(s, g4), a.d, ok);
         }
-        qp[n] = 0.f;
+        qp[n] = 0;
         slope[n] = 0.f;
         if constexpr (kBias) {
-            qp[n] = (float)(r.i + off);
+            qp[n] = r.i + off;
             slope[n] = a.m.slopes[b * a.m.slopes_bs + r.h] * kLog2e;
         }
     }
@@ -512,7 +513,7 @@ __device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* 
         const int ln = opaque_tid() & 63;
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
-            const float d0 = kBias ? qp[n] - (float)(j0 + 4 * (ln >> 4)) : 0.f;
+            const float d0 = kBias ? (float)(qp[n] - j0 - 4 * (ln >> 4)) : 0.f;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 const int m = j >> 2, e = j & 3;

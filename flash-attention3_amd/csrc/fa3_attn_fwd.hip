@@ -60,9 +60,15 @@ struct FwdRows {
     // keys of them, the longest axis, add less than 2^-34, fp32's half step
     // being 2^-25.  (Looked for only with a distance bias, which makes them.)
     static constexpr float kNone = 64.f;
+    // A bias's seed is off by fp32's rounding of the slope over a whole tile,
+    // also for the keys next to the row whose own bias is small: 64 slope e, a
+    // few times over, is under 2e-5 of a score up to here.
+    static constexpr float kGentle = 1.5f;
     f16x8 qf[2][kKs];
     int lim[2], id[2];
-    float qp[2], slope[2];
+    int qp[2];  // the rows' places among the keys
+    float slope[2];
+    bool gentle;  // no slope of the wave over kGentle
     f32x4 o[kDB][2];  // columns 16 db + 4 g4 + e of rows 16 n + l16
     float mx[2], sum[2];
     int lim_min, lim_max;  // over the rows
@@ -101,15 +107,17 @@ struct FwdRows {
 #pragma unroll
             for (int s = 0; s < kKs; ++s)  // (a scale below zero turns Q's signs)
                 qf[n][s] = attn_flip(attn_row8(q, p1_chunk<D>(s, g4), a.d, ok), a.flip);
-            qp[n] = 0.f;
+            qp[n] = 0;
             slope[n] = 0.f;
             if constexpr (kBias) {
-                qp[n] = (float)(r.i + off);
+                qp[n] = r.i + off;
                 slope[n] = a.m.slopes[b * a.m.slopes_bs + r.h] * kLog2e;
             }
             mx[n] = kNegInf;
             sum[n] = 0.f;
         }
+        gentle = !kBias || __ballot(!(__builtin_fabsf(slope[0]) <= kGentle &&
+                                      __builtin_fabsf(slope[1]) <= kGentle)) == 0;
 #pragma unroll
         for (int i = 0; i < kDB; ++i) o[i][0] = o[i][1] = f32x4{};
     }
@@ -128,13 +136,13 @@ struct FwdRows {
         bool linear = false;  // every row of the wave on one side of every key
         if constexpr (kBias && !kCap) {
             const bool past = q_first >= j0 + 16 * M - 1;
-            linear = (past || q_last <= j0) && c > 1e-30f;
-            const float j = (float)(j0 + 4 * ((opaque_tid() & 63) >> 4));
+            linear = (past || q_last <= j0) && gentle && c > 1e-30f;
+            const int j = j0 + 4 * ((opaque_tid() & 63) >> 4);
             const float inv = linear ? __builtin_amdgcn_rcpf(past ? c : -c) : 0.f;
 #pragma unroll
             for (int n = 0; n < 2; ++n) {
                 const float seed = slope[n] * inv;
-                if (linear) be[n] = -slope[n] * __builtin_fabsf(qp[n] - j);
+                if (linear) be[n] = -slope[n] * __builtin_fabsf((float)(qp[n] - j));
 #pragma unroll
                 for (int m = 0; m < M; ++m)
 #pragma unroll
@@ -201,11 +209,11 @@ struct FwdRows {
         }
         if constexpr (kBias) {
             if (!linear) {
-                const float j = (float)(j0 + 4 * ((opaque_tid() & 63) >> 4));
+                const int j = j0 + 4 * ((opaque_tid() & 63) >> 4);
 #pragma unroll
                 for (int n = 0; n < 2; ++n) {
-                    // (uncapped: the seed taken off again with the bias)
-                    const float d0 = qp[n] - j, b0 = be[n];
+                    // (exact: a difference of places, then fp32)
+                    const float d0 = (float)(qp[n] - j), b0 = be[n];
 #pragma unroll
                     for (int m = 0; m < M; ++m)
 #pragma unroll
@@ -671,7 +679,8 @@ AttnFwdPlan plan_attn_fwd(const AttnProblem& p) {
     }
     f.total = at;
     const int64_t all = groups * f.tiles * f.splits;
-    f.ok = rows < (1ll << 30) && all < (1ll << 30);
+    f.ok = rows < (1ll << 30) && all < kMaxGrid && groups * rows / 4 < kMaxGrid &&
+           (int64_t)p.batch * n_t < kMaxGrid;
     f.jobs = f.ok ? (int)all : 0;
     return f;
 }

@@ -52,6 +52,8 @@ struct AttnProblem {
 };
 
 constexpr int kAttnTile = 64;   // keys (or rows) streamed per step
+// Workgroups of a launch are held below this: their 256 threads count in 32 bits.
+constexpr int64_t kMaxGrid = 1 << 24;
 constexpr int kAttnRows = 128;  // rows (or keys) resident per workgroup
 
 inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }

@@ -80,8 +80,8 @@ ShaoboFa3AttnParams params_of(const Tensor& q, const Tensor& k, const Tensor& v,
     TORCH_CHECK_VALUE(q.is_cuda() && k.device() == q.device() && v.device() == q.device(),
                       "q, k and v must be on the same GPU");
     TORCH_CHECK_VALUE(D % 8 == 0 && D >= 8 && D <= 128, "head_dim must be a multiple of 8 up to 128");
-    constexpr int64_t kMost = 1 << 30;
-    TORCH_CHECK_VALUE(B * Hq < kMost && Sq <= kMost && Sk <= kMost && Hq <= (1 << 16),
+    constexpr int64_t kMost = 1 << 30;  // (what fits a launch is the library's to say)
+    TORCH_CHECK_VALUE(B < kMost && B * Hq < kMost && Sq <= kMost && Sk <= kMost && Hq <= (1 << 16),
                       "too many batch entries, heads or positions");
     ShaoboFa3AttnParams p;
     shaobo_fa3_attn_params_init(&p);
@@ -94,12 +94,12 @@ ShaoboFa3AttnParams params_of(const Tensor& q, const Tensor& k, const Tensor& v,
     p.dtype = dt == at::kBFloat16 ? SHAOBO_FA3_DTYPE_BF16 : SHAOBO_FA3_DTYPE_FP16;
     p.causal = o.causal ? 1 : 0;
     if (o.scale.has_value()) {
-        TORCH_CHECK_VALUE(std::isfinite((float)*o.scale), "softmax_scale must be finite");
+        TORCH_CHECK_VALUE(std::fabs(*o.scale) <= 1e30, "softmax_scale must be finite (1e30 at most)");
         p.softmax_scale = (float)*o.scale;
         p.softmax_scale_is_set = 1;
     }
-    TORCH_CHECK_VALUE(std::isfinite((float)o.softcap) && o.softcap >= 0.0,
-                      "softcap must be 0 (none) or positive and finite");
+    TORCH_CHECK_VALUE(o.softcap >= 0.0 && o.softcap <= 1e30,
+                      "softcap must be 0 (none) or positive and finite (1e30 at most)");
     p.softcap = (float)o.softcap;
     TORCH_CHECK_VALUE(o.softcap == 0.0 || p.softcap > 0.f, "softcap is too small for fp32");
     p.q = view(q, "q");
@@ -240,7 +240,7 @@ std::vector<Tensor> rotary(at::TensorList xs, const Tensor& positions, const Ten
         case at::kFloat: p.position_type = SHAOBO_FA3_POSITIONS_FP32; break;
         default: TORCH_CHECK_VALUE(false, "positions must be int32, int64 or fp32");
     }
-    TORCH_CHECK_VALUE(B * S <= (1 << 30), "too many positions");
+    TORCH_CHECK_VALUE(B < (1 << 24) && S < (1 << 24) && B * S < (1 << 24), "too many positions");
     p.batch = (int32_t)B;
     p.seqlen = (int32_t)S;
     p.head_dim = (int32_t)D;

@@ -265,7 +265,7 @@ def _in_rows(t):
     """t itself where the operators take its memory as it is, else a copy:
     gradients arrive in any layout (expanded, transposed, sliced)."""
     align = 16 // t.element_size()
-    if t.stride(-1) == 1 and t.data_ptr() % 16 == 0 and \
+    if t.stride(-1) == 1 and t.storage_offset() % align == 0 and \
             all(s % align == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1):
         return t
     return t.contiguous()

@@ -69,8 +69,8 @@ typedef struct ShaoboFa3AttnParams {
     int32_t dtype;     /* SHAOBO_FA3_DTYPE_FP16 or _BF16 */
     int32_t causal;    /* 0 or 1 */
     int32_t softmax_scale_is_set; /* 0: 1 / sqrt(head_dim) */
-    float softmax_scale;          /* any finite value */
-    float softcap;                /* 0: none */
+    float softmax_scale;          /* -1e30 to 1e30 */
+    float softcap;                /* 0: none; up to 1e30 */
 
     ShaoboFa3AttnTensor q, k, v;   /* inputs */
     ShaoboFa3AttnTensor out;       /* forward: written; backward: read */
@@ -121,7 +121,8 @@ int shaobo_fa3_attn_bwd(const ShaoboFa3AttnParams* params, void* stream);
  * the other elements are copied.  freqs in one row per axis cover positions
  * of one axis as well as time, height and width that own pairs each (zeros
  * elsewhere) or share them.  Angles are formed and reduced in fp64, so far
- * positions lose nothing; the rotation is fp32 with one rounding. */
+ * positions (integers up to 2^53) lose nothing; the rotation is fp32 with one
+ * rounding. */
 #define SHAOBO_FA3_POSITIONS_INT32 0
 #define SHAOBO_FA3_POSITIONS_INT64 1
 #define SHAOBO_FA3_POSITIONS_FP32 2

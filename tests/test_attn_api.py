@@ -62,6 +62,9 @@ PTR = 1 << 20  # a non-null address; nothing here reads it
     ({"softmax_scale_is_set": 1, "softmax_scale": math.nan}, F.INVALID_VALUE),
     ({"softmax_scale_is_set": 1, "softmax_scale": math.inf}, F.INVALID_VALUE),
     ({"softmax_scale_is_set": 1, "softmax_scale": -0.5}, F.SUCCESS),
+    ({"softmax_scale_is_set": 1, "softmax_scale": 1e31}, F.INVALID_VALUE),
+    ({"softcap": 1e31}, F.INVALID_VALUE),
+    ({"softcap": 1e30}, F.SUCCESS),
     ({"softcap": -1.0}, F.INVALID_VALUE),
     ({"softcap": math.inf}, F.INVALID_VALUE),
     ({"softcap": math.nan}, F.INVALID_VALUE),
@@ -81,6 +84,7 @@ PTR = 1 << 20  # a non-null address; nothing here reads it
     ({"seqlen_k": (1 << 30) + 1}, F.UNSUPPORTED),
     ({"batch": 1 << 29}, F.UNSUPPORTED),
     ({"seqlen_q": 1 << 30, "num_heads_q": 8}, F.UNSUPPORTED),
+    ({"batch": 1 << 20, "num_heads_q": 32, "num_heads_kv": 32}, F.UNSUPPORTED),  # (2^24 jobs and more)
     ({"seqlen_q": 0}, F.SUCCESS),
     ({"seqlen_k": 0}, F.SUCCESS),
 ])
@@ -202,7 +206,7 @@ def rotary_params(lib, **kw):
     ({"pairs": 65}, F.UNSUPPORTED), ({"pairs": 72}, F.UNSUPPORTED), ({"pairs": 0}, F.UNSUPPORTED),
     ({"head_dim": 132}, F.UNSUPPORTED), ({"head_dim": 520}, F.UNSUPPORTED),
     ({"positions": None}, F.INVALID_VALUE), ({"freqs": None}, F.INVALID_VALUE),
-    ({"seqlen": 1 << 30}, F.UNSUPPORTED), ({"batch": 0}, F.SUCCESS), ({"seqlen": 0}, F.SUCCESS),
+    ({"seqlen": 1 << 30}, F.UNSUPPORTED), ({"seqlen": 1 << 23}, F.UNSUPPORTED), ({"batch": 0}, F.SUCCESS), ({"seqlen": 0}, F.SUCCESS),
 ])
 def test_rotary_validation(lib, change, status):
     assert lib.shaobo_fa3_rotary(ctypes.byref(rotary_params(lib, **change)), None) == status

@@ -132,6 +132,9 @@ CASES = [
     # distance bias
     dict(Sq=150, slopes=1), dict(Sq=150, slopes=2, D=128, causal=False), dict(Sq=9, Sk=300, slopes=2),
     dict(Sq=130, slopes=1, softcap=20.0, D=128, dtype=HF), dict(Sq=100, Sk=50, slopes=1, causal=False),
+    # caps and scales at the ends of their range
+    dict(Sq=70, softcap=1e-38, D=128), dict(Sq=70, softcap=1e30), dict(Sq=70, softcap=1e-30, softmax_scale=1e8),
+    dict(Sq=70, softmax_scale=1e-35), dict(Sq=70, softmax_scale=1e-35, slopes=1), dict(Sq=70, softcap=100.0, std=30.0),
     # prefixes: none, inside a tile, past the keys
     dict(Sq=150, prefix=[0, 70]), dict(Sq=150, prefix=[149, 1000], D=128),
     dict(Sq=200, prefix=[65, -5], softcap=10.0, Hq=4), dict(Sq=40, Sk=100, prefix=[90, 10], slopes=1),
@@ -177,6 +180,39 @@ SPLIT = [
 def test_long_key_axis(T, case):
     print("[case]", case, flush=True)
     run_both(*make(case))
+
+
+@pytest.mark.parametrize("causal,D,cap", [(True, 64, 0.0), (False, 128, 0.0), (False, 64, 8.0)])
+def test_steep_and_rising_bias(T, causal, D, cap):
+    """Slopes from one that hides all but the next keys to ones below zero
+    (far keys weigh most): every row's scores, sums and their gradients."""
+    print("[case] slopes", causal, D, cap, flush=True)
+    q, k, v, do, o = make(dict(Sq=700, B=1, Hq=8, Hkv=4, D=D, causal=causal))
+    o["slopes"] = torch.tensor([300.0, 20.0, 3.0, 1.0, 0.7, 0.05, -0.02, -0.5], device="cuda")
+    if cap:
+        o["softcap"] = cap
+    run_both(q, k, v, do, o)
+
+
+def test_bias_at_far_places(T):
+    """Places past 2^24, where fp32 no longer tells neighbours apart: distances
+    are differences of whole numbers."""
+    print("[case] far places", flush=True)
+    Sk, D = (1 << 24) + 300, 8
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    k, v = (torch.randn(1, 1, Sk, D, generator=gen, device="cuda").to(HF) for _ in range(2))
+    q = torch.randn(1, 1, 5, D, generator=gen, device="cuda").to(HF)
+    slopes = torch.full((1,), 0.9, device="cuda")
+    out, lse = torch.ops.shaobo_fa3.attn_forward(q, k, v, True, None, 0.0, slopes)
+    # keys further than 2000 back weigh less than e^-1700
+    want, wlse, off, lse_off = A.forward(q, k[:, :, -2000:], v[:, :, -2000:], True, slopes=slopes)
+    within("lse", lse, wlse, lse_off)
+    within("out", out, want, off)
+    g = torch.ops.shaobo_fa3.attn_backward(torch.ones_like(q), q, k, v, out, lse, True, None, 0.0, slopes)
+    w = A.backward(torch.ones_like(q), q, k[:, :, -2000:], v[:, :, -2000:], out, lse, True, slopes=slopes)
+    within("dq", g[0], *w["dq"])
+    within("dk", g[1][:, :, -2000:], *w["dk"])
+    within("dv", g[2][:, :, -2000:], *w["dv"])
 
 
 # Backwards cut in every way: whole and halved jobs, parts over the heads and
@@ -525,7 +561,7 @@ def test_attention_layer_and_its_gradient(T):
     want = (p / torch.where(z == 0, torch.ones_like(z), z)) @ ref[2].repeat_interleave(2, 1)
     wgrads = torch.autograd.grad((want * w.double()).sum(), ref)
     u = torch.finfo(HF).eps / 2
-    for n, x, y in (("out", out, want), *zip(("dq", "dk", "dv"), grads, wgrads)):
+    for n, x, y in (("out", out.detach(), want.detach()), *zip(("dq", "dk", "dv"), grads, wgrads)):
         assert x.dtype == HF and x.shape == y.shape
         assert float((x.double() - y).norm()) <= 8 * u * float(y.norm()), n
 

@@ -129,6 +129,7 @@ hipError_t launch_attn_bwd(const AttnProblem& p, const ShaoboFa3AttnParams& a, A
     // (group after group leaves the last group's dKV jobs to the end: B2 Hq32
     // Hkv8 S4096 D128 causal 852 -> 1138 us, full 1613 -> 1743)
     x.by_group = 0;
+    x.rising = p.causal && f.jobs <= 512;
     x.div_rparts = make_fastdiv(f.row_parts);
     x.part = (float*)(ws + f.part_off);
     if (p.docs) {

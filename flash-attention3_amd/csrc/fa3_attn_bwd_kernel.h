@@ -29,7 +29,8 @@ struct BwdCfg {
 
 // Workgroup id's job: level < kv_tiles * parts is a dKV job's key tile and
 // part (first keys first: causal's longest), then come the dQ jobs, last rows
-// first.
+// first -- or, where the launch is no more than two jobs a CU, first rows
+// first: the longest dKV job then has the shortest dQ job beside it.
 struct BwdJob {
     int b, hkv, level;
 };
@@ -41,6 +42,12 @@ __device__ __forceinline__ BwdJob bwd_job(const Args& a, int id) {
     j.b = fdiv(a.div_hkv, grp);
     j.hkv = grp - j.b * a.heads_kv;
     return j;
+}
+
+template <typename Args>
+__device__ __forceinline__ int dq_tile(const Args& a, int level) {
+    const int x = level - a.kv_tiles * a.parts;
+    return a.rising ? x : a.q_tiles - 1 - x;
 }
 
 // One workgroup per 64 rows of a query head.
@@ -551,7 +558,7 @@ __device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* 
     const BwdJob e = bwd_job(z, blockIdx.x);
     const int ew = __builtin_amdgcn_readfirstlane(opaque_tid() >> 6), ers = ew / kQb;
     const int eqb = ew & (kQb - 1), eln = opaque_tid() & 63;
-    const int erow = ((z.kv_tiles * z.parts + z.q_tiles - 1 - e.level) * kQb + eqb) * 32;
+    const int erow = (dq_tile(z, e.level) * kQb + eqb) * 32;
     const float sc[2] = {z.scale, z.scale};
     FA3_LDS char* stg = smem + ew * C::kDB * 1024;
     if constexpr (kSplit == 2) {
@@ -582,7 +589,7 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_bwd_kernel(
     if (j.level < n)
         attn_dkv<D, kBf16, kCap != 0, kBias, kCap == 2, kSplit>(j.b, j.hkv, j.level, smem);
     else
-        attn_dq<D, kBf16, kCap != 0, kBias, kCap == 2, kSplit>(j.b, j.hkv, n + a.q_tiles - 1 - j.level, smem);
+        attn_dq<D, kBf16, kCap != 0, kBias, kCap == 2, kSplit>(j.b, j.hkv, dq_tile(a, j.level), smem);
 }
 
 // dV and dK from their parts, added in order; 8 columns a thread.

@@ -24,6 +24,7 @@ struct AttnFwdArgs {
     uint32_t flip;  // XORed into Q's 16-bit pairs
     int scored;     // 0: a scale of zero, Q is taken as zeros
     int levels, by_group;
+    int fold;  // levels from here on run the other way round
     FastDiv div_hkv, div_group, div_groups, div_gpart, div_splits, div_levels;
 };
 
@@ -373,6 +374,7 @@ __device__ __forceinline__ FwdJob fwd_job(const A& a, int id) {
     attn_job(id, a.groups, a.by_group, a.div_groups, a.div_gpart, a.div_levels, a.levels, level, j.grp);
     j.b = fdiv(a.div_hkv, j.grp);
     j.hkv = j.grp - j.b * a.heads_kv;
+    if (level >= a.fold) level = a.levels - 1 - (level - a.fold);
     const int tl = fdiv(a.div_splits, level);
     j.split = level - tl * a.splits;
     j.tile = a.tiles - 1 - tl;
@@ -719,6 +721,11 @@ hipError_t launch_attn_fwd(const AttnProblem& p, const ShaoboFa3AttnParams& a, A
     // (B2 H16 S8192 D64 with bias 668 -> 551, B2 Hq32 Hkv8 S4096 with
     // documents 250 -> 199).
     x.by_group = !p.causal || p.docs;
+    // Where two jobs a CU are the whole launch, the second ones come shortest
+    // first, so that the longest job gets the shortest beside it.
+    x.fold = x.levels;
+    if (f.jobs > 256 && f.jobs <= 512 && !x.by_group && f.splits == 1)
+        x.fold = ceil_div(256, x.groups);
     const bool cap = p.softcap > 0.f, bias = p.bias;
     // Maxima are taken over raw products: their scale must be positive.
     x.scored = 1;

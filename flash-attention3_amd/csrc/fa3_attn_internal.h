@@ -100,7 +100,7 @@ struct AttnBwdArgs {
     // adds them in order.
     int head_parts, row_parts, parts;
     float* part;
-    int levels, by_group;
+    int levels, by_group, rising;
     FastDiv div_hkv, div_group, div_groups, div_gpart, div_hq, div_blocks, div_parts, div_rparts,
         div_levels;
 };

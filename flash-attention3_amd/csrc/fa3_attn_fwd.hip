@@ -73,6 +73,8 @@ struct FwdRows {
     f32x4 o[kDB][2];  // columns 16 db + 4 g4 + e of rows 16 n + l16
     float mx[2], sum[2];
     int lim_min, lim_max;  // over the rows
+    float k1, cap2;        // capped
+    bool fine;
     int q_first, q_last;   // places of the first and last row among the keys
 
     // Rows row0 .. row0 + 31 of KV head hkv in batch entry b.
@@ -85,6 +87,9 @@ struct FwdRows {
         const int last = fdiv(a.div_group, any ? min(row0 + 32, a.rows) - 1 : 0);
         lim_min = any ? attn_limit(first, off, kv, a.m.causal, prefix) : 0x7fffffff;
         lim_max = any ? attn_limit(last, off, kv, a.m.causal, prefix) : 0;
+        k1 = kCap ? a.m.k1 : 0.f;
+        cap2 = kCap ? a.m.cap2 : 0.f;
+        fine = kCap && a.m.cap_fine;
         q_first = first + off;
         q_last = last + off;
 #pragma unroll
@@ -185,9 +190,7 @@ struct FwdRows {
         if (!kCap && !(kBias && !linear)) mask();
         attn_scores<D, kBf16, M, 4>(rd, tk, m0, qf, s);
         if constexpr (kCap) {
-            const auto& a = attn_args<Args>();
-            const float k1 = a.m.k1, cap2 = a.m.cap2;
-            if (a.m.cap_fine) {
+            if (fine) {
                 al = 1.f;
 #pragma unroll
                 for (int m = 0; m < M; ++m)
@@ -413,18 +416,26 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(
     const int rows_at = fdiv(a.div_group, wg_last) + off;
     TileWalk walk(ids == nullptr ? nullptr : a.m.range_k + (int64_t)b * a.m.blocks_k, begin,
                   min(begin + a.part, (wg_max + 63) >> 6), doc, rows_at >> 6);
+    // (held in scalar registers: read again per tile, as the arguments are
+    // elsewhere, they are waited for before the tile's loads go out; opaque,
+    // so that their multiples are not held too)
+    const int64_t k_rs = a.k.rs, v_rs = a.v.rs;
+    const bool wide = a.d == D;
     auto issue = [&](FA3_LDS char* st, int t) {
         const int j0 = t * 64, lane = opaque_tid() & 63;
-        const auto& a = attn_args<Args>();
-        if (j0 + 64 <= kv && a.d == D && !(walk.cls & kTileHidden)) {
-            attn_load_tile<D>(st, kp, a.k.rs, j0, w, lane);
-            attn_load_tile<D>(st + C::kTileBytes, vp, a.v.rs, j0, w, lane);
+        int64_t krs = k_rs, vrs = v_rs;
+        __asm__ volatile("" : "+s"(krs), "+s"(vrs));
+        if (j0 + 64 <= kv && wide && !(walk.cls & kTileHidden)) {
+            attn_load_tile<D>(st, kp, krs, j0, w, lane);
+            attn_load_tile<D>(st + C::kTileBytes, vp, vrs, j0, w, lane);
         } else {
+            const auto& a = attn_args<Args>();
             auto seen = [&](int j) { return ids == nullptr || ids[j] >= 0; };
-            attn_load_tile_edge<D>(st, kp, a.k.rs, j0, kv, a.d, w, lane, seen);
-            attn_load_tile_edge<D>(st + C::kTileBytes, vp, a.v.rs, j0, kv, a.d, w, lane, seen);
+            attn_load_tile_edge<D>(st, kp, krs, j0, kv, a.d, w, lane, seen);
+            attn_load_tile_edge<D>(st + C::kTileBytes, vp, vrs, j0, kv, a.d, w, lane, seen);
         }
-        if (ids != nullptr && w == 0) attn_load_ids(st + 2 * C::kTileBytes, ids, j0, a.sk, lane);
+        if (ids != nullptr && w == 0)
+            attn_load_ids(st + 2 * C::kTileBytes, ids, j0, attn_args<Args>().sk, lane);
     };
     const RegReader<D> rd(lane, 0);
     const float c = a.m.c;

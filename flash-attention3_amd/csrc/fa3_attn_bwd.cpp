@@ -77,7 +77,8 @@ AttnBwdPlan plan_attn_bwd(const AttnProblem& p) {
     f.range_q_off = take(p.docs ? (size_t)p.batch * q_steps * sizeof(AttnRange) : 0);
     f.part_off = take(parts > 1 ? (size_t)2 * parts * groups * p.sk * D * 4 : 0);
     f.total = at;
-    f.ok = rows < (1ll << 30) && jobs < kMaxGrid && blocks < kMaxGrid &&
+    const int64_t delta = blocks + ((int64_t)p.batch * (q_steps + k_steps) + 8) / 4;
+    f.ok = rows < (1ll << 30) && jobs < kMaxGrid && delta < kMaxGrid &&
            groups * p.sk / 4 < kMaxGrid;
     f.jobs = f.ok ? (int)jobs : 0;
     return f;
@@ -132,16 +133,16 @@ hipError_t launch_attn_bwd(const AttnProblem& p, const ShaoboFa3AttnParams& a, A
     x.rising = p.causal && f.jobs <= 512;
     x.div_rparts = make_fastdiv(f.row_parts);
     x.part = (float*)(ws + f.part_off);
+    x.delta_blocks = x.groups * p.group * (f.sqp / 64);
     if (p.docs) {
-        AttnRange* rk = (AttnRange*)(ws + f.range_k_off);
-        AttnRange* rq = (AttnRange*)(ws + f.range_q_off);
-        hipError_t e = launch_attn_ranges(m.doc_k, m.doc_k_bs, p.batch, p.sk, rk, stream);
-        if (e == hipSuccess) e = launch_attn_ranges(m.doc_q, m.doc_q_bs, p.batch, p.sq, rq, stream);
-        if (e != hipSuccess) return e;
-        m.range_k = rk;
-        m.range_q = rq;
+        m.range_k = (AttnRange*)(ws + f.range_k_off);
+        m.range_q = (AttnRange*)(ws + f.range_q_off);
         m.blocks_k = ceil_div(p.sk, 64);
         m.blocks_q = f.sqp / 64;
+        x.q_blocks = p.batch * m.blocks_q;
+        // (one set of documents for both: one set of ranges)
+        if (m.doc_k == m.doc_q && m.doc_k_bs == m.doc_q_bs && p.sk == p.sq) m.range_k = m.range_q;
+        else x.k_blocks = p.batch * m.blocks_k;
     }
     x.m = m;
     const int cap = p.softcap > 0.f ? m.cap_fine ? 2 : 1 : 0;

@@ -9,6 +9,14 @@
 // leaves -lse log2 e and -delta per row, padded to whole tiles: a row that
 // sees no key, or is not there, has -infinity in place of the first, which
 // makes its P zero.
+//
+// What bounds it.  As bwd_reg_kernel, power and two waves' products, LDS reads
+// and exponentials on one SIMD in large launches: B2 Hq32 Hkv8 S4096 D128
+// causal 852 us (806 TFLOP/s of five products), documents of ~1500 tokens 676
+// us (506 of the visible work; a document of 3391 tokens among them makes
+// the longest job).  Small ones are bound by a job's chain, hence the cuts of
+// plan_attn_bwd.  dQ recomputes S and dP (seven products instead of five):
+// adding dS K across workgroups would need atomics or an S^2-sized workspace.
 #pragma once
 
 #include "fa3_attn_device.h"
@@ -50,10 +58,23 @@ __device__ __forceinline__ int dq_tile(const Args& a, int level) {
     return a.rising ? x : a.q_tiles - 1 - x;
 }
 
-// One workgroup per 64 rows of a query head.
+// One workgroup per 64 rows of a query head; with documents, behind them, one
+// per four 64-position blocks of the queries' and then the keys' documents
+// (a launch of their own each took 2.5 us).
 template <int D, bool kBf16>
 __global__ __launch_bounds__(256) void attn_delta_kernel(AttnBwdArgs a) {
     constexpr int kLanes = D / 8, kRows = 256 / kLanes;
+    if ((int)blockIdx.x >= a.delta_blocks) {
+        const int lane = threadIdx.x & 63;
+        int x = ((int)blockIdx.x - a.delta_blocks) * 4 + (int)(threadIdx.x >> 6);
+        const int nq = (a.q_blocks + 3) / 4 * 4;
+        if (x < a.q_blocks)
+            attn_range(a.m.doc_q, a.m.doc_q_bs, a.sq, a.m.blocks_q, x, (AttnRange*)a.m.range_q, lane);
+        x -= nq;
+        if (x >= 0 && x < a.k_blocks)
+            attn_range(a.m.doc_k, a.m.doc_k_bs, a.sk, a.m.blocks_k, x, (AttnRange*)a.m.range_k, lane);
+        return;
+    }
     const int blk = blockIdx.x, nb = a.sqp / 64;
     const int bh = fdiv(a.div_blocks, blk), t = blk - bh * nb;
     const int b = fdiv(a.div_hq, bh), h = bh - b * a.heads_q;
@@ -623,7 +644,7 @@ __global__ __launch_bounds__(256) void attn_sum_kernel(AttnBwdArgs a) {
 // The kernels of one call: delta, the jobs, and the parts' sum.
 template <int D, bool kBf16>
 void launch_bwd(const AttnBwdArgs& x, const AttnBwdPlan& f, int cap, bool bias, hipStream_t stream) {
-    const int blocks = x.groups * x.group * (x.sqp / 64);
+    const int blocks = x.delta_blocks + ceil_div(x.q_blocks, 4) + ceil_div(x.k_blocks, 4);
     if (blocks > 0)
         hipLaunchKernelGGL((attn_delta_kernel<D, kBf16>), dim3(blocks), dim3(256), 0, stream, x);
     auto go = [&](auto kernel) {

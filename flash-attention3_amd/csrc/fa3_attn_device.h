@@ -58,6 +58,21 @@ __device__ __forceinline__ float attn_tanh_fine(float s, float k1) {
     return __builtin_fabsf(u) < 0.125f ? t : far;
 }
 
+// The AttnRange of 64-position block x of ids [batch][n], by one wave.
+__device__ __forceinline__ void attn_range(const int* ids, int64_t bs, int n, int blocks, int x,
+                                           AttnRange* out, int lane) {
+    const int b = x / blocks, i = (x - b * blocks) * 64 + lane;
+    const int id = i < n ? ids[b * bs + i] : -1;
+    int lo = id >= 0 ? id : 0x7fffffff, hi = id >= 0 ? id : -1;
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) {
+        lo = min(lo, __shfl_xor(lo, o));
+        hi = max(hi, __shfl_xor(hi, o));
+    }
+    if (__ballot(id < 0)) lo = ~lo;
+    if (lane == 0) out[x] = AttnRange{lo, hi};
+}
+
 // A document as masks compare it: every negative one meets none.
 __device__ __forceinline__ int doc_of(int id) { return id < 0 ? -3 : id; }
 

@@ -6,7 +6,20 @@
 // rows: S^T = K Q^T with Q resident in registers as the B operand, the
 // softmax down each lane's column, and O^T += V^T P^T, whose B operand is P
 // as the score product left it, rounded (fa3_bwd_reg_kernel.h says why that
-// needs no exchange).  K and V tiles go through two LDS stages.
+// needs no exchange).  K and V tiles go through two LDS stages, two (D 128)
+// or three (D 64) workgroups share a CU.
+//
+// What bounds it.  The vector units as much as the matrix units: an element
+// costs 16 cycles of exponential and about 16 more (a fma, a sum, half a
+// maximum, half a conversion), a cap 40 on top, against 2 D / 8 cycles of
+// products.  Measured: B2 Hq32 Hkv8 S4096 D128 causal 280 us (980 TFLOP/s),
+// B2 H16 S8192 D64 full 627 us (877) and with a distance bias 590 (932 of the
+// nominal work: tiles without weight are left), documents of ~1500 tokens at
+// S4096 169 us (693 of the visible work).  Small launches are bound by one
+// wave's chain, ~2 600 cycles a 32 x 32 step of which 512 are products:
+// making the next tile's scores behind this tile's exponentials (a pipeline
+// within the wave) did not shorten it (S2011 capped 48.9 -> 52.2 us), nor did
+// sending the loads out later.
 #include "fa3_attn_device.h"
 
 namespace fa3 {
@@ -480,7 +493,9 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(
 // Few rows (32 at most of a KV head: single tokens), no documents: a
 // workgroup's four waves all hold them and take every fourth 32-key block
 // each, through two LDS stages of their own -- no barrier until they meet.
-// Bound by reading the cache.
+// Bound by reading the cache: 5.4 TB/s for 16 caches of 8192 keys (Hkv 8, D
+// 128, 99 us, the rate of a large copy), 4.9 where they are filled to
+// different lengths (68.8 us).
 template <int D>
 struct TokenCfg {
     static constexpr int kBlock = 32 * D * 2;   // 32 rows of K or V
@@ -633,18 +648,8 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnFwdArgs a) {
 // One wave per 64 positions.
 __global__ __launch_bounds__(256) void attn_ranges_kernel(const int* ids, int64_t bs, int n,
                                                           int blocks, int total, AttnRange* out) {
-    const int x = blockIdx.x * 4 + (int)(threadIdx.x >> 6), lane = threadIdx.x & 63;
-    if (x >= total) return;
-    const int b = x / blocks, t = x - b * blocks, i = t * 64 + lane;
-    const int id = i < n ? ids[b * bs + i] : -1;
-    int lo = id >= 0 ? id : 0x7fffffff, hi = id >= 0 ? id : -1;
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) {
-        lo = min(lo, __shfl_xor(lo, o));
-        hi = max(hi, __shfl_xor(hi, o));
-    }
-    if (__ballot(id < 0)) lo = ~lo;
-    if (lane == 0) out[x] = AttnRange{lo, hi};
+    const int x = blockIdx.x * 4 + (int)(threadIdx.x >> 6);
+    if (x < total) attn_range(ids, bs, n, blocks, x, out, threadIdx.x & 63);
 }
 
 AttnView view(const ShaoboFa3AttnTensor& t) {
@@ -652,15 +657,6 @@ AttnView view(const ShaoboFa3AttnTensor& t) {
 }
 
 }  // namespace
-
-hipError_t launch_attn_ranges(const int* ids, int64_t bs, int batch, int n, AttnRange* out,
-                              hipStream_t stream) {
-    const int blocks = ceil_div(n, 64), total = batch * blocks;
-    if (total > 0)
-        hipLaunchKernelGGL(attn_ranges_kernel, dim3(ceil_div(total, 4)), dim3(256), 0, stream, ids,
-                           bs, n, blocks, total, out);
-    return hipGetLastError();
-}
 
 AttnFwdPlan plan_attn_fwd(const AttnProblem& p) {
     AttnFwdPlan f{};
@@ -748,8 +744,9 @@ hipError_t launch_attn_fwd(const AttnProblem& p, const ShaoboFa3AttnParams& a, A
     if (f.jobs == 0) return hipSuccess;
     if (p.docs && p.sk > 0) {
         AttnRange* r = (AttnRange*)(ws + f.range_off);
-        const hipError_t e = launch_attn_ranges(m.doc_k, m.doc_k_bs, p.batch, p.sk, r, stream);
-        if (e != hipSuccess) return e;
+        const int blocks = ceil_div(p.sk, 64), total = p.batch * blocks;
+        hipLaunchKernelGGL(attn_ranges_kernel, dim3(ceil_div(total, 4)), dim3(256), 0, stream,
+                           m.doc_k, m.doc_k_bs, p.sk, blocks, total, r);
         m.range_k = r;
         m.blocks_k = ceil_div(p.sk, 64);
     }

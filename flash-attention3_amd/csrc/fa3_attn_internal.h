@@ -94,6 +94,7 @@ struct AttnBwdArgs {
     int heads_q, heads_kv, group, sq, sk, d, sqp;
     int rows;  // group * sq
     int kv_tiles, q_tiles, groups;
+    int delta_blocks, q_blocks, k_blocks;  // attn_delta_kernel's: rows, then document ranges
     // dKV jobs per key tile: head_parts ranges of the group's heads times
     // row_parts ranges of the query tiles.  More than one: their fp32 sums go
     // to part [head_parts * row_parts][dV, dK][groups][sk][D] and attn_sum_kernel
@@ -113,9 +114,6 @@ hipError_t launch_attn_fwd(const AttnProblem& p, const ShaoboFa3AttnParams& a, A
                            hipStream_t stream);
 hipError_t launch_attn_bwd(const AttnProblem& p, const ShaoboFa3AttnParams& a, AttnMask m,
                            hipStream_t stream);
-// AttnRange of every 64-position block of ids [batch][n].
-hipError_t launch_attn_ranges(const int* ids, int64_t bs, int batch, int n, AttnRange* out,
-                              hipStream_t stream);
 hipError_t launch_rotary(const ShaoboFa3RotaryParams& p, hipStream_t stream);
 
 }  // namespace fa3

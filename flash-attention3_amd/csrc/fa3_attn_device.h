@@ -16,17 +16,18 @@ constexpr float kNegInf = -__builtin_inff();
 // 16 zero bytes: where the loads of rows and columns outside a tensor read.
 __device__ __attribute__((aligned(16))) const uint32_t attn_zeros[4] = {0, 0, 0, 0};
 
-// max over the four lanes of equal lane % 16.  v_permlane{32,16}_swap with
-// one register on both sides leave a lane's own and its partner's value.
+// max over the four lanes of equal lane % 16, NaN if one of them is.
+// v_permlane{32,16}_swap with one register on both sides leave a lane's own
+// and its partner's value.
 __device__ __forceinline__ float max_groups(float x) {
     const uint32_t u = __builtin_bit_cast(uint32_t, x);
     auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
-    x = __builtin_fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]),
-                        __builtin_bit_cast(float, (uint32_t)r[1]));
+    x = __builtin_elementwise_maximum(__builtin_bit_cast(float, (uint32_t)r[0]),
+                                      __builtin_bit_cast(float, (uint32_t)r[1]));
     const uint32_t v = __builtin_bit_cast(uint32_t, x);
     r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
-    return __builtin_fmaxf(__builtin_bit_cast(float, (uint32_t)r[0]),
-                           __builtin_bit_cast(float, (uint32_t)r[1]));
+    return __builtin_elementwise_maximum(__builtin_bit_cast(float, (uint32_t)r[0]),
+                                         __builtin_bit_cast(float, (uint32_t)r[1]));
 }
 __device__ __forceinline__ float sum_groups(float x) {
     const uint32_t u = __builtin_bit_cast(uint32_t, x);

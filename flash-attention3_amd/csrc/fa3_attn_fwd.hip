@@ -255,7 +255,7 @@ struct FwdRows {
                     x = __builtin_elementwise_maximum(x, s[m][n][e]);
             top[n] = max_groups(__builtin_fmaf(al, x, be[n]));
             up |= top[n] > mx[n] + kLazy;
-            some |= top[n] > mx[n] - kNone;
+            some |= !(top[n] <= mx[n] - kNone);  // (NaN is some)
         }
         if (kBias && !__ballot(some)) return;
         if (__ballot(up)) {
@@ -286,6 +286,41 @@ struct FwdRows {
                 bp[n] = pack8<kBf16>(p);
             }
             reg_grads<D, kBf16, false>(rd, tv, tv, m0 / 2 + r, bp, bp, o, o);
+        }
+    }
+
+    // Whether row `row` of KV head hkv sees any key at all: lane g4 of its four
+    // looks at every fourth, last first (with causality its own document is
+    // there).  What init() read is read again: not held over the tile loop.
+    template <bool kDocs, typename A>
+    static __device__ __forceinline__ bool sees(const A& z, int row, int b, int hkv, int g4) {
+        const AttnRow r = attn_row(row, z.rows, hkv, z.group, z.div_group);
+        const int kv = attn_kv(z.m, b, z.sk);
+        const int lim = r.ok ? attn_limit(r.i, kv - z.sq, kv, z.m.causal, attn_prefix(z.m, b)) : 0;
+        bool any = lim > 0;
+        if (kDocs && any && z.m.doc_k != nullptr) {
+            const int* ids = z.m.doc_k + b * z.m.doc_k_bs;
+            const int id = z.m.doc_q[b * z.m.doc_q_bs + r.i];
+            any = false;
+#pragma unroll 1
+            for (int j = lim - 1 - g4; j >= 0 && !any; j -= 4) any = doc_of(ids[j]) == id;
+        }
+        return max_groups(any ? 1.f : 0.f) > 0.f;
+    }
+
+    // After the last tile.  A row without a maximum but with a sum has met NaN:
+    // in what it sees, or it sees nothing and its Q or other rows' keys held
+    // it, which counts for nothing.
+    template <bool kDocs>
+    __device__ __forceinline__ void settle(int row0, int b, int hkv) {
+        const int ln = opaque_tid() & 63;
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const bool odd = mx[n] == kNegInf && sum_groups(sum[n]) != 0.f;
+            if (!__ballot(odd)) continue;
+            // (by all lanes: they meet in it.  finish() clears o)
+            const bool some = sees<kDocs>(attn_args<Args>(), row0 + 16 * n + (ln & 15), b, hkv, ln >> 4);
+            if (odd && !some) sum[n] = 0.f;
         }
     }
 
@@ -344,9 +379,9 @@ struct FwdRows {
 #pragma unroll
         for (int n = 0; n < 2; ++n) {
             const float l = sum_groups(sum[n]);
-            const bool none = mx[n] == kNegInf;
+            const bool none = mx[n] == kNegInf && l == 0.f;
             inv[n] = none ? 0.f : 1.f / l;
-            if (none) {  // (its Q may have been NaN)
+            if (none) {  // (other rows' V may have been NaN)
 #pragma unroll
                 for (int i = 0; i < kDB; ++i) o[i][n] = f32x4{};
             }
@@ -481,6 +516,7 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(
     barrier();  // every wave is done with the stages: they take the outputs
     const FwdJob e = fwd_job(attn_args<Args>(), blockIdx.x);  // (decoded again: not held over the loop)
     const int ew = __builtin_amdgcn_readfirstlane(opaque_tid() >> 6), eqb = ew & (kQb - 1);
+    rows.template settle<true>((e.tile * kQb + eqb) * 32, e.b, e.hkv);
     if constexpr (kSplit > 1) {
         rows.template meet<kSplit>((FA3_LDS float*)smem, smem + 2048, ew, eqb, ew / kQb);
         if (ew / kQb > 0) return;
@@ -586,6 +622,7 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 2 : 1) void attn_token_kerne
     barrier();
     const FwdJob e = fwd_job(attn_args<Args>(), blockIdx.x);
     const int ew = __builtin_amdgcn_readfirstlane(opaque_tid() >> 6);
+    rows.template settle<false>(0, e.b, e.hkv);
     rows.template meet<4>((FA3_LDS float*)smem, smem + 2048, ew, 0, ew);
     if (ew > 0) return;
     rows.finish(0, e.b, e.hkv, e.grp, e.split, smem + 2048);
@@ -594,9 +631,10 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 2 : 1) void attn_token_kerne
 // Joins the parts of a split key axis: with w_s = exp2(l_s - max l), out =
 // sum w_s o_s / sum w_s.  D / 8 lanes hold a row, 8 columns each.  kWays
 // groups of them take every kWays-th part of it, whose sums meet at the end:
-// many parts are few rows, which leave only latency to win (32 parts, 32 rows:
-// 18 us with one way, 8 with four at D 128), and few parts are many rows,
-// which fill the chip (2 parts, 8 044 rows: 14 us with one way, 21 with four).
+// many parts are few rows, which leave only latency to win (whole calls: B1
+// Hq32 Hkv8 Sk16384 D128 in 32 parts 37.1 us with one way, 19.4 with four), and
+// few parts are many rows, which fill the chip (B1 Hq16 Hkv4 S2011 in two parts
+// 59.2 with one way, 66.0 with four).
 template <int D, bool kBf16, int kWays>
 __global__ __launch_bounds__(256) void attn_join_kernel(AttnFwdArgs a) {
     constexpr int kLanes = D / 8, kRow = kLanes * kWays;
@@ -634,10 +672,11 @@ __global__ __launch_bounds__(256) void attn_join_kernel(AttnFwdArgs a) {
     const int grp = (int)(rg / a.rows), r = (int)(rg - (int64_t)grp * a.rows);
     const int b = fdiv(a.div_hkv, grp), hkv = grp - b * a.heads_kv;
     const AttnRow x = attn_row(r, a.rows, hkv, a.group, a.div_group);
-    const float inv = z > 0.f ? 1.f / z : 0.f;
+    const bool none = z == 0.f;  // (NaN is not)
+    const float inv = none ? 0.f : 1.f / z;
     if (lane == 0)
         a.lse[((int64_t)b * a.heads_q + x.h) * a.sq + x.i] =
-            z > 0.f ? (top + __builtin_amdgcn_logf(z)) * 0.69314718055994531f : kNegInf;
+            none ? kNegInf : (top + __builtin_amdgcn_logf(z)) * 0.69314718055994531f;
     if (lane >= kLanes || col >= a.d) return;
     f16x8 v;
 #pragma unroll

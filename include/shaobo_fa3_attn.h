@@ -26,9 +26,11 @@
  *
  * Keys at kv and behind, and keys with a negative document, take no part
  * whatever their K and V hold (NaN included), and neither do queries that
- * see no key, whatever their Q and dO hold.  Other values must be finite: a
- * NaN or infinity in one visible key or row can reach every row and key of
- * its batch entry and KV head.
+ * see no key, whatever their Q and dO hold.  A NaN in a row's Q or in a key
+ * it sees makes the row's outputs NaN (but V of keys that a distance bias
+ * leaves less than 2^-64 of the row's largest weight may not be looked at);
+ * a NaN or infinity in one visible key or row can also reach other rows and
+ * keys of its batch entry and KV head, rows that see no key excepted.
  *
  * Nothing is allocated; launches go to `stream` (a hipStream_t of the
  * current GPU, NULL = the null stream) and are not waited for, so they can

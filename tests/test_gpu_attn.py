@@ -312,6 +312,36 @@ def test_causal_rows_without_keys_may_hold_anything(T):
         assert torch.equal(x, grads[n]), n
 
 
+@pytest.mark.parametrize("extra", [{}, dict(softcap=10.0), dict(slopes=1), dict(causal=False),
+                                   dict(docs=40.0)], ids=lambda e: "-".join(e) or "causal")
+@pytest.mark.parametrize("Sq,Sk", [(1, 1), (1, 70), (1, 3000), (150, 150), (40, 3000), (600, 600)])
+def test_visible_nan_shows(T, Sq, Sk, extra):
+    """A row whose Q is NaN, or that sees a key that is, has NaN for output and
+    log-sum-exp, never the zeros of a row that sees nothing; rows that see
+    nothing stay zeros."""
+    print("[case] visible NaN", Sq, Sk, extra, flush=True)
+    q, k, v, do, o = make(dict(Sq=Sq, Sk=Sk, D=128, Hq=4, **extra))
+    docs = o.get("documents")
+    if docs is not None and Sq > 2:
+        docs[0, Sq - 2] = 99999  # (a document without keys)
+    see = A.visible(0, Sq, Sk, o["causal"], docs, o.get("documents_k"), None, None, "cuda")[0]
+    q2 = q.clone()
+    q2[0, 1] = math.nan
+    out, lse = torch.ops.shaobo_fa3.attn_forward(q2, k, v, *op_args(o))
+    rows = see.any(1)
+    assert torch.isnan(out[0, 1][rows]).all() and torch.isnan(lse[0, 1][rows]).all()
+    assert (out[0, 1][~rows] == 0).all() and (lse[0, 1][~rows] == -math.inf).all()
+    assert torch.isfinite(out[1]).all() and torch.isfinite(out[0, 2:]).all()
+    for j in {0, Sk // 2, Sk - 1}:
+        k2 = k.clone()
+        k2[0, 1, j, 5] = math.nan  # (KV head 1: query heads 2 and 3)
+        out, lse = torch.ops.shaobo_fa3.attn_forward(q, k2, v, *op_args(o))
+        assert torch.isnan(out[0, 2:][:, see[:, j]]).all(), j
+        assert torch.isnan(lse[0, 2:][:, see[:, j]]).all(), j
+        assert (out[0, 2:][:, ~rows] == 0).all() and (lse[0, 2:][:, ~rows] == -math.inf).all()
+        assert torch.isfinite(out[1]).all() and torch.isfinite(out[0, :2]).all()
+
+
 def test_strides(T):
     """Heads of one packed tensor, expanded keys, and rows far apart."""
     print("[case] strides", flush=True)

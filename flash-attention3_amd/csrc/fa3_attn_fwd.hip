@@ -13,9 +13,9 @@
 // costs 16 cycles of exponential and about 16 more (a fma, a sum, half a
 // maximum, half a conversion), a cap 40 on top, against 2 D / 8 cycles of
 // products.  Measured: B2 Hq32 Hkv8 S4096 D128 causal 280 us (980 TFLOP/s),
-// B2 H16 S8192 D64 full 627 us (877) and with a distance bias 590 (932 of the
+// B2 H16 S8192 D64 full 627 us (877) and with a distance bias 597 (921 of the
 // nominal work: tiles without weight are left), documents of ~1500 tokens at
-// S4096 169 us (693 of the visible work).  Small launches are bound by one
+// S4096 171 us (684 of the visible work).  Small launches are bound by one
 // wave's chain, ~2 600 cycles a 32 x 32 step of which 512 are products:
 // making the next tile's scores behind this tile's exponentials (a pipeline
 // within the wave) did not shorten it (S2011 capped 48.9 -> 52.2 us), nor did
@@ -37,7 +37,6 @@ struct AttnFwdArgs {
     uint32_t flip;  // XORed into Q's 16-bit pairs
     int scored;     // 0: a scale of zero, Q is taken as zeros
     int levels, by_group;
-    int fold;  // levels from here on run the other way round
     FastDiv div_hkv, div_group, div_groups, div_gpart, div_splits, div_levels;
 };
 
@@ -425,7 +424,6 @@ __device__ __forceinline__ FwdJob fwd_job(const A& a, int id) {
     attn_job(id, a.groups, a.by_group, a.div_groups, a.div_gpart, a.div_levels, a.levels, level, j.grp);
     j.b = fdiv(a.div_hkv, j.grp);
     j.hkv = j.grp - j.b * a.heads_kv;
-    if (level >= a.fold) level = a.levels - 1 - (level - a.fold);
     const int tl = fdiv(a.div_splits, level);
     j.split = level - tl * a.splits;
     j.tile = a.tiles - 1 - tl;
@@ -702,12 +700,20 @@ AttnFwdPlan plan_attn_fwd(const AttnProblem& p) {
     const int64_t rows = (int64_t)p.group * p.sq, groups = (int64_t)p.batch * p.heads_kv;
     const int D = p.d > 64 ? 128 : 64;
     const int n_t = ceil_div(p.sk, 64);
+    // One 32-row block: every wave on the cache, not one of four (B1 Hq32 Hkv8
+    // Sk16384 D128 19.4 us, 291 by row tiles with the key axis whole).
     f.token = rows <= 32 && !p.docs;
+    // 64-row jobs until two of 128 rows a CU fill the chip: B1 Hq16 Hkv4 S2011
+    // 45.0 us against 58.1, but B2 Hq32 Hkv8 S4096 398 against 302.
     f.split = !f.token && groups * ceil_div(rows, kAttnRows) < 512 ? 2 : 1;
     f.tiles = f.token ? 1 : ceil_div(rows, kAttnRows / f.split);
     f.splits = 1;
     f.part = n_t;
     const int64_t jobs = groups * f.tiles;
+    // Jobs that leave the chip half empty cut the key axis, as long as a part
+    // keeps a few tiles: B1 H7 S1923 32.6 us in two parts, 42.4 whole, but B1
+    // Hq32 Hkv8 S512 23.3 in two and 16.2 whole.  (A CU holds one workgroup of
+    // the kernel for few rows at D 128, two otherwise.)
     const int fill = f.token && D == 128 ? 256 : 512, least = f.token ? 4 : 8;
     if (jobs > 0 && 2 * jobs <= fill && n_t >= 2 * least) {
         const int want = (int)(fill / jobs), most = n_t / least;
@@ -767,11 +773,6 @@ hipError_t launch_attn_fwd(const AttnProblem& p, const ShaoboFa3AttnParams& a, A
     // (B2 H16 S8192 D64 with bias 668 -> 551, B2 Hq32 Hkv8 S4096 with
     // documents 250 -> 199).
     x.by_group = !p.causal || p.docs;
-    // Where two jobs a CU are the whole launch, the second ones come shortest
-    // first, so that the longest job gets the shortest beside it.
-    x.fold = x.levels;
-    if (f.jobs > 256 && f.jobs <= 512 && !x.by_group && f.splits == 1)
-        x.fold = ceil_div(256, x.groups);
     const bool cap = p.softcap > 0.f, bias = p.bias;
     // Maxima are taken over raw products: their scale must be positive.
     x.scored = 1;

@@ -125,11 +125,6 @@ hipError_t launch_attn_bwd(const AttnProblem& p, const ShaoboFa3AttnParams& a, A
     x.row_parts = f.row_parts;
     x.parts = f.head_parts * f.row_parts;
     x.div_parts = make_fastdiv(x.parts);
-    x.levels = f.kv_tiles * x.parts + f.q_tiles;
-    x.div_levels = make_fastdiv(x.levels);
-    // (group after group leaves the last group's dKV jobs to the end: B2 Hq32
-    // Hkv8 S4096 D128 causal 852 -> 1138 us, full 1613 -> 1743)
-    x.by_group = 0;
     x.rising = p.causal && f.jobs <= 512;
     x.div_rparts = make_fastdiv(f.row_parts);
     x.part = (float*)(ws + f.part_off);

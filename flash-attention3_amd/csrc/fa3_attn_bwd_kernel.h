@@ -24,7 +24,6 @@
 namespace fa3 {
 namespace {
 
-
 template <int D>
 struct BwdCfg {
     using R = RegCfg<D>;
@@ -46,7 +45,9 @@ template <typename Args>
 __device__ __forceinline__ BwdJob bwd_job(const Args& a, int id) {
     BwdJob j;
     int grp;
-    attn_job(id, a.groups, a.by_group, a.div_groups, a.div_gpart, a.div_levels, a.levels, j.level, grp);
+    // (group after group leaves the last group's dKV jobs to the end: B2 Hq32
+    // Hkv8 S4096 D128 causal 852 -> 1138 us, full 1613 -> 1743)
+    attn_job(id, a.groups, false, a.div_groups, a.div_gpart, a.div_gpart, 0, j.level, grp);
     j.b = fdiv(a.div_hkv, grp);
     j.hkv = grp - j.b * a.heads_kv;
     return j;

@@ -101,9 +101,8 @@ struct AttnBwdArgs {
     // adds them in order.
     int head_parts, row_parts, parts;
     float* part;
-    int levels, by_group, rising;
-    FastDiv div_hkv, div_group, div_groups, div_gpart, div_hq, div_blocks, div_parts, div_rparts,
-        div_levels;
+    int rising;
+    FastDiv div_hkv, div_group, div_groups, div_gpart, div_hq, div_blocks, div_parts, div_rparts;
 };
 void launch_attn_bwd_d64_fp16(const AttnBwdArgs&, const AttnBwdPlan&, int cap, bool bias, hipStream_t);
 void launch_attn_bwd_d64_bf16(const AttnBwdArgs&, const AttnBwdPlan&, int cap, bool bias, hipStream_t);

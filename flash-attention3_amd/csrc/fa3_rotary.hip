@@ -4,9 +4,9 @@
 // once, in LDS, and turns every head's row with them, 16 bytes (or 16 and
 // their partners') a thread at a time.  Bound by HBM, x read once and written
 // once: B2 S8192 Hq32 + Hkv8 D128 bf16 69 us, 4.8 TB/s, a large copy's rate.
-// Angles are
-// sum_a positions[a] freqs[a][p] in fp64, reduced to [-1/2, 1/2] turns there:
-// at a million positions an fp32 product would be off by 0.06 radians.
+// Angles are sum_a positions[a] freqs[a][p] in fp64, reduced to [-1/2, 1/2]
+// turns there: at a million positions an fp32 product would be off by 0.06
+// radians.
 #include "fa3_attn_internal.h"
 #include "fa3_bwd_device.h"
 

@@ -709,6 +709,52 @@ def test_graph_capture(T, case):
             assert torch.equal(x, y) and torch.equal(x, z)
 
 
+def test_training_step_captured(T):
+    """Rotary, attention and their gradient through autograd in one graph,
+    replayed between eager steps."""
+    q, k, v, do, o = make(dict(Sq=130, Hq=4, Hkv=2, D=128, docs=60.0, softcap=20.0))
+    q, k, v = (x.detach().requires_grad_() for x in (q, k, v))
+    pos = torch.arange(130, device="cuda").expand(1, 2, 130)
+    freqs = T.rotary_freqs([64], device="cuda")
+
+    def step():
+        qr, kr = T.rotary(q, k, positions=pos, freqs=freqs)
+        out = T.score_attention(qr, kr, v, causal=True, softcap=20.0, documents=o["documents"])
+        return torch.autograd.grad(out, (q, k, v), do)
+
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            step()
+    torch.cuda.current_stream().wait_stream(s)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for seed in (4, 5, 6):
+        with torch.no_grad():
+            for a, b in zip((q, k, v, do), make(dict(Sq=130, Hq=4, Hkv=2, D=128), seed)):
+                a.copy_(b)
+        want = [x.clone() for x in step()]
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(want, got):
+            assert torch.equal(x, y)
+
+
+def test_operators_under_torch_library_checks(T):
+    """Schemas and fake implementations agree with what the operators do."""
+    q, k, v, do, o = make(dict(Sq=70, Hq=4, Hkv=2, docs=30.0, bshd=True))
+    out, lse = torch.ops.shaobo_fa3.attn_forward(q, k, v, *op_args(o))
+    pos = torch.arange(70, device="cuda").expand(1, 2, 70)
+    freqs = T.rotary_freqs([32], device="cuda")
+    checks = ("test_schema", "test_faketensor")
+    for op, args in (("attn_forward", (q, k, v, *op_args(o))),
+                     ("attn_backward", (do, q, k, v, out, lse, *op_args(o))),
+                     ("rotary", ([q, k], pos, freqs))):
+        torch.library.opcheck(getattr(torch.ops.shaobo_fa3, op).default, args, test_utils=checks)
+
+
 # ---------------------------------------------------------------------------
 def refused(match, fn, error=ValueError):
     with pytest.raises(error, match=match):

@@ -195,7 +195,7 @@ class _Attention(torch.autograd.Function):
     def backward(ctx, dout):
         q, k, v, out, lse = ctx.saved_tensors
         dq, dk, dv, _ = torch.ops.shaobo_fa3.flash_attn_backward(
-            dout.contiguous(), q, k, v, out, lse, ctx.causal, ctx.scale, False)
+            _in_rows(dout.contiguous()), q, k, v, out, lse, ctx.causal, ctx.scale, False)
         return dq, dk, dv, None, None
 
 
@@ -263,12 +263,13 @@ if _ATTN:
 
 def _in_rows(t):
     """t itself where the operators take its memory as it is, else a copy:
-    gradients arrive in any layout (expanded, transposed, sliced)."""
+    gradients arrive in any layout (expanded, transposed, sliced) and from any
+    element on (a part of a joined vector's, which contiguous() leaves there)."""
     align = 16 // t.element_size()
     if t.stride(-1) == 1 and t.storage_offset() % align == 0 and \
             all(s % align == 0 for n, s in zip(t.shape[:-1], t.stride()[:-1]) if n > 1):
         return t
-    return t.contiguous()
+    return t.clone(memory_format=torch.contiguous_format)
 
 
 class _ScoreAttention(torch.autograd.Function):

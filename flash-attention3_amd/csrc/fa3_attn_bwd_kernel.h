@@ -593,6 +593,14 @@ __device__ __forceinline__ void attn_dq(int b, int hkv, int tile, FA3_LDS char* 
         if (ers == 1) return;
         reg_add<C::kDB>(slot, acc, eln);
     }
+    // (a row that sees no key: zeros, but zeros that may have met a NaN of
+    // other rows' keys)
+#pragma unroll
+    for (int n = 0; n < 2; ++n)
+        if (nl[n] == kNegInf) {
+#pragma unroll
+            for (int i = 0; i < C::kDB; ++i) acc[i][n] = f32x4{};
+        }
     attn_store<D, kBf16>(acc, sc, z.d, stg, [&](int r) -> _Float16* {
         const AttnRow x = attn_row(erow + r, z.rows, e.hkv, z.group, z.div_group);
         return x.ok ? z.dq.p + e.b * z.dq.bs + x.h * z.dq.hs + x.i * z.dq.rs : nullptr;

@@ -47,3 +47,42 @@ def test_gradients_that_start_anywhere(T, dtype, offset):
                   (lambda *x: T.attention(*x), (q, k, v))):
         for a, b in zip(grads(f, xs, True), grads(f, xs, False)):
             assert torch.equal(a, b)
+
+
+@pytest.mark.parametrize("where", ["q", "k", "v", "dout"])
+@pytest.mark.parametrize("case", [
+    dict(Sq=150, D=128, Hq=4, docs=40.0), dict(Sq=150, D=64, dtype=HF, Hq=4, docs=40.0),
+    dict(Sq=150, D=128, Hq=4, docs=40.0, causal=False, softcap=10.0), dict(Sq=100, Sk=60, D=128, slopes=1),
+    dict(Sq=100, Sk=60, D=72, dtype=HF, softcap=200.0), dict(Sq=70, D=64, kv=[9, 70]),
+    # (jobs of whole 128 rows)
+    dict(B=12, Hq=24, Hkv=12, Sq=600, D=128, docs=40.0)], ids=str)
+def test_gradients_of_rows_without_keys(T, case, where):
+    """A NaN in what some rows see (or in their own Q or dO): the rows of its
+    tiles that see nothing have a gradient of zero all the same, and other
+    batch entries stay as they are."""
+    print("[case] keyless rows", case, where, flush=True)
+    q, k, v, do, o = make(case)
+    B, _, Sq, _ = q.shape
+    Sk = k.shape[2]
+    if "docs" in case:
+        o["documents_k"] = o["documents"].clone()
+        o["documents"][0, 60:70] = 99999  # (a document without keys)
+    seen = A.visible(0, Sq, Sk, o["causal"], o.get("documents"), o.get("documents_k"), None,
+                     o.get("kv_lens"), "cuda")[0]
+    rows, keys = seen.any(1), seen.any(0)
+    assert rows.any() and not rows.all()
+    for bad in (math.nan, math.inf):
+        x = dict(q=q, k=k, v=v, dout=do)
+        x[where] = x[where].clone()
+        hit = rows if where in ("q", "dout") else keys
+        x[where][0, 0, hit.nonzero()[0, 0], 5] = bad
+        out, lse = torch.ops.shaobo_fa3.attn_forward(x["q"], x["k"], x["v"], *op_args(o))
+        dq, dk, dv, delta = torch.ops.shaobo_fa3.attn_backward(
+            x["dout"], x["q"], x["k"], x["v"], out, lse, *op_args(o))
+        torch.cuda.synchronize()
+        assert (lse[0, :, ~rows] == -math.inf).all()
+        for t in (out[0], dq[0]):
+            assert (t[:, ~rows] == 0).all()
+        assert (delta[0, :, ~rows] == 0).all()
+        for t in (out, dq, dk, dv, delta):
+            assert torch.isfinite(t[1:]).all()

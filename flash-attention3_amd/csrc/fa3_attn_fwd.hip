@@ -299,7 +299,7 @@ struct FwdRows {
         bool any = lim > 0;
         if (kDocs && any && z.m.doc_k != nullptr) {
             const int* ids = z.m.doc_k + b * z.m.doc_k_bs;
-            const int id = z.m.doc_q[b * z.m.doc_q_bs + r.i];
+            const int id = max(z.m.doc_q[b * z.m.doc_q_bs + r.i], -1);
             any = false;
 #pragma unroll 1
             for (int j = lim - 1 - g4; j >= 0 && !any; j -= 4) any = doc_of(ids[j]) == id;

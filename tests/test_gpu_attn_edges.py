@@ -86,3 +86,29 @@ def test_gradients_of_rows_without_keys(T, case, where):
         assert (delta[0, :, ~rows] == 0).all()
         for t in (out, dq, dk, dv, delta):
             assert torch.isfinite(t[1:]).all()
+
+
+@pytest.mark.parametrize("Sq,causal", [(150, True), (150, False), (1111, True)])
+@pytest.mark.parametrize("pad", [-1, -2, -3, -4, -2147483648])
+def test_every_negative_document_is_padding(T, pad, Sq, causal):
+    """Padding on both sides under any negative document, a NaN in a key that
+    the other rows see, junk in the padding: its rows stay zeros, and take no
+    part in the backward."""
+    print("[case] padding", pad, Sq, causal, flush=True)
+    q, k, v, do, o = make(dict(Sq=Sq, D=128, Hq=4, causal=causal))
+    ids = torch.zeros(2, Sq, dtype=torch.int32, device="cuda")
+    ids[0, 100:110] = pad
+    ids[1, 7] = pad
+    o["documents"] = ids
+    here = ids < 0
+    k[:, 0, 60, 3] = math.nan
+    q, do = (torch.where(here[:, None, :, None], math.nan, t).to(BF) for t in (q, do))
+    out, lse = torch.ops.shaobo_fa3.attn_forward(q, k, v, *op_args(o))
+    dq, dk, dv, delta = torch.ops.shaobo_fa3.attn_backward(do, q, k, v, out, lse, *op_args(o))
+    torch.cuda.synchronize()
+    for b in range(2):
+        assert (lse[b, :, here[b]] == -math.inf).all()
+        assert all((t[b, :, here[b]] == 0).all() for t in (out, dq, delta))
+        # (KV head 1 holds no NaN that counts)
+        assert all(torch.isfinite(t[b, 2:]).all() for t in (out, dq, delta))
+        assert all(torch.isfinite(t[b, 1]).all() for t in (dk, dv))

@@ -26,7 +26,12 @@ void* stream_of(const Tensor& t) {
     return c10::hip::getCurrentHIPStreamMasqueradingAsCUDA(t.device().index()).stream();
 }
 
+// What the library refuses is a ValueError as the checks here are (they leave
+// it what does not fit a launch); a HIP error is not.
 void check_status(int st, const char* entry) {
+    TORCH_CHECK_VALUE(st != SHAOBO_FA3_STATUS_INVALID_VALUE, entry, ": ", shaobo_fa3_status_string(st));
+    TORCH_CHECK_VALUE(st != SHAOBO_FA3_STATUS_UNSUPPORTED, entry, ": ", shaobo_fa3_status_string(st),
+                      ", more rows, heads or positions than a launch takes");
     TORCH_CHECK(st == SHAOBO_FA3_STATUS_SUCCESS, entry, ": ", shaobo_fa3_status_string(st));
 }
 
@@ -164,12 +169,12 @@ std::tuple<Tensor, Tensor> attn_forward(
     const optional<Tensor>& kv_lens) {
     ShaoboFa3AttnParams p = params_of(
         q, k, v, Options{causal, scale, softcap, slopes, documents, documents_k, prefix_lens, kv_lens});
+    check_status(shaobo_fa3_attn_fwd_validate(&p), "shaobo_fa3_attn_fwd");  // (before it takes memory)
     const Guard guard(q.device());
     const Tensor out = like(q);
     const Tensor lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
     p.out = view(out, "out");
     p.softmax_lse = lse.data_ptr<float>();
-    check_status(shaobo_fa3_attn_fwd_validate(&p), "shaobo_fa3_attn_fwd");
     const Tensor ws = workspace(shaobo_fa3_attn_fwd_workspace_bytes(&p), q, &p);
     check_status(shaobo_fa3_attn_fwd(&p, stream_of(q)), "shaobo_fa3_attn_fwd");
     return {out, lse};
@@ -191,9 +196,10 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attn_backward(
                           softmax_lse.sizes() == q.sizes().slice(0, 3) &&
                           softmax_lse.is_contiguous() && softmax_lse.device() == q.device(),
                       "softmax_lse must be contiguous fp32 [batch, heads_q, sequence]");
-    const Guard guard(q.device());
     p.dout = view(dout, "dout");
     p.out = view(out, "out");
+    check_status(shaobo_fa3_attn_bwd_validate(&p), "shaobo_fa3_attn_bwd");
+    const Guard guard(q.device());
     p.softmax_lse = softmax_lse.data_ptr<float>();
     const Tensor dq = like(q), dk = like(k), dv = like(v);
     const Tensor delta = at::empty_like(softmax_lse);
@@ -201,7 +207,6 @@ std::tuple<Tensor, Tensor, Tensor, Tensor> attn_backward(
     p.dk = view(dk, "dk");
     p.dv = view(dv, "dv");
     p.softmax_d = delta.data_ptr<float>();
-    check_status(shaobo_fa3_attn_bwd_validate(&p), "shaobo_fa3_attn_bwd");
     const Tensor ws = workspace(shaobo_fa3_attn_bwd_workspace_bytes(&p), q, &p);
     check_status(shaobo_fa3_attn_bwd(&p, stream_of(q)), "shaobo_fa3_attn_bwd");
     return {dq, dk, dv, delta};

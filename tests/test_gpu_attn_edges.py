@@ -112,3 +112,23 @@ def test_every_negative_document_is_padding(T, pad, Sq, causal):
         # (KV head 1 holds no NaN that counts)
         assert all(torch.isfinite(t[b, 2:]).all() for t in (out, dq, delta))
         assert all(torch.isfinite(t[b, 1]).all() for t in (dk, dv))
+
+
+def test_launches_that_do_not_fit_are_value_errors(T):
+    """More rows or positions than a launch takes: refused as every other
+    argument is, before any memory is taken for outputs."""
+    ops = torch.ops.shaobo_fa3
+    row = torch.zeros(1, 1, 1, 8, dtype=BF, device="cuda")
+    for B, H, S in ((1 << 19, 32, 1), (1, 16, 1 << 23), (1 << 12, 1 << 12, 1)):
+        q = row.expand(B, H, S, 8)
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.max_memory_allocated()
+        with pytest.raises(ValueError, match="shaobo_fa3_attn_fwd"):
+            ops.attn_forward(q, q, q, True)
+        assert torch.cuda.max_memory_allocated() == before
+    # (a backward whose lse is there is asked for its own launch)
+    q = row.expand(1, 16, 1 << 22, 8)
+    lse = torch.zeros(1, 16, 1 << 22, device="cuda")
+    with pytest.raises(ValueError, match="shaobo_fa3_attn_bwd"):
+        ops.attn_backward(q, q, q, q, q, lse, True)

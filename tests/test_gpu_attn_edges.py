@@ -4,9 +4,10 @@ import math
 
 import pytest
 
+import attn_differences as X
 import attn_oracle as A
 import shaobo_fa3 as F
-from test_gpu_attn import BF, HF, i32, make, op_args, randn, run_both
+from test_gpu_attn import BF, HF, make, op_args, oracle_options, randn
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -132,3 +133,25 @@ def test_launches_that_do_not_fit_are_value_errors(T):
     lse = torch.zeros(1, 16, 1 << 22, device="cuda")
     with pytest.raises(ValueError, match="shaobo_fa3_attn_bwd"):
         ops.attn_backward(q, q, q, q, q, lse, True)
+
+
+@pytest.mark.parametrize("case", [
+    dict(Sq=60, Hq=4, D=64, dtype=HF, softcap=3.0, slopes=1, prefix=[20, 0], docs=25.0, std=2.0),
+    dict(Sq=60, Hq=4, D=128, softcap=3.0, slopes=1, prefix=[20, 0], docs=25.0, std=2.0),
+    dict(Sq=140, Hq=4, D=64, dtype=HF), dict(Sq=90, Sk=150, D=72, causal=False, slopes=2, kv=[150, 101]),
+    dict(Sq=70, Hq=6, Hkv=1, D=128, dtype=HF, softcap=150.0, std=20.0, softmax_scale=-0.1)], ids=str)
+def test_gradients_of_every_head_against_differences(T, case):
+    """dq, dk and dv of each (batch entry, head) along themselves against
+    central differences of the fp64 forward; every tolerance, made from the
+    counted roundings, is a tenth of its derivative at most."""
+    print("[case] differences", case, flush=True)
+    q, k, v, do, o = make(case)
+    out, lse = torch.ops.shaobo_fa3.attn_forward(q, k, v, *op_args(o))
+    grads = dict(zip(("dq", "dk", "dv"),
+                     torch.ops.shaobo_fa3.attn_backward(do, q, k, v, out, lse, *op_args(o))))
+
+    def fail(n, b, h, off, tol, slope):
+        raise AssertionError(f"{n}[{b}, {h}]: {off:.3e} off a derivative of {slope:.3e}, "
+                             f"{tol:.3e} allowed")
+
+    assert X.blocks(q, k, v, do, out, lse, grads, oracle_options(o), fail) >= X.LEAST

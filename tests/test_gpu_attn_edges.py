@@ -1,6 +1,7 @@
 """The attention layer where autograd, other rows' values and padding meet it
 in ways that the plain cases do not."""
 import math
+from concurrent.futures import ThreadPoolExecutor
 
 import pytest
 
@@ -155,3 +156,59 @@ def test_gradients_of_every_head_against_differences(T, case):
                              f"{tol:.3e} allowed")
 
     assert X.blocks(q, k, v, do, out, lse, grads, oracle_options(o), fail) >= X.LEAST
+
+
+@pytest.mark.parametrize("case", [
+    dict(B=1, Hq=8, Hkv=1, Sq=700, D=128),                     # dK and dV from parts
+    dict(B=2, Hq=8, Hkv=2, Sq=500, D=128, docs=90.0, softcap=20.0),
+    dict(B=1, Hq=8, Hkv=2, Sq=3, Sk=5000, D=128, slopes=1)], ids=str)
+def test_backwards_on_two_streams_at_once(T, case):
+    """Each call has scratch of its own: row statistics, flags, document
+    ranges and parts pass between up to three kernels of each."""
+    print("[case] two streams", case, flush=True)
+    inputs = [make(case, seed) for seed in (1, 2)]
+    ops = torch.ops.shaobo_fa3
+
+    def step(q, k, v, do, o):
+        out, lse = ops.attn_forward(q, k, v, *op_args(o))
+        return (out, lse, *ops.attn_backward(do, q, k, v, out, lse, *op_args(o)))
+
+    want = [step(*x) for x in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(6):
+        for i, x in enumerate(inputs):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(step(*x))
+    torch.cuda.synchronize()
+    for a, runs in zip(want, got):
+        for b in runs:
+            assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+def test_training_steps_in_two_threads(T):
+    """Two host threads, a stream each: their steps are those of one."""
+    print("[case] two threads", flush=True)
+    inputs = [make(dict(B=2, Hq=6, Hkv=2, Sq=300, D=64, docs=70.0), seed) for seed in (1, 2)]
+
+    def step(q, k, v, do, o):
+        xs = [t.detach().clone().requires_grad_() for t in (q, k, v)]
+        out = T.score_attention(*xs, causal=True, documents=o["documents"])
+        out.backward(do)
+        return [out.detach()] + [t.grad for t in xs]
+
+    want = [step(*x) for x in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+
+    def work(i):
+        with torch.cuda.stream(streams[i]):
+            runs = [step(*inputs[i]) for _ in range(6)]
+            streams[i].synchronize()
+        return runs
+
+    with ThreadPoolExecutor(2) as pool:
+        for a, runs in zip(want, pool.map(work, range(2))):
+            for b in runs:
+                assert all(torch.equal(x, y) for x, y in zip(a, b))

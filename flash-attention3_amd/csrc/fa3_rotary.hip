@@ -4,9 +4,10 @@
 // once, in LDS, and turns every head's row with them, 16 bytes (or 16 and
 // their partners') a thread at a time.  Bound by HBM, x read once and written
 // once: B2 S8192 Hq32 + Hkv8 D128 bf16 69 us, 4.8 TB/s, a large copy's rate.
-// Angles are sum_a positions[a] freqs[a][p] in fp64, reduced to [-1/2, 1/2]
-// turns there: at a million positions an fp32 product would be off by 0.06
-// radians.
+// Angles are sum_a positions[a] freqs[a][p], reduced to [-1/2, 1/2] turns in
+// fp64 with what its products round off carried along (axis_turns): at a
+// million positions an fp32 product would be off by 0.06 radians, at 2^40 an
+// fp64 one by 0.0002.
 #include "fa3_attn_internal.h"
 #include "fa3_bwd_device.h"
 
@@ -76,6 +77,18 @@ __device__ __forceinline__ double position(const void* p, int type, int64_t i) {
     return (double)((const float*)p)[i];
 }
 
+// x f / (2 pi) less a whole number of turns, for |x f| up to 2^53 within 2^-50
+// of a turn.  g + gl is f / (2 pi), gl what g's rounding left off (an fma gives
+// a product's exactly) with the constant's second half; t + tl likewise is its
+// product with x.  Whole turns come off t exactly.
+__device__ __forceinline__ double axis_turns(double x, double f) {
+#pragma clang fp contract(off)
+    constexpr double kTurn = 0x1.45f306dc9c883p-3, kTurnLow = -0x1.6b01ec5417056p-57;  // 1 / (2 pi)
+    const double g = f * kTurn, gl = __builtin_fma(f, kTurn, -g) + f * kTurnLow;
+    const double t = x * g, tl = __builtin_fma(x, g, -t) + x * gl;
+    return (t - rint(t)) + (tl - rint(tl));
+}
+
 template <typename T, bool kInterleaved>
 __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a, int type) {
     extern __shared__ __attribute__((aligned(16))) float2 turn[];  // [tokens][pairs] cos, sin
@@ -85,9 +98,8 @@ __global__ __launch_bounds__(kRotaryThreads) void rotary_kernel(RotaryArgs a, in
         const int b = fdiv(a.div_seq, n0 + t), s = n0 + t - b * a.seqlen;
         double rev = 0.0;
         for (int x = 0; x < a.axes; ++x)
-            rev += position(a.positions, type, x * a.p_as + b * a.p_bs + s * a.p_rs) *
-                   (double)a.freqs[x * a.pairs + p];
-        rev *= 0.15915494309189533577;  // 1 / (2 pi)
+            rev += axis_turns(position(a.positions, type, x * a.p_as + b * a.p_bs + s * a.p_rs),
+                              a.freqs[x * a.pairs + p]);
         rev -= rint(rev);
         float sn, cs;
         sincospif(2.f * (float)rev, &sn, &cs);

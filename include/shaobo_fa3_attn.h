@@ -122,9 +122,10 @@ int shaobo_fa3_attn_bwd(const ShaoboFa3AttnParams* params, void* stream);
  * by the negative angle where `inverse` (the gradient, and the way back);
  * the other elements are copied.  freqs in one row per axis cover positions
  * of one axis as well as time, height and width that own pairs each (zeros
- * elsewhere) or share them.  Angles are formed and reduced in fp64, so far
- * positions (integers up to 2^53) lose nothing; the rotation is fp32 with one
- * rounding. */
+ * elsewhere) or share them.  Angles are reduced to a turn before they become
+ * fp32, off by 2^-50 of a turn at most an axis where |position| and |position
+ * freq| are up to 2^53 (integers past that are rounded to fp64 first), so far
+ * positions lose nothing; the rotation is fp32, rounded to 16 bits once. */
 #define SHAOBO_FA3_POSITIONS_INT32 0
 #define SHAOBO_FA3_POSITIONS_INT64 1
 #define SHAOBO_FA3_POSITIONS_FP32 2

@@ -2,6 +2,7 @@
 in ways that the plain cases do not."""
 import math
 from concurrent.futures import ThreadPoolExecutor
+from fractions import Fraction
 
 import pytest
 
@@ -212,3 +213,42 @@ def test_training_steps_in_two_threads(T):
         for a, runs in zip(want, pool.map(work, range(2))):
             for b in runs:
                 assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+TURN = Fraction(62831853071795864769252867665590057683943387987502116419498891846, 10 ** 64)  # 2 pi
+
+
+@pytest.mark.parametrize("inverse", [False, True])
+@pytest.mark.parametrize("bits,axes,kind", [
+    (20, 1, torch.int32), (31, 3, torch.int32), (32, 1, torch.int64), (40, 2, torch.int64),
+    (53, 1, torch.int64), (53, 4, torch.int64), (24, 2, torch.float32), (50, 1, torch.float32)],
+    ids=str)
+def test_rotary_at_far_positions(T, bits, axes, kind, inverse):
+    """Positions up to 2^53 against angles reduced as exact fractions.  The
+    angle's fp32 remainder and the sine are off by 2^-22 together (as at near
+    positions), the products and their sum by 2^-23 each."""
+    print("[case] far positions", bits, axes, kind, flush=True)
+    gen = torch.Generator(device="cuda").manual_seed(bits)
+    P, S = 32, 24
+    pos = torch.randint(2 ** (bits - 1), 2 ** bits, (axes, 1, S), generator=gen, device="cuda")
+    pos[:, :, ::2] *= -1
+    pos = pos.to(kind)
+    freqs = torch.rand(axes, P, generator=gen, device="cuda")
+    freqs[:, 0] = 1.0
+    x = torch.randn(1, 2, S, 2 * P, generator=gen, device="cuda")
+    (y,) = torch.ops.shaobo_fa3.rotary([x], pos, freqs, False, inverse)
+    torch.cuda.synchronize()
+    at = [[Fraction(n) for n in row] for row in pos[:, 0].tolist()]
+    per = [[Fraction(f) for f in row] for row in freqs.tolist()]
+    angle = torch.empty(S, P, dtype=torch.float64)
+    for s in range(S):
+        for p in range(P):
+            turns = sum(at[a][s] * per[a][p] for a in range(axes)) / TURN
+            angle[s, p] = float((turns - round(turns)) * TURN)
+    if inverse:
+        angle = -angle
+    a, b = x.double().cpu().split(P, 3)
+    got = y.double().cpu().split(P, 3)
+    for g, want in zip(got, (a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin())):
+        off = (a.abs() + b.abs()) * 2.0 ** -21 + 2.0 ** -24 * want.abs()
+        assert ((g - want).abs() <= off).all(), float(((g - want).abs() - off).max())

@@ -42,9 +42,9 @@ __device__ __forceinline__ float sum_groups(float x) {
 //   1 - 2 / (exp(2 s scale / softcap) + 1),  k1 = 2 scale log2 e / softcap.
 // Both ends come out right (exp2 overflows to infinity: 1; underflows: -1).
 // The result is off by about 2^-24 absolutely, the score by softcap times
-// that; with a cap over kAttnCapFine, where that would show, scores below
-// softcap / 8 take the series u - u^3 / 3 + 2 u^5 / 15 - 17 u^7 / 315 (next
-// term 62 / 2835 u^9, 1.3e-9 of the value at 1 / 8).
+// that; with a cap over kCapFine (fa3_attn_api.cpp), where that would show,
+// scores below softcap / 8 take the series u - u^3 / 3 + 2 u^5 / 15 -
+// 17 u^7 / 315 (next term 62 / 2835 u^9, 1.3e-9 of the value at 1 / 8).
 __device__ __forceinline__ float attn_tanh(float s, float k1) {
     const float r = __builtin_amdgcn_rcpf(fast_exp2(s * k1) + 1.f);
     return __builtin_fmaf(-2.f, r, 1.f);

@@ -38,7 +38,7 @@ struct AttnMask {
     int64_t slopes_bs;
     int causal;
     // x = log2-domain score: s c, or with a cap cap2 tanh(s / softcap) from
-    // e = exp2(s k1) (see attn_cap)
+    // e = exp2(s k1) (see attn_tanh)
     float c, k1, cap2;
     int cap_fine;  // caps large enough that small scores need tanh's series
 };
@@ -51,7 +51,6 @@ struct AttnProblem {
     bool causal, bias, docs;
 };
 
-constexpr int kAttnTile = 64;   // keys (or rows) streamed per step
 // Workgroups of a launch are held below this: their 256 threads count in 32 bits.
 constexpr int64_t kMaxGrid = 1 << 24;
 constexpr int kAttnRows = 128;  // rows (or keys) resident per workgroup

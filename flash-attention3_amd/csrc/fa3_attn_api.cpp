@@ -188,7 +188,7 @@ int shaobo_fa3_rotary(const ShaoboFa3RotaryParams* params, void* stream) {
         p->dtype != SHAOBO_FA3_DTYPE_FP32)
         return SHAOBO_FA3_STATUS_UNSUPPORTED;
     if (p->head_dim > 512 || p->head_dim % 8 != 0 || p->pairs % 8 != 0 || p->pairs < 8 ||
-        2 * p->pairs > p->head_dim || p->axes > 4)
+        p->pairs > p->head_dim / 2 || p->axes > 4)
         return SHAOBO_FA3_STATUS_UNSUPPORTED;
     const int align = p->dtype == SHAOBO_FA3_DTYPE_FP32 ? 4 : 8;
     for (int k = 0; k < p->tensors; ++k) {

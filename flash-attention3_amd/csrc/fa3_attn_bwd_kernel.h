@@ -12,11 +12,12 @@
 //
 // What bounds it.  As bwd_reg_kernel, power and two waves' products, LDS reads
 // and exponentials on one SIMD in large launches: B2 Hq32 Hkv8 S4096 D128
-// causal 852 us (806 TFLOP/s of five products), documents of ~1500 tokens 676
-// us (506 of the visible work; a document of 3391 tokens among them makes
-// the longest job).  Small ones are bound by a job's chain, hence the cuts of
-// plan_attn_bwd.  dQ recomputes S and dP (seven products instead of five):
-// adding dS K across workgroups would need atomics or an S^2-sized workspace.
+// causal 852-872 us (806-788 TFLOP/s of five products), documents of ~1500
+// tokens 656-676 us (521-506 of the visible work; a document of 3391 tokens
+// among them makes the longest job).  Small ones are bound by a job's chain,
+// hence the cuts of plan_attn_bwd.  dQ recomputes S and dP (seven products
+// instead of five): adding dS K across workgroups would need atomics or an
+// S^2-sized workspace.
 #pragma once
 
 #include "fa3_attn_device.h"

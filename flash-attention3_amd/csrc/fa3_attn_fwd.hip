@@ -12,14 +12,14 @@
 // What bounds it.  The vector units as much as the matrix units: an element
 // costs 16 cycles of exponential and about 16 more (a fma, a sum, half a
 // maximum, half a conversion), a cap 40 on top, against 2 D / 8 cycles of
-// products.  Measured: B2 Hq32 Hkv8 S4096 D128 causal 280 us (980 TFLOP/s),
-// B2 H16 S8192 D64 full 627 us (877) and with a distance bias 597 (921 of the
-// nominal work: tiles without weight are left), documents of ~1500 tokens at
-// S4096 171 us (684 of the visible work).  Small launches are bound by one
-// wave's chain, ~2 600 cycles a 32 x 32 step of which 512 are products:
-// making the next tile's scores behind this tile's exponentials (a pipeline
-// within the wave) did not shorten it (S2011 capped 48.9 -> 52.2 us), nor did
-// sending the loads out later.
+// products.  Measured, from box to box: B2 Hq32 Hkv8 S4096 D128 causal 280-299
+// us (980-920 TFLOP/s), B2 H16 S8192 D64 full 627-662 us (877-830) and with a
+// distance bias 555-600 (990-916 of the nominal work: tiles without weight are
+// left), documents of ~1500 tokens at S4096 162-171 us (722-684 of the visible
+// work).  Small launches are bound by one wave's chain, ~2 600 cycles a 32 x 32
+// step of which 512 are products: making the next tile's scores behind this
+// tile's exponentials (a pipeline within the wave) did not shorten it (S2011
+// capped 48.9 -> 52.2 us), nor did sending the loads out later.
 #include "fa3_attn_device.h"
 
 namespace fa3 {
@@ -529,7 +529,7 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(
 // each, through two LDS stages of their own -- no barrier until they meet.
 // Bound by reading the cache: 5.4 TB/s for 16 caches of 8192 keys (Hkv 8, D
 // 128, 99 us, the rate of a large copy), 4.9 where they are filled to
-// different lengths (68.8 us).
+// different lengths (64-69 us).
 template <int D>
 struct TokenCfg {
     static constexpr int kBlock = 32 * D * 2;   // 32 rows of K or V

@@ -3,8 +3,8 @@
 // A workgroup takes one to eight tokens: it forms their cosines and sines
 // once, in LDS, and turns every head's row with them, 16 bytes (or 16 and
 // their partners') a thread at a time.  Bound by HBM, x read once and written
-// once: B2 S8192 Hq32 + Hkv8 D128 bf16 69 us, 4.8 TB/s, a large copy's rate.
-// Angles are sum_a positions[a] freqs[a][p], reduced to [-1/2, 1/2] turns in
+// once: B2 S8192 Hq32 + Hkv8 D128 bf16 66-69 us, 4.9-5.1 TB/s, a large copy's
+// rate.  Angles are sum_a positions[a] freqs[a][p], reduced to [-1/2, 1/2] turns in
 // fp64 with what its products round off carried along (axis_turns): at a
 // million positions an fp32 product would be off by 0.06 radians, at 2^40 an
 // fp64 one by 0.0002.

@@ -20,9 +20,10 @@
  *   out_i   = sum_j softmax(s)_ij v_j over the visible keys; 0 if none is
  *   lse_i   = log sum_j exp(s_ij);                        -inf if none is
  * The backward returns dq, dk, dv of these outputs from out and lse; slopes
- * have no gradient.  Sums, softmax statistics and dot products are fp32; P
- * and dS are rounded to the tensors' type before their products with V, dO,
- * Q and K, and the outputs once more.  Results are bitwise reproducible.
+ * have no gradient.  Sums, softmax statistics, dot products and biases are
+ * fp32; P and dS are rounded to the tensors' type before their products with
+ * V, dO, Q and K, and the outputs once more (in fp16 a dS below 2^-14 loses
+ * bits as gradients do: scale the loss).  Results are bitwise reproducible.
  *
  * Keys at kv and behind, and keys with a negative document, take no part
  * whatever their K and V hold (NaN included), and neither do queries that

@@ -9,7 +9,7 @@ import pytest
 import attn_differences as X
 import attn_oracle as A
 import shaobo_fa3 as F
-from test_gpu_attn import BF, HF, make, op_args, oracle_options, randn
+from test_gpu_attn import BF, HF, make, op_args, oracle_options, randn, within
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -252,3 +252,31 @@ def test_rotary_at_far_positions(T, bits, axes, kind, inverse):
     for g, want in zip(got, (a * angle.cos() - b * angle.sin(), b * angle.cos() + a * angle.sin())):
         off = (a.abs() + b.abs()) * 2.0 ** -21 + 2.0 ** -24 * want.abs()
         assert ((g - want).abs() <= off).all(), float(((g - want).abs() - off).max())
+
+
+@pytest.mark.parametrize("B,Hq,Hkv,S,D,causal,dtype", [
+    (1, 4, 4, 384, 128, True, HF), (2, 8, 2, 256, 64, True, BF), (1, 4, 1, 512, 128, False, BF),
+    (2, 3, 3, 128, 64, False, HF)])
+def test_the_forward_feeds_either_backward(T, monkeypatch, B, Hq, Hkv, S, D, causal, dtype):
+    """Without options both backwards are the gradient of attn_forward, within
+    the oracle's bound.  The other one's operands may carry the scale: a score
+    is off by half a step of each of its products then, and an operand of the
+    last products by half a step more, as much as dS (so twice that bound)."""
+    print("[case] either backward", B, Hq, Hkv, S, D, causal, dtype, flush=True)
+    q, k, v, do, o = make(dict(B=B, Hq=Hq, Hkv=Hkv, Sq=S, D=D, causal=causal, dtype=dtype))
+    out, lse = torch.ops.shaobo_fa3.attn_forward(q, k, v, causal)
+    both = (torch.ops.shaobo_fa3.attn_backward(do, q, k, v, out, lse, causal),
+            torch.ops.shaobo_fa3.flash_attn_backward(do, q, k, v, out, lse, causal))
+    torch.cuda.synchronize()
+    init, u = A.Head.__init__, torch.finfo(dtype).eps / 2
+
+    def scaled(self, q, k, scale, *rest):
+        init(self, q, k, scale, *rest)
+        self.dx = self.dx + u * scale * (self.q.abs() @ self.k.abs().t().contiguous()) * self.seen
+
+    want = [A.backward(do, q, k, v, out, lse, causal)]
+    monkeypatch.setattr(A.Head, "__init__", scaled)
+    want.append(A.backward(do, q, k, v, out, lse, causal))
+    for times, grads, w in zip((1, 2), both, want):
+        for n, g in zip(("dq", "dk", "dv", "delta"), grads):
+            within(n, g, w[n][0], times * w[n][1])

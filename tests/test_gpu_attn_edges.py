@@ -1,5 +1,6 @@
 """The attention layer where autograd, other rows' values and padding meet it
 in ways that the plain cases do not."""
+import functools
 import math
 from concurrent.futures import ThreadPoolExecutor
 from fractions import Fraction
@@ -12,6 +13,8 @@ import shaobo_fa3 as F
 from test_gpu_attn import BF, HF, make, op_args, oracle_options, randn, within
 
 torch = pytest.importorskip("torch")
+import torch.utils.checkpoint  # noqa: E402
+
 pytestmark = pytest.mark.gpu
 
 
@@ -280,3 +283,46 @@ def test_the_forward_feeds_either_backward(T, monkeypatch, B, Hq, Hkv, S, D, cau
     for times, grads, w in zip((1, 2), both, want):
         for n, g in zip(("dq", "dk", "dv", "delta"), grads):
             within(n, g, w[n][0], times * w[n][1])
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_documents_are_any_numbers(T, causal):
+    """Only the numbers' order and sign count, up to the type's last ones."""
+    print("[case] document numbers", causal, flush=True)
+    q, k, v, do, o = make(dict(Sq=400, Hq=4, D=64, causal=causal))
+    small = torch.tensor([0, 1, 2, 3, -1], dtype=torch.int32, device="cuda")
+    large = torch.tensor([0, 70000, 2147483646, 2147483647, -2147483648], dtype=torch.int32, device="cuda")
+    for pick in (torch.arange(400, device="cuda") // 90, torch.arange(400, device="cuda") * 7 % 5,
+                 torch.full((400,), 3, device="cuda")):
+        got = []
+        for names in (small, large):
+            o["documents"] = names[pick][None].expand(2, 400).contiguous()
+            out, lse = torch.ops.shaobo_fa3.attn_forward(q, k, v, *op_args(o))
+            got.append((out, lse, *torch.ops.shaobo_fa3.attn_backward(do, q, k, v, out, lse, *op_args(o))))
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(*got))
+
+
+def test_layers_under_tracing_and_recomputation(T):
+    """The layer traced through the operators' fake implementations, and
+    recomputed in its backward: the eager step's outputs and gradients."""
+    print("[case] tracing", flush=True)
+    q, k, v, do, o = make(dict(Sq=100, Hq=4, D=64, docs=30.0, bshd=True))
+    pos = torch.arange(100, device="cuda").expand(1, 2, 100)
+    freqs = T.rotary_freqs([32], device="cuda")
+
+    def layer(q, k, v):
+        q, k = T.rotary(q, k, positions=pos, freqs=freqs)
+        return T.score_attention(q, k, v, softcap=10.0, documents=o["documents"])
+
+    def step(f):
+        xs = [t.detach().clone(memory_format=torch.preserve_format).requires_grad_() for t in (q, k, v)]
+        out = f(*xs)
+        out.backward(do)
+        return [out.detach()] + [x.grad for x in xs]
+
+    want = step(layer)
+    traced = torch.compile(layer, backend="aot_eager")
+    again = functools.partial(torch.utils.checkpoint.checkpoint, layer, use_reentrant=False)
+    for f in (traced, again):
+        assert all(torch.equal(x, y) for x, y in zip(want, step(f)))

@@ -14,11 +14,6 @@ namespace {
 using fa3::AttnMask;
 using fa3::AttnProblem;
 
-constexpr float kLog2E = 1.44269504088896340736f;
-// Caps over this take tanh's series for small scores (fa3_attn_device.h,
-// attn_tanh_fine): below it the plain form's error, the cap times 2^-23, is
-// under 1.2e-5 of a score's unit.
-constexpr float kCapFine = 100.f;
 // Sequences and head counts are held below these, so that rows, tiles and
 // jobs count in 32 bits (their products are checked by the plans).
 constexpr int32_t kMaxLen = 1 << 30;
@@ -90,14 +85,7 @@ AttnMask mask_of(const ShaoboFa3AttnParams& a, const AttnProblem& p) {
     m.slopes = a.slopes;
     m.slopes_bs = a.slopes_batch_stride;
     m.causal = a.causal;
-    m.c = p.scale * kLog2E;
-    if (p.softcap > 0.f) {
-        // (a tiny cap: the largest fp32, so that a score of zero stays one)
-        const double k1 = 2.0 * p.scale / p.softcap * kLog2E;
-        m.k1 = (float)std::fmin(std::fmax(k1, -3e38), 3e38);
-        m.cap2 = p.softcap * kLog2E;
-        m.cap_fine = p.softcap > kCapFine;
-    }
+    fa3::set_scores(&m, p.scale, p.softcap);
     return m;
 }
 

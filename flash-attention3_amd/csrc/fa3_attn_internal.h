@@ -43,6 +43,23 @@ struct AttnMask {
     int cap_fine;  // caps large enough that small scores need tanh's series
 };
 
+// Caps over this take tanh's series for small scores (fa3_attn_device.h,
+// attn_tanh_fine): below it the plain form's error, the cap times 2^-23, is
+// under 1.2e-5 of a score's unit.
+constexpr float kCapFine = 100.f;
+// A mask's score options from a scale and a cap (0: none).
+inline void set_scores(AttnMask* m, float scale, float softcap) {
+    constexpr float kLog2E = 1.44269504088896340736f;
+    m->c = scale * kLog2E;
+    if (softcap > 0.f) {
+        // (a tiny cap: the largest fp32, so that a score of zero stays one)
+        const double k1 = 2.0 * scale / softcap * kLog2E;
+        m->k1 = (float)(k1 < -3e38 ? -3e38 : k1 > 3e38 ? 3e38 : k1);
+        m->cap2 = softcap * kLog2E;
+        m->cap_fine = softcap > kCapFine;
+    }
+}
+
 // A resolved problem: checked, default scale applied.
 struct AttnProblem {
     int batch, heads_q, heads_kv, group, sq, sk, d;
@@ -56,6 +73,23 @@ constexpr int64_t kMaxGrid = 1 << 24;
 constexpr int kAttnRows = 128;  // rows (or keys) resident per workgroup
 
 inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
+
+// The forward kernels' arguments.
+struct AttnFwdArgs {
+    static constexpr bool kPaged = false;
+    AttnView q, k, v, out;
+    float* lse;
+    float* part_o;  // splits > 1: [splits][groups * rows][D] fp32
+    float* part_l;  //             [splits][groups * rows]
+    AttnMask m;
+    int heads_q, heads_kv, group, sq, sk, d;
+    int rows;  // group * sq
+    int tiles, splits, part, groups;
+    uint32_t flip;  // XORed into Q's 16-bit pairs
+    int scored;     // 0: a scale of zero, Q is taken as zeros
+    int levels, by_group;
+    FastDiv div_hkv, div_group, div_groups, div_gpart, div_splits, div_levels;
+};
 
 struct AttnFwdPlan {
     bool token;  // the kernel for few rows

@@ -1,0 +1,339 @@
+// Few rows of a KV head against 4-bit pages: 16 kBlocks rows a workgroup,
+// whose four waves all hold them and take every fourth block of 32 keys each,
+// straight from HBM to registers.
+//
+// A lane's share of a block, with r = lane % 16 and g = lane / 16:
+//   K   16 bytes (D 64: 8) of rows r and 16 + r, channels D / 4 g ..: the A
+//       operand of S^T = K Q^T whose k-step s stands for the channels D / 4 g +
+//       8 s .. of each g, in Q's operand too; a row's codes are read once by
+//       four lanes that lie together;
+//   V   the D / 16 channels D / 16 r .. of the rows 4 g + 0..3 and 16 + 4 g +
+//       0..3, whose scores are the lane's own: two rows' codes of a channel put
+//       side by side in a byte become two levels side by side, a pair of the A
+//       operand of O^T += V^T P^T (two shifts and two selects for 16 codes,
+//       then one conversion for two levels);
+//   scales  of those rows, K's and V's.
+// Levels are exact, the scale of K meets the fp32 score, that of V meets P
+// before its rounding to bf16.  Two blocks' loads are out at a time; there is
+// no barrier before the waves meet.
+#pragma once
+
+#include "fa3_cache_attn_kernel.h"
+
+namespace fa3 {
+namespace {
+
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+template <int D>
+struct FourBlock {
+    typedef typename std::conditional<D == 128, u32x4, u32x2>::type Codes;
+    typedef typename std::conditional<D == 128, uint32_t, uint16_t>::type Piece;
+    Codes k[2];
+    Piece v[8];
+    f32x4 ks[2], vs[2];
+
+    // row: the block's first in its page; pk, pv: the page and head
+    __device__ __forceinline__ void load(const char* pk, const char* pv, int row, int shift,
+                                         int lane) {
+        const int l16 = lane & 15, g4 = lane >> 4;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            k[t] = *(const Codes*)(pk + (row + 16 * t + l16) * (D / 2) + g4 * (D / 8));
+            const int at = (D / 2 << shift) + (row + 16 * t + 4 * g4) * 4;
+            ks[t] = *(const f32x4*)(pk + at);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                v[4 * t + e] = *(const Piece*)(pv + (row + 16 * t + 4 * g4 + e) * (D / 2) + l16 * (D / 32));
+            vs[t] = *(const f32x4*)(pv + at);
+        }
+    }
+};
+
+template <int D, int kBlocks>
+struct FourCfg {
+    static constexpr int kDB = D / 16;
+    static constexpr int kSlot = kBlocks * (kDB * 1024 + 256);  // a wave's outputs and sums
+    static constexpr int kMax = 4 * kBlocks * 256;              // the waves' maxima
+    static constexpr int kBytes = kMax + 3 * kSlot;
+};
+
+template <int D, bool kBf16, bool kCap, bool kBias, int kBlocks>
+__global__ __launch_bounds__(kRegThreads, kBlocks == 1 ? 3 : 2) void cache_four_kernel(CacheAttnArgs) {
+    typedef CacheAttnArgs Args;
+    const auto& a = attn_args<Args>();
+    using C = FourCfg<D, kBlocks>;
+    constexpr int kKs = D / 32, kDB = D / 16;
+    constexpr float kLazy = 8.f;  // as FwdRows: rescaled only past 2^8
+    __shared__ __attribute__((aligned(16))) char smem_raw[C::kBytes];
+    FA3_LDS char* smem = (FA3_LDS char*)smem_raw;
+    const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = lane >> 4;
+    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const CacheJob job = cache_job(a, blockIdx.x, 16 * kBlocks);
+    const CacheSpan span = cache_span(a, job);
+    const int first = span.begin + w, end = span.end;
+    const int n = end > first ? (end - first + 3) >> 2 : 0;
+    const char* kh = a.x.cv.k + job.hkv * a.x.cv.k_hs;
+    const char* vh = a.x.cv.v + job.hkv * a.x.cv.v_hs;
+    const int64_t k_ps = a.x.cv.k_ps, v_ps = a.x.cv.v_ps;
+    const int shift = a.x.cv.shift;
+    auto issue = [&](FourBlock<D>& f, const CacheBlock& x) {
+        if (x.page < 0) return;
+        f.load(kh + x.page * k_ps, vh + x.page * v_ps, x.j0 & ((1 << shift) - 1), shift,
+               opaque_tid() & 63);
+    };
+    FourBlock<D> f0, f1;
+    CacheBlock b0 = cache_block(a, job, first, end);
+    issue(f0, b0);
+    CacheBlock b1 = cache_block(a, job, first + 4, end);
+    issue(f1, b1);
+
+    f16x8 qf[kBlocks][kKs];
+    int lim[kBlocks], place[kBlocks];
+    float slope[kBlocks], mx[kBlocks], sum[kBlocks];
+    f32x4 o[kDB][kBlocks];  // channels kDB (4 g4 + e) + i of row l16
+#pragma unroll
+    for (int q = 0; q < kBlocks; ++q) {
+        const AttnRow r = attn_row(job.row0 + 16 * q + l16, job.rows, job.hkv, a.group, a.div_group);
+        const _Float16* p = a.q.p + job.b * a.q.bs + r.h * a.q.hs + r.i * a.q.rs;
+#pragma unroll
+        for (int s = 0; s < kKs; ++s)
+            qf[q][s] = attn_flip(attn_row8(p, D / 32 * g4 + s, D, r.ok && a.scored), a.flip);
+        lim[q] = r.ok ? attn_limit(r.i, job.off, job.kv, a.m.causal, job.prefix) : 0;
+        place[q] = r.i + job.off;
+        slope[q] = kBias ? a.m.slopes[job.b * a.m.slopes_bs + r.h] * kLog2e : 0.f;
+        mx[q] = kNegInf;
+        sum[q] = 0.f;
+#pragma unroll
+        for (int i = 0; i < kDB; ++i) o[i][q] = f32x4{};
+    }
+    // below it every row sees every key
+    int lim_min = 0x7fffffff;
+    if (min(job.row0 + 16 * kBlocks, job.end) > job.rows) lim_min = 0;
+    else lim_min = attn_limit(fdiv(a.div_group, job.row0), job.off, job.kv, a.m.causal, job.prefix);
+    const float c = a.m.c, k1 = kCap ? a.m.k1 : 0.f, cap2 = kCap ? a.m.cap2 : 0.f;
+    const bool fine = kCap && a.m.cap_fine;
+    const int kv = job.kv;
+
+    auto step = [&](FourBlock<D>& f, int j0) {
+        f32x4 s[2][kBlocks];
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int q = 0; q < kBlocks; ++q) s[t][q] = f32x4{};
+#pragma unroll
+            for (int i = 0; i < kKs; ++i) {
+                const f16x8 x = cache_levels8<kBf16>(f.k[t][i]);
+#pragma unroll
+                for (int q = 0; q < kBlocks; ++q)
+                    s[t][q] = mfma_16x16x32<kBf16>(x, qf[q][i], s[t][q]);
+            }
+#pragma unroll
+            for (int q = 0; q < kBlocks; ++q) s[t][q] *= f.ks[t];
+        }
+        // log2-domain scores
+#pragma unroll
+        for (int q = 0; q < kBlocks; ++q)
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    float x = s[t][q][e];
+                    if constexpr (kCap)
+                        x = (fine ? attn_tanh_fine(x, k1) : attn_tanh(x, k1)) * cap2;
+                    else
+                        x *= c;
+                    if constexpr (kBias)
+                        x = __builtin_fmaf(-slope[q], __builtin_fabsf((float)(place[q] - (j0 + 16 * t + 4 * g4 + e))), x);
+                    s[t][q][e] = x;
+                }
+        if (j0 + 32 > lim_min) {
+#pragma unroll
+            for (int q = 0; q < kBlocks; ++q) {
+                const int k = lim[q] - (j0 + 4 * g4);
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e)
+                        s[t][q][e] = 16 * t + e < k ? s[t][q][e] : kNegInf;
+            }
+        }
+        if (j0 + 32 > kv) {  // (rows behind the sequence hold anything)
+            const int k = kv - (j0 + 4 * g4);
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) f.vs[t][e] = 16 * t + e < k ? f.vs[t][e] : 0.f;
+        }
+        float top[kBlocks];
+        bool up = false;
+#pragma unroll
+        for (int q = 0; q < kBlocks; ++q) {
+            float x = s[0][q][0];
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) x = __builtin_elementwise_maximum(x, s[t][q][e]);
+            top[q] = max_groups(x);
+            up |= top[q] > mx[q] + kLazy;
+        }
+        if (__ballot(up)) {
+#pragma unroll
+            for (int q = 0; q < kBlocks; ++q) {
+                const float m = __builtin_fmaxf(mx[q], top[q]);
+                const float y = mx[q] == kNegInf ? 0.f : fast_exp2(mx[q] - m);
+                mx[q] = m;
+                sum[q] *= y;
+#pragma unroll
+                for (int i = 0; i < kDB; ++i) o[i][q] *= y;
+            }
+        }
+        f16x8 bp[kBlocks];
+#pragma unroll
+        for (int q = 0; q < kBlocks; ++q) {
+            const float m = mx[q] == kNegInf ? 0.f : mx[q];
+            float p[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                p[j] = fast_exp2(s[j >> 2][q][j & 3] - m);
+                sum[q] += p[j];
+                p[j] *= f.vs[j >> 2][j & 3];
+            }
+            bp[q] = pack8<true>(p);
+        }
+        // x[j][0]: even channels' codes of two rows, a byte each; x[j][1]: odd ones'
+        uint32_t x[4][2];
+        if constexpr (D == 128) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t y = f.v[2 * j], z = f.v[2 * j + 1];
+                x[j][0] = (y & 0x0F0F0F0Fu) | ((z << 4) & 0xF0F0F0F0u);
+                x[j][1] = ((y >> 4) & 0x0F0F0F0Fu) | (z & 0xF0F0F0F0u);
+            }
+        } else {  // (bytes 0, 1: rows 2 j and 2 j + 1; bytes 2, 3: 2 j + 4 and 2 j + 5)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t y = f.v[2 * j] | ((uint32_t)f.v[2 * j + 4] << 16);
+                const uint32_t z = f.v[2 * j + 1] | ((uint32_t)f.v[2 * j + 5] << 16);
+                x[j][0] = (y & 0x0F0F0F0Fu) | ((z << 4) & 0xF0F0F0F0u);
+                x[j][1] = ((y >> 4) & 0x0F0F0F0Fu) | (z & 0xF0F0F0F0u);
+                x[j + 2][0] = x[j][0] >> 16;
+                x[j + 2][1] = x[j][1] >> 16;
+            }
+        }
+        auto product = [&](auto sel) {
+            constexpr int kSel = decltype(sel)::value;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const u32x4 y = {cache_levels<true, kSel>(x[0][h]), cache_levels<true, kSel>(x[1][h]),
+                                 cache_levels<true, kSel>(x[2][h]), cache_levels<true, kSel>(x[3][h])};
+#pragma unroll
+                for (int q = 0; q < kBlocks; ++q)
+                    o[2 * kSel + h][q] = mfma_16x16x32<true>(__builtin_bit_cast(f16x8, y), bp[q], o[2 * kSel + h][q]);
+            }
+        };
+        product(std::integral_constant<int, 0>{});
+        product(std::integral_constant<int, 1>{});
+        if constexpr (D == 128) {
+            product(std::integral_constant<int, 2>{});
+            product(std::integral_constant<int, 3>{});
+        }
+    };
+    for (int x = 0; x < n; x += 2) {
+        const CacheBlock b2 = cache_block(attn_args<Args>(), job, first + 4 * x + 8, end);
+        if (b0.page >= 0) step(f0, b0.j0);
+        b0 = b2;
+        issue(f0, b0);
+        const CacheBlock b3 = cache_block(attn_args<Args>(), job, first + 4 * x + 12, end);
+        if (b1.page >= 0) step(f1, b1.j0);
+        b1 = b3;
+        issue(f1, b1);
+    }
+
+    // A row without a maximum but with a sum has met NaN (FwdRows::settle).
+    const auto& z = attn_args<Args>();
+    const CacheJob e = cache_job(z, blockIdx.x, 16 * kBlocks);
+#pragma unroll
+    for (int q = 0; q < kBlocks; ++q) {
+        sum[q] = sum_groups(sum[q]);
+        const bool odd = mx[q] == kNegInf && sum[q] != 0.f;
+        if (!__ballot(odd)) continue;
+        const bool some = cache_sees(z, e.row0 + 16 * q + l16, e.b, e.hkv, g4);
+        if (odd && !some) sum[q] = 0.f;
+    }
+    // The waves meet: sums and outputs at the largest maximum, wave 0 adds.
+    FA3_LDS float* xm = (FA3_LDS float*)smem;
+#pragma unroll
+    for (int q = 0; q < kBlocks; ++q) xm[(w * kBlocks + q) * 64 + lane] = mx[q];
+    wait_vm_lgkm0<0>();
+    barrier();
+    FA3_LDS char* slots = smem + C::kMax;
+#pragma unroll
+    for (int q = 0; q < kBlocks; ++q) {
+        float m = kNegInf;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) m = __builtin_fmaxf(m, xm[(k * kBlocks + q) * 64 + lane]);
+        const float y = mx[q] == kNegInf && sum[q] == 0.f ? 0.f : fast_exp2(mx[q] - (m == kNegInf ? 0.f : m));
+        // (a NaN that is one: mx -inf, y 0, and the sum stays NaN)
+        mx[q] = m;
+        sum[q] *= y;
+        if (y == 0.f && sum[q] == 0.f) {  // (other rows' V may have been NaN)
+#pragma unroll
+            for (int i = 0; i < kDB; ++i) o[i][q] = f32x4{};
+        } else {
+#pragma unroll
+            for (int i = 0; i < kDB; ++i) o[i][q] *= y;
+        }
+    }
+    if (w > 0) {
+        FA3_LDS char* slot = slots + (w - 1) * C::kSlot;
+#pragma unroll
+        for (int q = 0; q < kBlocks; ++q) {
+#pragma unroll
+            for (int i = 0; i < kDB; ++i)
+                *(FA3_LDS f32x4*)(slot + (q * kDB + i) * 1024 + lane * 16) = o[i][q];
+            *(FA3_LDS float*)(slot + kBlocks * kDB * 1024 + q * 256 + lane * 4) = sum[q];
+        }
+    }
+    wait_vm_lgkm0<0>();
+    barrier();
+    if (w > 0) return;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+        FA3_LDS char* slot = slots + k * C::kSlot;
+#pragma unroll
+        for (int q = 0; q < kBlocks; ++q) {
+#pragma unroll
+            for (int i = 0; i < kDB; ++i)
+                o[i][q] += *(FA3_LDS f32x4*)(slot + (q * kDB + i) * 1024 + lane * 16);
+            sum[q] += *(FA3_LDS float*)(slot + kBlocks * kDB * 1024 + q * 256 + lane * 4);
+        }
+    }
+#pragma unroll
+    for (int q = 0; q < kBlocks; ++q) {
+        const int row = e.row0 + 16 * q + l16;
+        if (row >= e.end) continue;
+        const bool none = mx[q] == kNegInf && sum[q] == 0.f;
+        const float inv = none ? 0.f : 1.f / sum[q];
+        const float lse2 = none ? kNegInf : mx[q] + __builtin_amdgcn_logf(sum[q]);
+        float y[4 * kDB];  // channels 4 kDB g4 ..
+#pragma unroll
+        for (int i = 0; i < 4 * kDB; ++i) y[i] = none ? 0.f : o[i % kDB][q][i / kDB] * inv;
+        if (z.splits > 1) {
+            const int64_t at = ((int64_t)e.split * z.groups + e.grp) * z.rows + row;
+            if (g4 == 0) z.part_l[at] = lse2;
+            float* p = z.part_o + at * D + 4 * kDB * g4;
+#pragma unroll
+            for (int i = 0; i < kDB; ++i) *(f32x4*)(p + 4 * i) = *(const f32x4*)(y + 4 * i);
+            continue;
+        }
+        const AttnRow r = attn_row(row, e.end, e.hkv, z.group, z.div_group);
+        if (g4 == 0) z.lse[((int64_t)e.b * z.heads_q + r.h) * z.sq + r.i] = lse2 * 0.69314718055994531f;
+        _Float16* p = z.out.p + e.b * z.out.bs + r.h * z.out.hs + r.i * z.out.rs + 4 * kDB * g4;
+#pragma unroll
+        for (int i = 0; i < kDB / 2; ++i) *(f16x8*)(p + 8 * i) = pack8<kBf16>(y + 8 * i);
+    }
+}
+
+}  // namespace
+}  // namespace fa3

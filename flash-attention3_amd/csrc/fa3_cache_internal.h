@@ -1,0 +1,83 @@
+// Host-side interface between the paged cache's C entries (fa3_cache_api.cpp)
+// and its kernels.  Nothing here is exported.
+#pragma once
+
+#include "fa3_attn_internal.h"
+#include "shaobo_fa3_cache.h"
+
+namespace fa3 {
+
+// A cache as the kernels take it; strides in bytes.
+struct CacheView {
+    char *k, *v;
+    int64_t k_ps, k_hs, k_rs, v_ps, v_hs, v_rs;
+    const int* table;
+    int64_t table_s;
+    const int* kv_lens;
+    const int* new_lens;  // null: all
+    int pages, width, shift;  // a page has 1 << shift rows
+};
+
+// A resolved attention problem.
+struct CacheProblem {
+    int batch, heads_q, heads_kv, group, sq, d;
+    int sk;  // places of a sequence's pages
+    int page, count;  // count 0: every page
+    bool bf16, four, causal, bias;
+    float scale, softcap;
+};
+
+struct CacheAttnExtra {
+    CacheView cv;
+    const int* selected;  // [batch * heads_kv][sq][count], or null
+    int count, per_query;
+    FastDiv div_per_query;
+};
+struct CacheAttnArgs : AttnFwdArgs {
+    static constexpr bool kPaged = true;
+    CacheAttnExtra x;
+};
+
+struct CachePlan {
+    bool token;   // a kernel for few rows
+    int row_tile; // rows of its jobs: 16 or 32
+    int split;    // otherwise: workgroups of 128 / split rows
+    int tiles;    // row tiles of a KV head (selected pages: of all its queries)
+    int per_query;  // selected pages: row tiles of one query's heads
+    int splits;   // parts of the key axis
+    int jobs;
+    size_t po_off, pl_off, total;
+    bool ok;
+};
+CachePlan plan_cache_attn(const CacheProblem& p);
+
+// Pages that one workgroup of the scoring kernel takes, and its plan.
+struct CacheSelectPlan {
+    int chunks;  // parts of a sequence's pages, scored by a workgroup each
+    size_t total;
+    bool ok;
+};
+CacheSelectPlan plan_cache_select(const ShaoboFa3CacheSelectParams& p);
+
+// How an append's workgroups share the tokens and heads.
+struct AppendGrid {
+    int units, run, segments, hq, hk, parts_q, parts_k;
+    size_t lds;
+    bool ok;
+};
+AppendGrid append_grid(const ShaoboFa3CacheAppendParams& p);
+
+CacheView cache_view(const ShaoboFa3Cache& c);
+
+hipError_t launch_cache_append(const ShaoboFa3CacheAppendParams& p, hipStream_t stream);
+hipError_t launch_cache_read(const ShaoboFa3CacheReadParams& p, hipStream_t stream);
+hipError_t launch_cache_select(const ShaoboFa3CacheSelectParams& p, hipStream_t stream);
+// The attention kernels, compiled one file per head dim and bits.
+void launch_cache_d64_16(const CacheAttnArgs&, const CacheProblem&, const CachePlan&, hipStream_t);
+void launch_cache_d128_16(const CacheAttnArgs&, const CacheProblem&, const CachePlan&, hipStream_t);
+void launch_cache_d64_4(const CacheAttnArgs&, const CacheProblem&, const CachePlan&, hipStream_t);
+void launch_cache_d128_4(const CacheAttnArgs&, const CacheProblem&, const CachePlan&, hipStream_t);
+hipError_t launch_cache_attn(const CacheProblem& p, const ShaoboFa3CacheAttnParams& a, AttnMask m,
+                             hipStream_t stream);
+
+}  // namespace fa3

@@ -153,6 +153,71 @@ class RotaryParams(ctypes.Structure):
         ("in_", AttnTensor * 2), ("out", AttnTensor * 2)]
 
 
+class CachePages(ctypes.Structure):
+    """ShaoboFa3CachePages (include/shaobo_fa3_cache.h)."""
+    _fields_ = [("data", ctypes.c_void_p), ("page_stride", ctypes.c_int64),
+                ("head_stride", ctypes.c_int64), ("row_stride", ctypes.c_int64)]
+
+
+class Cache(ctypes.Structure):
+    """ShaoboFa3Cache (include/shaobo_fa3_cache.h)."""
+    _fields_ = [(n, ctypes.c_int32) for n in ("batch", "num_heads_kv", "head_dim", "dtype", "bits",
+                                              "pages", "page_size", "width")] + [
+        ("k", CachePages), ("v", CachePages), ("page_table", ctypes.c_void_p),
+        ("page_table_stride", ctypes.c_int64), ("kv_lens", ctypes.c_void_p),
+        ("new_lens", ctypes.c_void_p), ("bounds", ctypes.c_void_p)]
+
+
+class CacheAppendParams(ctypes.Structure):
+    """ShaoboFa3CacheAppendParams (include/shaobo_fa3_cache.h)."""
+    _fields_ = [("struct_size", ctypes.c_uint32)] + [
+        (n, ctypes.c_int32) for n in ("seqlen", "num_heads_q", "axes", "pairs", "interleaved",
+                                      "position_type")] + [
+        ("cache", Cache), ("k", AttnTensor), ("v", AttnTensor), ("q", AttnTensor),
+        ("q_out", AttnTensor), ("positions", ctypes.c_void_p),
+        ("position_axis_stride", ctypes.c_int64), ("position_batch_stride", ctypes.c_int64),
+        ("position_row_stride", ctypes.c_int64), ("freqs", ctypes.c_void_p)]
+
+
+class CacheAttnParams(ctypes.Structure):
+    """ShaoboFa3CacheAttnParams (include/shaobo_fa3_cache.h)."""
+    _fields_ = [("struct_size", ctypes.c_uint32)] + [
+        (n, ctypes.c_int32) for n in ("seqlen", "num_heads_q", "causal", "softmax_scale_is_set")] + [
+        ("softmax_scale", ctypes.c_float), ("softcap", ctypes.c_float), ("count", ctypes.c_int32),
+        ("cache", Cache), ("q", AttnTensor), ("out", AttnTensor), ("softmax_lse", ctypes.c_void_p),
+        ("slopes", ctypes.c_void_p), ("slopes_batch_stride", ctypes.c_int64),
+        ("prefix_lens", ctypes.c_void_p), ("selected", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class CacheSelectParams(ctypes.Structure):
+    """ShaoboFa3CacheSelectParams (include/shaobo_fa3_cache.h)."""
+    _fields_ = [("struct_size", ctypes.c_uint32)] + [
+        (n, ctypes.c_int32) for n in ("seqlen", "num_heads_q", "count")] + [
+        ("cache", Cache), ("q", AttnTensor), ("selected", ctypes.c_void_p),
+        ("workspace", ctypes.c_void_p), ("workspace_bytes", ctypes.c_size_t)]
+
+
+class CacheReadParams(ctypes.Structure):
+    """ShaoboFa3CacheReadParams (include/shaobo_fa3_cache.h)."""
+    _fields_ = [("struct_size", ctypes.c_uint32), ("seqlen", ctypes.c_int32), ("cache", Cache),
+                ("k", AttnTensor), ("v", AttnTensor)]
+
+
+def _declare_cache(lib):
+    for name, cls, sized in (("append", CacheAppendParams, False), ("attn", CacheAttnParams, True),
+                             ("select", CacheSelectParams, True), ("read", CacheReadParams, False)):
+        P = ctypes.POINTER(cls)
+        fns = [(f"cache_{name}_params_init", [P], None),
+               (f"cache_{name}", [P, ctypes.c_void_p], ctypes.c_int)]
+        if sized:
+            fns += [(f"cache_{name}_validate", [P], ctypes.c_int),
+                    (f"cache_{name}_workspace_bytes", [P], ctypes.c_size_t)]
+        for fn_name, args, res in fns:
+            fn = getattr(lib, "shaobo_fa3_" + fn_name)
+            fn.argtypes, fn.restype = args, res
+
+
 def _declare_attn(lib):
     A, R = ctypes.POINTER(AttnParams), ctypes.POINTER(RotaryParams)
     for name, args, res in (
@@ -234,6 +299,7 @@ def load(path=LIB_PATH):
         lib.shaobo_fa3_ext_bwd_v2_plan.argtypes = [ctypes.POINTER(Params), ctypes.POINTER(Plan)]
         lib.shaobo_fa3_ext_bwd_v2_plan.restype = ctypes.c_int
         _declare_attn(lib)
+        _declare_cache(lib)
         if path != LIB_PATH:
             return lib
         _LIB = lib

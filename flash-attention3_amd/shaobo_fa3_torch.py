@@ -216,7 +216,17 @@ def attention(q, k, v, causal=True, softmax_scale=None):
 #       -> dq, dk, dv, softmax_d
 #
 # The three are registered by lib/_fa3_torch_attn.so (csrc/fa3_torch_attn.cpp);
-# `rotary` and `score_attention` below add their gradients.
+# `rotary` and `score_attention` below add their gradients.  The same library
+# has the operators of a paged cache (csrc/fa3_torch_cache.cpp), for serving:
+#
+#   torch.ops.shaobo_fa3.cache_append(k, v, k_pages!, v_pages!, page_table, kv_lens,
+#       new_lens, q, positions, freqs, interleaved, bounds!) -> [turned q] or []
+#   torch.ops.shaobo_fa3.cache_attn(q, k_pages, v_pages, page_table, kv_lens, new_lens,
+#       causal, softmax_scale, softcap, slopes, prefix_lens, selected) -> out, lse
+#   torch.ops.shaobo_fa3.cache_select(q, bounds, page_table, kv_lens, page_size, count,
+#       new_lens) -> selected
+#   torch.ops.shaobo_fa3.cache_read(k_pages, v_pages, page_table, kv_lens, seqlen, dtype)
+#       -> k, v
 _ATTN_PATH = os.path.join(os.path.dirname(F.LIB_PATH), "_fa3_torch_attn.so")
 
 
@@ -259,6 +269,27 @@ if _ATTN:
     @torch.library.register_fake("shaobo_fa3::rotary")
     def _(xs, positions, freqs, interleaved=False, inverse=False):
         return [torch.empty_like(x) for x in xs]
+
+    @torch.library.register_fake("shaobo_fa3::cache_append")
+    def _(k, v, k_pages, v_pages, page_table, kv_lens, new_lens=None, q=None, positions=None,
+          freqs=None, interleaved=False, bounds=None):
+        return [] if q is None else [torch.empty_like(q)]
+
+    @torch.library.register_fake("shaobo_fa3::cache_attn")
+    def _(q, k_pages, v_pages, page_table, kv_lens, new_lens=None, causal=True, softmax_scale=None,
+          softcap=0.0, slopes=None, prefix_lens=None, selected=None):
+        return torch.empty_like(q), q.new_empty(q.shape[:3], dtype=torch.float32)
+
+    @torch.library.register_fake("shaobo_fa3::cache_select")
+    def _(q, bounds, page_table, kv_lens, page_size, count, new_lens=None):
+        return q.new_empty((q.shape[0], bounds.shape[1], q.shape[2], count), dtype=torch.int32)
+
+    @torch.library.register_fake("shaobo_fa3::cache_read")
+    def _(k_pages, v_pages, page_table, kv_lens, seqlen, dtype):
+        row = k_pages.shape[3]
+        shape = (page_table.shape[0], k_pages.shape[1], seqlen,
+                 2 * (row - 4) if k_pages.dtype == torch.uint8 else row)
+        return k_pages.new_empty(shape, dtype=dtype), k_pages.new_empty(shape, dtype=dtype)
 
 
 def _in_rows(t):
@@ -370,3 +401,91 @@ def rotary_freqs(sections, theta=10000.0, device=None):
         freqs[a, at:at + n] = inv[at:at + n].float()
         at += n
     return freqs.to(device)
+
+
+# ---------------------------------------------------------------------------
+# The paged cache (include/shaobo_fa3_cache.h says what the operators compute).
+def cache_pages(pages, heads_kv, page_size, head_dim, dtype=torch.bfloat16, bits=16, bounds=False,
+                device="cuda"):
+    """(k_pages, v_pages, bounds) of a cache of `pages` pages of page_size (32
+    to 1024, a power of two) places, zeros: [pages, heads_kv, page_size,
+    head_dim] in dtype, or held in 4 bits uint8 [pages, heads_kv, page_size,
+    head_dim / 2 + 4], whose last two axes are one block of codes and scales;
+    bounds [pages, heads_kv, 2, head_dim] for cache_select, or None."""
+    if bits not in (4, 16):
+        raise ValueError("a cache is held in 16 bits or in 4")
+    row, kind = (head_dim, dtype) if bits == 16 else (head_dim // 2 + 4, torch.uint8)
+    k, v = (torch.zeros(pages, heads_kv, page_size, row, dtype=kind, device=device)
+            for _ in range(2))
+    b = torch.zeros(pages, heads_kv, 2, head_dim, dtype=dtype, device=device) if bounds else None
+    return k, v, b
+
+
+def _no_gradient(*tensors):
+    _need_attn()
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError("the cache's operators have no gradient: pass detached tensors")
+
+
+def cache_append(k, v, k_pages, v_pages, *, page_table, kv_lens, new_lens=None, q=None,
+                 positions=None, freqs=None, interleaved=False, bounds=None):
+    """Writes new tokens' keys, turned by their positions, and values into a
+    cache's pages; returns q turned likewise (None without q).
+
+    k, v [B, Hkv, S, D], q [B, Hq, S, D], fp16 or bf16, in rows as
+    score_attention takes them; k_pages, v_pages and bounds as cache_pages makes
+    them (4 bits: D 64 or 128).
+
+    page_table   int32 [B, width]: the page of a sequence's places
+                 [n * page_size, (n + 1) * page_size); a number that is no page:
+                 nothing is written there
+    kv_lens      int32 [B]: tokens of each sequence, the new ones included
+    new_lens     int32 [B]: how many of the S rows are tokens (default: all),
+                 the rest is padding; token i is at place kv_lens - new_lens + i
+    freqs        fp32 [axes, pairs] as rotary takes them; None: nothing is turned
+    positions    [axes, B, S] as rotary takes them; None: one axis, the places
+    bounds       follow the keys written, for cache_select
+
+    Written pages must belong to one sequence each."""
+    _no_gradient(k, v, q)
+    out = torch.ops.shaobo_fa3.cache_append(k, v, k_pages, v_pages, page_table, kv_lens, new_lens, q,
+                                            positions, freqs, interleaved, bounds)
+    return out[0] if out else None
+
+
+def cache_attention(q, k_pages, v_pages, *, page_table, kv_lens, new_lens=None, causal=True,
+                    softmax_scale=None, softcap=0.0, slopes=None, prefix_lens=None, selected=None,
+                    return_lse=False):
+    """Softmax attention of new tokens to their sequences in a paged cache
+    (after cache_append): score_attention with its options, where token i is at
+    place kv_lens - new_lens + i and keys whose page is none are left out.
+
+    selected     int32 [B, Hkv, S, count] (cache_select): only these pages'
+                 keys are looked at; a page listed twice counts twice
+
+    Padding rows give zeros, and -inf in the log-sum-exp that return_lse=True
+    also returns (fp32 [B, Hq, S])."""
+    _no_gradient(q, slopes)
+    out, lse = torch.ops.shaobo_fa3.cache_attn(q, k_pages, v_pages, page_table, kv_lens, new_lens,
+                                               causal, softmax_scale, softcap, slopes, prefix_lens,
+                                               selected)
+    return (out, lse) if return_lse else out
+
+
+def cache_select(q, bounds, *, page_table, kv_lens, page_size, count, new_lens=None):
+    """The `count` pages that each new token and KV head is to look at, int32
+    [B, Hkv, S, count], ascending, -1 behind them: the token's own page, and of
+    those before it the ones whose bounds allow the largest score of any head of
+    the group (for a positive softmax scale).  bounds as cache_append keeps them
+    (q turned as it returns it)."""
+    _no_gradient(q)
+    return torch.ops.shaobo_fa3.cache_select(q, bounds, page_table, kv_lens, page_size, count,
+                                             new_lens)
+
+
+def cache_read(k_pages, v_pages, *, page_table, kv_lens, seqlen, dtype=torch.bfloat16):
+    """k and v [B, Hkv, seqlen, D] in dtype: the first seqlen places of every
+    sequence as the cache holds them, zeros at and behind kv_lens and where
+    there is no page."""
+    _no_gradient()
+    return torch.ops.shaobo_fa3.cache_read(k_pages, v_pages, page_table, kv_lens, seqlen, dtype)

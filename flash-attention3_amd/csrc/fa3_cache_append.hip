@@ -33,16 +33,16 @@ struct AppendArgs {
     const float* freqs;
     int type, axes, pairs;
     int seqlen, heads_q, heads_kv, d;
-    int run, segments;  // log2 of a workgroup's places; runs of a sequence
-    int hq, hk;         // heads a workgroup takes of q; of k and v
-    int parts_q, parts_k;
+    // log2 of a workgroup's places, and runs of a sequence; k's beside q's and v's
+    int run, segments, run_k, segments_k;
+    int hq, hk, hv;  // heads a workgroup takes
+    int parts_q, parts_k, batch;
     int units;          // of a turned row: 16-byte pieces (with their partners, where those lie apart)
-    FastDiv div_segments, div_pairs, div_units, div_row, div_hq, div_hk;
+    FastDiv div_segments, div_segments_k, div_pairs, div_units, div_row, div_hq, div_hk, div_hv;
 };
 
 constexpr int kAppendThreads = 256;
 constexpr int kAppendTokens = 16;  // of a run at a time
-constexpr int kAppendRows = 64;    // of k in LDS
 
 template <bool kBf16>
 __device__ __forceinline__ float value16(_Float16 x) {
@@ -128,10 +128,10 @@ struct AppendRun {
 template <bool kBf16, bool kFour, bool kV>
 __device__ __forceinline__ void put_rows(const AppendRun& r, int c0, int n, const _Float16* kept) {
     const auto& a = attn_args<AppendArgs>();
-    const int d = a.d, units = d / 8, per = a.hk, shift = a.c.shift, total = n * per * units;
+    const int d = a.d, units = d / 8, per = kV ? a.hv : a.hk, shift = a.c.shift, total = n * per * units;
     for (int x0 = 0; x0 < total; x0 += kAppendThreads) {
         const int x = x0 + threadIdx.x, row = fdiv(a.div_row, x), u = x - row * units;
-        const int t = fdiv(a.div_hk, row), h = row - t * per, i = c0 + t;
+        const int t = fdiv(kV ? a.div_hv : a.div_hk, row), h = row - t * per, i = c0 + t;
         const bool ok = x < total && h < r.heads && i >= r.t0 && i < r.t1;
         f16x8 y{};
         if (ok) {
@@ -202,26 +202,28 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(AppendArgs
     extern __shared__ __attribute__((aligned(16))) char append_lds[];
     double2* turn = (double2*)append_lds;  // [tokens][pairs] cos, sin
     _Float16* kept = (_Float16*)(append_lds + kAppendTokens * a.pairs * 16);  // [tokens][heads][d]
+    int part = blockIdx.y;
+    const bool is_q = part < a.parts_q;
+    if (!is_q) part -= a.parts_q;
+    const bool is_v = !is_q && part >= a.parts_k, is_k = !is_q && !is_v;
+    if (is_v) part -= a.parts_k;
     AppendRun r;
-    r.b = fdiv(a.div_segments, blockIdx.x);
+    r.b = fdiv(is_k ? a.div_segments_k : a.div_segments, blockIdx.x);
+    if (r.b >= a.batch) return;  // (k's runs may be longer, and fewer)
+    const int seg = blockIdx.x - r.b * (is_k ? a.segments_k : a.segments), run = is_k ? a.run_k : a.run;
     const int kv = cache_kv(a.c, r.b), fresh = cache_new(a.c, r.b, a.seqlen);
     // rows i0 .. i1 - 1 of the call, at places place0 + i
     r.place0 = kv - fresh;
-    r.run0 = ((r.place0 >> a.run) + (int)(blockIdx.x - r.b * a.segments)) << a.run;
+    r.run0 = ((r.place0 >> run) + seg) << run;
     r.i0 = max(r.run0 - r.place0, 0);
-    r.i1 = min(r.run0 + (1 << a.run) - r.place0, a.seqlen);
+    r.i1 = min(r.run0 + (1 << run) - r.place0, a.seqlen);
     if (r.i0 >= r.i1) return;
     // tokens among them (a place below 0 or a page that is none: not written)
     r.page = -1;
     if (r.run0 >= 0 && r.i0 < fresh) r.page = cache_page_scalar(a.c, r.b, (r.place0 + r.i0) >> a.c.shift);
     r.t0 = r.i0;
     r.t1 = r.page >= 0 ? min(r.i1, fresh) : r.t0;
-    int part = blockIdx.y;
-    const bool is_q = part < a.parts_q;
-    if (!is_q) part -= a.parts_q;
-    const bool is_v = !is_q && part >= a.parts_k;
-    if (is_v) part -= a.parts_k;
-    const int per = is_q ? a.hq : a.hk;
+    const int per = is_q ? a.hq : is_k ? a.hk : a.hv;
     r.h0 = part * per;
     r.heads = min(per, (is_q ? a.heads_q : a.heads_kv) - r.h0);
     if (is_v) {
@@ -354,23 +356,35 @@ AppendGrid append_grid(const ShaoboFa3CacheAppendParams& p) {
     // A run of 16 places, fewer where the call has fewer; bounds: a whole page.
     int run = 1;
     while (run < kAppendTokens && run < p.seqlen) run *= 2;
-    if (c.bounds != nullptr) run = c.page_size;
+    const int run_k = c.bounds != nullptr ? c.page_size : run;
     g.run = log2_of(run);
-    g.segments = (int)(((int64_t)p.seqlen + run - 2) / run) + 1;
-    // Heads that give a workgroup's threads two rounds of work at a time; of k
-    // and v as many as LDS and the bounds' threads hold.
-    const int tokens = run < kAppendTokens ? run : kAppendTokens;
-    const int tokens1 = tokens < p.seqlen ? tokens : p.seqlen;
-    g.hq = ceil_div(2 * kAppendThreads, tokens1 * g.units);
-    if (g.hq > p.num_heads_q) g.hq = p.num_heads_q > 0 ? p.num_heads_q : 1;
-    g.hk = c.head_dim > 64 ? 4 : 8;
-    if (g.hk * tokens > kAppendRows) g.hk = kAppendRows / tokens;
-    if (g.hk > c.num_heads_kv) g.hk = c.num_heads_kv;
+    g.run_k = log2_of(run_k);
+    auto runs = [&](int n) { return (int)(((int64_t)p.seqlen + n - 2) / n) + 1; };
+    g.segments = runs(run);
+    g.segments_k = runs(run_k);
+    // A token's cosines are formed by every workgroup that turns some of its
+    // heads, at a cost of about 8 of them: as many heads each as leave a
+    // thousand workgroups to q, and few where tokens are few; of k what LDS and
+    // the bounds' threads hold (8192 tokens, Hq32 Hkv8 D128: 56 us with 4 of
+    // each, APPEND_US with 16 and 8).
+    const int64_t n = (int64_t)c.batch * g.segments;
+    auto share = [&](int heads, int least) {
+        const int64_t x = heads * n / 1024;
+        return (int)(x < least ? (least < heads ? least : heads) : x < heads ? x : heads);
+    };
+    g.hq = p.num_heads_q > 0 ? share(p.num_heads_q, 4) : 1;
+    g.hk = share(c.num_heads_kv, 4);
+    g.hv = share(c.num_heads_kv, 4);
+    const int most = c.bounds != nullptr ? 256 / (c.head_dim / 2) : 8;
+    if (g.hk > most) g.hk = most;
     g.parts_q = p.num_heads_q > 0 ? ceil_div(p.num_heads_q, g.hq) : 0;
     g.parts_k = ceil_div(c.num_heads_kv, g.hk);
+    g.parts_v = ceil_div(c.num_heads_kv, g.hv);
+    int tokens = run_k < kAppendTokens ? run_k : kAppendTokens;
+    if (tokens > p.seqlen) tokens = p.seqlen;
     g.lds = (size_t)kAppendTokens * pairs * 16 + (size_t)tokens * g.hk * c.head_dim * 2;
-    g.ok = (int64_t)c.batch * g.segments * (g.parts_q + 2 * g.parts_k) < kMaxGrid &&
-           g.parts_q + 2 * g.parts_k < 65536;
+    const int parts = g.parts_q + g.parts_k + g.parts_v;
+    g.ok = n * parts < kMaxGrid && parts < 65536;
     return g;
 }
 
@@ -397,19 +411,25 @@ hipError_t launch_cache_append(const ShaoboFa3CacheAppendParams& p, hipStream_t 
     a.d = p.cache.head_dim;
     a.run = g.run;
     a.segments = g.segments;
+    a.run_k = g.run_k;
+    a.segments_k = g.segments_k;
+    a.batch = p.cache.batch;
     a.hq = g.hq;
     a.hk = g.hk;
+    a.hv = g.hv;
     a.parts_q = g.parts_q;
     a.parts_k = g.parts_k;
     a.units = g.units;
     a.div_segments = make_fastdiv(g.segments);
+    a.div_segments_k = make_fastdiv(g.segments_k);
     a.div_pairs = make_fastdiv(a.pairs);
     a.div_units = make_fastdiv(g.units);
     a.div_row = make_fastdiv(a.d / 8);
     a.div_hq = make_fastdiv(g.hq);
     a.div_hk = make_fastdiv(g.hk);
+    a.div_hv = make_fastdiv(g.hv);
     auto go = [&](auto kernel) {
-        hipLaunchKernelGGL(kernel, dim3(p.cache.batch * g.segments, g.parts_q + 2 * g.parts_k),
+        hipLaunchKernelGGL(kernel, dim3(p.cache.batch * g.segments, g.parts_q + g.parts_k + g.parts_v),
                            dim3(kAppendThreads), g.lds, stream, a);
     };
     auto pick = [&](auto bf, auto four) {

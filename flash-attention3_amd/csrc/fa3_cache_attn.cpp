@@ -10,7 +10,7 @@ CachePlan plan_cache_attn(const CacheProblem& p) {
     // Selected pages are a query's own, and its heads few rows.
     f.token = p.count > 0 || rows <= 32;
     const int64_t at_once = p.count > 0 ? p.group : rows;
-    f.row_tile = p.four && at_once <= 16 ? 16 : 32;
+    f.row_tile = at_once <= 16 ? 16 : 32;
     f.split = !f.token && groups * ceil_div(rows, kAttnRows) < 512 ? 2 : 1;
     f.per_query = ceil_div(p.group, f.row_tile);
     const int64_t tiles = p.count > 0 ? (int64_t)p.sq * f.per_query
@@ -21,7 +21,7 @@ CachePlan plan_cache_attn(const CacheProblem& p) {
     // Jobs that leave the chip half empty cut the key axis, as long as a part
     // keeps 256 keys (tiles: 512).  How many parts there are goes by the places
     // that the pages have; a sequence's own length is cut into them on the GPU.
-    const int fill = f.token ? (p.four ? (f.row_tile == 16 ? 768 : 512) : D == 128 ? 256 : 512) : 512;
+    const int fill = f.token ? 256 * ((p.four || D == 64 ? 4 : 3) - f.row_tile / 16) : 512;
     const int64_t keys = p.count > 0 ? (int64_t)p.count * p.page : p.sk;
     const int least = f.token ? 256 : 512;
     if (jobs > 0 && 2 * jobs <= fill && keys >= 2 * least) {

@@ -1,10 +1,10 @@
 // Attention to a paged cache: the kernels of fa3_attn_fwd.hip with a page
 // looked up for every 32 or 64 keys.
 //
-// cache_token_kernel and cache_tile_kernel walk 16-bit pages as those do dense
-// tensors.  From 4-bit pages cache_tile_kernel makes its LDS tiles itself: a
-// thread loads the codes of the next tile before this one's products and
-// writes their levels, 16 bits each, behind them.
+// cache_tile_kernel walks 16-bit pages as attn_fwd_kernel does dense tensors.
+// From 4-bit pages it makes its LDS tiles itself: a thread loads the codes of
+// the next tile before this one's products and writes their levels, 16 bits
+// each, behind them.
 #pragma once
 
 #include "fa3_attn_fwd_kernel.h"
@@ -108,97 +108,6 @@ __device__ __forceinline__ CacheBlock cache_block(const A& a, const CacheJob& j,
     x.j0 = (p << shift) + ((at & ((1 << (shift - 5)) - 1)) << 5);
     if (x.j0 < j.lim) x.page = cache_page_scalar(a.x.cv, j.b, p);
     return x;
-}
-
-// Few rows, 16 bits: attn_token_kernel with pages.
-template <int D, bool kBf16, bool kCap, bool kBias>
-__global__ __launch_bounds__(kRegThreads, D == 64 ? 2 : 1) void cache_token_kernel(CacheAttnArgs) {
-    typedef CacheAttnArgs Args;
-    const auto& a = attn_args<Args>();
-    using C = TokenCfg<D>;
-    __shared__ __attribute__((aligned(1024))) char smem_raw[C::kBytes];
-    FA3_LDS char* smem = (FA3_LDS char*)smem_raw;
-    const int lane = threadIdx.x & 63;
-    const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const CacheJob job = cache_job(a, blockIdx.x, 32);
-    const int b = job.b, hkv = job.hkv, kv = job.kv;
-    const CacheSpan span = cache_span(a, job);
-    // this wave's x-th block is span.begin + w + 4 x
-    const int first = span.begin + w, end = span.end;
-    const int n = end > first ? (end - first + 3) >> 2 : 0;
-    auto load = [&](FA3_LDS char* st, const char* head, int64_t ps, int64_t rs, const CacheBlock& x,
-                    bool whole, int d, int mask) {
-        constexpr int kRows = 512 / D, kC = D / 8;
-        const int ln = opaque_tid() & 63, row = ln / kC;
-        const uint32_t cc = ((uint32_t)(ln % kC) ^ reg_swz<D>(row)) & (kC - 1);
-        const char* p = head + x.page * ps + ((x.j0 & mask) + row) * rs;
-        auto put = [&](int j, const char* y) {
-            __builtin_amdgcn_global_load_lds((const void*)y, (FA3_LDS void*)(st + j * 1024), 16, 0, 0);
-        };
-        auto chunk = [&](int j) { return (cc ^ reg_swz<D>(kRows * j)) & (kC - 1); };
-        if (whole) {
-#pragma unroll
-            for (int j = 0; j < C::kLd; ++j) put(j, p + (kRows * j) * rs + chunk(j) * 16);
-        } else {
-#pragma unroll
-            for (int j = 0; j < C::kLd; ++j) {
-                const bool ok = x.page >= 0 && x.j0 + kRows * j + row < kv && (int)chunk(j) * 8 < d;
-                put(j, ok ? p + (kRows * j) * rs + chunk(j) * 16 : (const char*)attn_zeros);
-            }
-        }
-    };
-    // one stage: always 2 kLd loads, which the waits below count
-    auto issue = [&](FA3_LDS char* st, const CacheBlock& x) {
-        const auto& a = attn_args<Args>();
-        const bool whole = x.page >= 0 && x.j0 + 32 <= kv && a.d == D;
-        const int mask = (1 << a.x.cv.shift) - 1;
-        load(st, a.x.cv.k + hkv * a.x.cv.k_hs, a.x.cv.k_ps, a.x.cv.k_rs, x, whole, a.d, mask);
-        load(st + C::kBlock, a.x.cv.v + hkv * a.x.cv.v_hs, a.x.cv.v_ps, a.x.cv.v_rs, x, whole, a.d, mask);
-    };
-    FA3_LDS char* s0 = smem + w * 2 * C::kStage;
-    FA3_LDS char* s1 = s0 + C::kStage;
-    CacheBlock cur = cache_block(a, job, first, end);
-    if (n > 0) issue(s0, cur);
-    CacheBlock next = cache_block(a, job, first + 4, end);
-    FwdRows<D, kBf16, kCap, kBias, Args> rows;
-    rows.init(a, job.row0, job.rows, job.end, b, hkv, kv, job.prefix, job.off, lane);
-    rows.load(a, job.row0, job.rows, b, hkv, job.off, lane);
-    const RegReader<D> rd(lane, 0);
-    const float c = a.m.c;
-    int x = 0;
-    auto stage = [&](FA3_LDS char* __restrict__ ld, const FA3_LDS char* __restrict__ st) {
-        // (looked up a block ahead: two loads that wait for each other)
-        const CacheBlock far = cache_block(attn_args<Args>(), job, first + 4 * x + 8, end);
-        wait_vm_lgkm0<63>();  // (the block read from ld before is done with)
-        wall();
-        if (x + 1 < n) {
-            issue(ld, next);
-            wall();
-            wait_vm_lgkm0<2 * C::kLd>();
-        } else {
-            wait_vm_lgkm0<0>();
-        }
-        __atomic_signal_fence(__ATOMIC_SEQ_CST);
-        wall();
-        if (cur.page >= 0)
-            rows.template step<2>(rd, st, st + C::kBlock, 0, cur.j0, nullptr, c);
-        cur = next;
-        next = far;
-        ++x;
-    };
-    while (x < n) {
-        stage(s1, s0);
-        if (x >= n) break;
-        stage(s0, s1);
-    }
-    wait_vm_lgkm0<0>();
-    barrier();
-    const CacheJob e = cache_job(attn_args<Args>(), blockIdx.x, 32);
-    const int ew = __builtin_amdgcn_readfirstlane(opaque_tid() >> 6);
-    rows.template settle<false>(e.row0, e.b, e.hkv);
-    rows.template meet<4>((FA3_LDS float*)smem, smem + 2048, ew, 0, ew);
-    if (ew > 0) return;
-    rows.finish(e.row0, e.end, e.b, e.hkv, e.grp, e.split, smem + 2048);
 }
 
 template <int D, bool kFour>

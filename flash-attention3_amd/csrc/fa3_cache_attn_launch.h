@@ -2,7 +2,7 @@
 // rows (fa3_cache_attn_d*_*.hip).
 #pragma once
 
-#include "fa3_cache_four_kernel.h"
+#include "fa3_cache_few_kernel.h"
 
 namespace fa3 {
 namespace {
@@ -16,11 +16,8 @@ void launch_cache(const CacheAttnArgs& x, const CacheProblem& p, const CachePlan
     auto kinds = [&](auto cz, auto bi) {
         constexpr bool kC = decltype(cz)::value, kBi = decltype(bi)::value;
         if (f.token) {
-            if constexpr (kFour)
-                f.row_tile == 16 ? go(cache_four_kernel<D, kBf16, kC, kBi, 1>)
-                                 : go(cache_four_kernel<D, kBf16, kC, kBi, 2>);
-            else
-                go(cache_token_kernel<D, kBf16, kC, kBi>);
+            f.row_tile == 16 ? go(cache_few_kernel<D, kBf16, kC, kBi, kFour, 1>)
+                             : go(cache_few_kernel<D, kBf16, kC, kBi, kFour, 2>);
         } else if (f.split == 2) {
             go(cache_tile_kernel<D, kBf16, kC, kBi, kFour, 2>);
         } else {

@@ -1,21 +1,21 @@
-// Few rows of a KV head against 4-bit pages: 16 kBlocks rows a workgroup,
-// whose four waves all hold them and take every fourth block of 32 keys each,
-// straight from HBM to registers.
+// Few rows of a KV head: 16 kBlocks rows a workgroup, whose four waves all hold
+// them and take every fourth block of 32 keys each, straight from HBM to
+// registers.
 //
 // A lane's share of a block, with r = lane % 16 and g = lane / 16:
-//   K   16 bytes (D 64: 8) of rows r and 16 + r, channels D / 4 g ..: the A
-//       operand of S^T = K Q^T whose k-step s stands for the channels D / 4 g +
-//       8 s .. of each g, in Q's operand too; a row's codes are read once by
-//       four lanes that lie together;
+//   K   the channels D / 4 g .. of rows r and 16 + r: the A operand of S^T = K
+//       Q^T whose k-step s stands for the channels D / 4 g + 8 s .. of each g,
+//       in Q's operand too; a row is read once by four lanes that lie together;
 //   V   the D / 16 channels D / 16 r .. of the rows 4 g + 0..3 and 16 + 4 g +
-//       0..3, whose scores are the lane's own: two rows' codes of a channel put
-//       side by side in a byte become two levels side by side, a pair of the A
-//       operand of O^T += V^T P^T (two shifts and two selects for 16 codes,
-//       then one conversion for two levels);
-//   scales  of those rows, K's and V's.
-// Levels are exact, the scale of K meets the fp32 score, that of V meets P
-// before its rounding to bf16.  Two blocks' loads are out at a time; there is
-// no barrier before the waves meet.
+//       0..3, whose scores are the lane's own.  Two rows' values of a channel
+//       side by side are a pair of the A operand of O^T += V^T P^T: of 16 bits
+//       by one byte permutation; of 4 bits two rows' codes are put into one
+//       byte (two shifts and two selects for 16 codes), which one conversion
+//       makes two levels of;
+//   4 bits: the scales of those rows, K's and V's.  Levels are exact, the
+//       scale of K meets the fp32 score, that of V meets P before its rounding
+//       to bf16.
+// Two blocks' loads are out at a time; there is no barrier before the waves meet.
 #pragma once
 
 #include "fa3_cache_attn_kernel.h"
@@ -25,22 +25,29 @@ namespace {
 
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 
-template <int D>
-struct FourBlock {
+// Where a sequence's blocks lie.
+struct FewPages {
+    const char *k, *v;  // the KV head's
+    int64_t k_ps, k_rs, v_ps, v_rs;
+    int shift, d;
+};
+
+template <int D, bool kFour>
+struct FewBlock {  // 4 bits
     typedef typename std::conditional<D == 128, u32x4, u32x2>::type Codes;
     typedef typename std::conditional<D == 128, uint32_t, uint16_t>::type Piece;
     Codes k[2];
     Piece v[8];
     f32x4 ks[2], vs[2];
 
-    // row: the block's first in its page; pk, pv: the page and head
-    __device__ __forceinline__ void load(const char* pk, const char* pv, int row, int shift,
-                                         int lane) {
-        const int l16 = lane & 15, g4 = lane >> 4;
+    __device__ __forceinline__ void load(const FewPages& p, const CacheBlock& x, int lane) {
+        const int l16 = lane & 15, g4 = lane >> 4, row = x.j0 & ((1 << p.shift) - 1);
+        const char* pk = p.k + x.page * p.k_ps;
+        const char* pv = p.v + x.page * p.v_ps;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             k[t] = *(const Codes*)(pk + (row + 16 * t + l16) * (D / 2) + g4 * (D / 8));
-            const int at = (D / 2 << shift) + (row + 16 * t + 4 * g4) * 4;
+            const int at = (D / 2 << p.shift) + (row + 16 * t + 4 * g4) * 4;
             ks[t] = *(const f32x4*)(pk + at);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
@@ -48,21 +55,137 @@ struct FourBlock {
             vs[t] = *(const f32x4*)(pv + at);
         }
     }
+    // rows n and behind hold anything: none of it is to reach a product
+    __device__ __forceinline__ void cut(int n, int lane) {
+        const int k = n - 4 * (lane >> 4);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) vs[t][e] = 16 * t + e < k ? vs[t][e] : 0.f;
+    }
+    template <bool kBf16>
+    __device__ __forceinline__ f16x8 key(int t, int s) const {
+        return cache_levels8<kBf16>(k[t][s]);
+    }
+    // use(i, operand) for every channel i of the lane
+    template <typename F>
+    __device__ __forceinline__ void values(F use) const {
+        // x[j][0]: even channels' codes of rows 2 j and 2 j + 1, a byte each; x[j][1]: odd ones'
+        uint32_t x[4][2];
+        if constexpr (D == 128) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t y = v[2 * j], z = v[2 * j + 1];
+                x[j][0] = (y & 0x0F0F0F0Fu) | ((z << 4) & 0xF0F0F0F0u);
+                x[j][1] = ((y >> 4) & 0x0F0F0F0Fu) | (z & 0xF0F0F0F0u);
+            }
+        } else {  // (bytes 0, 1: rows 2 j and 2 j + 1; bytes 2, 3: 2 j + 4 and 2 j + 5)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const uint32_t y = v[2 * j] | ((uint32_t)v[2 * j + 4] << 16);
+                const uint32_t z = v[2 * j + 1] | ((uint32_t)v[2 * j + 5] << 16);
+                x[j][0] = (y & 0x0F0F0F0Fu) | ((z << 4) & 0xF0F0F0F0u);
+                x[j][1] = ((y >> 4) & 0x0F0F0F0Fu) | (z & 0xF0F0F0F0u);
+                x[j + 2][0] = x[j][0] >> 16;
+                x[j + 2][1] = x[j][1] >> 16;
+            }
+        }
+        auto byte = [&](auto sel) {
+            constexpr int kSel = decltype(sel)::value;
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const u32x4 y = {cache_levels<true, kSel>(x[0][h]), cache_levels<true, kSel>(x[1][h]),
+                                 cache_levels<true, kSel>(x[2][h]), cache_levels<true, kSel>(x[3][h])};
+                use(2 * kSel + h, __builtin_bit_cast(f16x8, y));
+            }
+        };
+        byte(std::integral_constant<int, 0>{});
+        byte(std::integral_constant<int, 1>{});
+        if constexpr (D == 128) {
+            byte(std::integral_constant<int, 2>{});
+            byte(std::integral_constant<int, 3>{});
+        }
+    }
+};
+
+template <int D>
+struct FewBlock<D, false> {  // 16 bits
+    typedef typename std::conditional<D == 128, u32x4, u32x2>::type Piece;
+    f16x8 k[2][D / 32];
+    Piece v[8];
+
+    __device__ __forceinline__ void load(const FewPages& p, const CacheBlock& x, int lane) {
+        const int l16 = lane & 15, g4 = lane >> 4, row = x.j0 & ((1 << p.shift) - 1);
+        const char* pk = p.k + x.page * p.k_ps + (row + l16) * p.k_rs + g4 * (D / 2);
+        const char* pv = p.v + x.page * p.v_ps + (row + 4 * g4) * p.v_rs + l16 * (D / 8);
+        if (p.d == D) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+#pragma unroll
+                for (int s = 0; s < D / 32; ++s) k[t][s] = *(const f16x8*)(pk + 16 * t * p.k_rs + 16 * s);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v[4 * t + e] = *(const Piece*)(pv + (16 * t + e) * p.v_rs);
+            }
+            return;
+        }
+        const bool in = l16 * (D / 16) < p.d;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int s = 0; s < D / 32; ++s)
+                k[t][s] = *(const f16x8*)(g4 * (D / 4) + 8 * s < p.d ? pk + 16 * t * p.k_rs + 16 * s
+                                                                    : (const char*)attn_zeros);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                v[4 * t + e] = *(const Piece*)(in ? pv + (16 * t + e) * p.v_rs : (const char*)attn_zeros);
+        }
+    }
+    __device__ __forceinline__ void cut(int n, int lane) {
+        const int k = n - 4 * (lane >> 4);
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+                for (int i = 0; i < D / 32; ++i)
+                    v[4 * t + e][i] = 16 * t + e < k ? v[4 * t + e][i] : 0u;
+    }
+    template <bool kBf16>
+    __device__ __forceinline__ f16x8 key(int t, int s) const {
+        return k[t][s];
+    }
+    template <typename F>
+    __device__ __forceinline__ void values(F use) const {
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i) {
+            u32x4 y;
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                y[j] = __builtin_amdgcn_perm(v[2 * j + 1][i / 2], v[2 * j][i / 2],
+                                             i % 2 ? 0x07060302u : 0x05040100u);
+            use(i, __builtin_bit_cast(f16x8, y));
+        }
+    }
 };
 
 template <int D, int kBlocks>
-struct FourCfg {
+struct FewCfg {
     static constexpr int kDB = D / 16;
     static constexpr int kSlot = kBlocks * (kDB * 1024 + 256);  // a wave's outputs and sums
     static constexpr int kMax = 4 * kBlocks * 256;              // the waves' maxima
     static constexpr int kBytes = kMax + 3 * kSlot;
 };
 
-template <int D, bool kBf16, bool kCap, bool kBias, int kBlocks>
-__global__ __launch_bounds__(kRegThreads, kBlocks == 1 ? 3 : 2) void cache_four_kernel(CacheAttnArgs) {
+// Waves a SIMD holds: by the registers of two blocks and the rows' outputs.
+constexpr int few_waves(int D, bool four, int blocks) {
+    return (four || D == 64 ? 4 : 3) - blocks;
+}
+
+template <int D, bool kBf16, bool kCap, bool kBias, bool kFour, int kBlocks>
+__global__ __launch_bounds__(kRegThreads, few_waves(D, kFour, kBlocks)) void cache_few_kernel(CacheAttnArgs) {
     typedef CacheAttnArgs Args;
     const auto& a = attn_args<Args>();
-    using C = FourCfg<D, kBlocks>;
+    using C = FewCfg<D, kBlocks>;
     constexpr int kKs = D / 32, kDB = D / 16;
     constexpr float kLazy = 8.f;  // as FwdRows: rescaled only past 2^8
     __shared__ __attribute__((aligned(16))) char smem_raw[C::kBytes];
@@ -73,16 +196,12 @@ __global__ __launch_bounds__(kRegThreads, kBlocks == 1 ? 3 : 2) void cache_four_
     const CacheSpan span = cache_span(a, job);
     const int first = span.begin + w, end = span.end;
     const int n = end > first ? (end - first + 3) >> 2 : 0;
-    const char* kh = a.x.cv.k + job.hkv * a.x.cv.k_hs;
-    const char* vh = a.x.cv.v + job.hkv * a.x.cv.v_hs;
-    const int64_t k_ps = a.x.cv.k_ps, v_ps = a.x.cv.v_ps;
-    const int shift = a.x.cv.shift;
-    auto issue = [&](FourBlock<D>& f, const CacheBlock& x) {
-        if (x.page < 0) return;
-        f.load(kh + x.page * k_ps, vh + x.page * v_ps, x.j0 & ((1 << shift) - 1), shift,
-               opaque_tid() & 63);
+    const FewPages at{a.x.cv.k + job.hkv * a.x.cv.k_hs, a.x.cv.v + job.hkv * a.x.cv.v_hs,
+                      a.x.cv.k_ps, a.x.cv.k_rs, a.x.cv.v_ps, a.x.cv.v_rs, a.x.cv.shift, a.d};
+    auto issue = [&](FewBlock<D, kFour>& f, const CacheBlock& x) {
+        if (x.page >= 0) f.load(at, x, opaque_tid() & 63);
     };
-    FourBlock<D> f0, f1;
+    FewBlock<D, kFour> f0, f1;
     CacheBlock b0 = cache_block(a, job, first, end);
     issue(f0, b0);
     CacheBlock b1 = cache_block(a, job, first + 4, end);
@@ -98,7 +217,7 @@ __global__ __launch_bounds__(kRegThreads, kBlocks == 1 ? 3 : 2) void cache_four_
         const _Float16* p = a.q.p + job.b * a.q.bs + r.h * a.q.hs + r.i * a.q.rs;
 #pragma unroll
         for (int s = 0; s < kKs; ++s)
-            qf[q][s] = attn_flip(attn_row8(p, D / 32 * g4 + s, D, r.ok && a.scored), a.flip);
+            qf[q][s] = attn_flip(attn_row8(p, D / 32 * g4 + s, a.d, r.ok && a.scored), a.flip);
         lim[q] = r.ok ? attn_limit(r.i, job.off, job.kv, a.m.causal, job.prefix) : 0;
         place[q] = r.i + job.off;
         slope[q] = kBias ? a.m.slopes[job.b * a.m.slopes_bs + r.h] * kLog2e : 0.f;
@@ -115,7 +234,7 @@ __global__ __launch_bounds__(kRegThreads, kBlocks == 1 ? 3 : 2) void cache_four_
     const bool fine = kCap && a.m.cap_fine;
     const int kv = job.kv;
 
-    auto step = [&](FourBlock<D>& f, int j0) {
+    auto step = [&](FewBlock<D, kFour>& f, int j0) {
         f32x4 s[2][kBlocks];
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -123,13 +242,15 @@ __global__ __launch_bounds__(kRegThreads, kBlocks == 1 ? 3 : 2) void cache_four_
             for (int q = 0; q < kBlocks; ++q) s[t][q] = f32x4{};
 #pragma unroll
             for (int i = 0; i < kKs; ++i) {
-                const f16x8 x = cache_levels8<kBf16>(f.k[t][i]);
+                const f16x8 x = f.template key<kBf16>(t, i);
 #pragma unroll
                 for (int q = 0; q < kBlocks; ++q)
                     s[t][q] = mfma_16x16x32<kBf16>(x, qf[q][i], s[t][q]);
             }
+            if constexpr (kFour) {
 #pragma unroll
-            for (int q = 0; q < kBlocks; ++q) s[t][q] *= f.ks[t];
+                for (int q = 0; q < kBlocks; ++q) s[t][q] *= f.ks[t];
+            }
         }
         // log2-domain scores
 #pragma unroll
@@ -158,13 +279,7 @@ __global__ __launch_bounds__(kRegThreads, kBlocks == 1 ? 3 : 2) void cache_four_
                         s[t][q][e] = 16 * t + e < k ? s[t][q][e] : kNegInf;
             }
         }
-        if (j0 + 32 > kv) {  // (rows behind the sequence hold anything)
-            const int k = kv - (j0 + 4 * g4);
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) f.vs[t][e] = 16 * t + e < k ? f.vs[t][e] : 0.f;
-        }
+        if (j0 + 32 > kv) f.cut(kv - j0, opaque_tid() & 63);
         float top[kBlocks];
         bool up = false;
 #pragma unroll
@@ -197,47 +312,14 @@ __global__ __launch_bounds__(kRegThreads, kBlocks == 1 ? 3 : 2) void cache_four_
             for (int j = 0; j < 8; ++j) {
                 p[j] = fast_exp2(s[j >> 2][q][j & 3] - m);
                 sum[q] += p[j];
-                p[j] *= f.vs[j >> 2][j & 3];
+                if constexpr (kFour) p[j] *= f.vs[j >> 2][j & 3];
             }
-            bp[q] = pack8<true>(p);
+            bp[q] = pack8<kBf16 || kFour>(p);
         }
-        // x[j][0]: even channels' codes of two rows, a byte each; x[j][1]: odd ones'
-        uint32_t x[4][2];
-        if constexpr (D == 128) {
+        f.values([&](int i, f16x8 x) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t y = f.v[2 * j], z = f.v[2 * j + 1];
-                x[j][0] = (y & 0x0F0F0F0Fu) | ((z << 4) & 0xF0F0F0F0u);
-                x[j][1] = ((y >> 4) & 0x0F0F0F0Fu) | (z & 0xF0F0F0F0u);
-            }
-        } else {  // (bytes 0, 1: rows 2 j and 2 j + 1; bytes 2, 3: 2 j + 4 and 2 j + 5)
-#pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const uint32_t y = f.v[2 * j] | ((uint32_t)f.v[2 * j + 4] << 16);
-                const uint32_t z = f.v[2 * j + 1] | ((uint32_t)f.v[2 * j + 5] << 16);
-                x[j][0] = (y & 0x0F0F0F0Fu) | ((z << 4) & 0xF0F0F0F0u);
-                x[j][1] = ((y >> 4) & 0x0F0F0F0Fu) | (z & 0xF0F0F0F0u);
-                x[j + 2][0] = x[j][0] >> 16;
-                x[j + 2][1] = x[j][1] >> 16;
-            }
-        }
-        auto product = [&](auto sel) {
-            constexpr int kSel = decltype(sel)::value;
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const u32x4 y = {cache_levels<true, kSel>(x[0][h]), cache_levels<true, kSel>(x[1][h]),
-                                 cache_levels<true, kSel>(x[2][h]), cache_levels<true, kSel>(x[3][h])};
-#pragma unroll
-                for (int q = 0; q < kBlocks; ++q)
-                    o[2 * kSel + h][q] = mfma_16x16x32<true>(__builtin_bit_cast(f16x8, y), bp[q], o[2 * kSel + h][q]);
-            }
-        };
-        product(std::integral_constant<int, 0>{});
-        product(std::integral_constant<int, 1>{});
-        if constexpr (D == 128) {
-            product(std::integral_constant<int, 2>{});
-            product(std::integral_constant<int, 3>{});
-        }
+            for (int q = 0; q < kBlocks; ++q) o[i][q] = mfma_16x16x32<kBf16 || kFour>(x, bp[q], o[i][q]);
+        });
     };
     for (int x = 0; x < n; x += 2) {
         const CacheBlock b2 = cache_block(attn_args<Args>(), job, first + 4 * x + 8, end);
@@ -331,7 +413,8 @@ __global__ __launch_bounds__(kRegThreads, kBlocks == 1 ? 3 : 2) void cache_four_
         if (g4 == 0) z.lse[((int64_t)e.b * z.heads_q + r.h) * z.sq + r.i] = lse2 * 0.69314718055994531f;
         _Float16* p = z.out.p + e.b * z.out.bs + r.h * z.out.hs + r.i * z.out.rs + 4 * kDB * g4;
 #pragma unroll
-        for (int i = 0; i < kDB / 2; ++i) *(f16x8*)(p + 8 * i) = pack8<kBf16>(y + 8 * i);
+        for (int i = 0; i < kDB / 2; ++i)
+            if (4 * kDB * g4 + 8 * i < z.d) *(f16x8*)(p + 8 * i) = pack8<kBf16>(y + 8 * i);
     }
 }
 

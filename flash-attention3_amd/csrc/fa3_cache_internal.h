@@ -61,7 +61,7 @@ CacheSelectPlan plan_cache_select(const ShaoboFa3CacheSelectParams& p);
 
 // How an append's workgroups share the tokens and heads.
 struct AppendGrid {
-    int units, run, segments, hq, hk, parts_q, parts_k;
+    int units, run, segments, run_k, segments_k, hq, hk, hv, parts_q, parts_k, parts_v;
     size_t lds;
     bool ok;
 };

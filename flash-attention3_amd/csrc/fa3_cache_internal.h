@@ -61,8 +61,7 @@ CacheSelectPlan plan_cache_select(const ShaoboFa3CacheSelectParams& p);
 
 // How an append's workgroups share the tokens and heads.
 struct AppendGrid {
-    int units, run, segments, run_k, segments_k, hq, hk, hv, parts_q, parts_k, parts_v;
-    size_t lds;
+    int units, lanes, tokens, run, segments, run_k, segments_k, hq, hk, hv, parts_q, parts_k, parts_v;
     bool ok;
 };
 AppendGrid append_grid(const ShaoboFa3CacheAppendParams& p);

@@ -3,31 +3,79 @@
 
 namespace fa3 {
 
+namespace {
+
+int64_t ceil64(int64_t a, int64_t b) { return (a + b - 1) / b; }
+
+// Parts of the key axis for jobs of few rows: as many as fill the chip once,
+// and then up to twice as many where those leave the CUs less uneven (the most
+// jobs a CU has, by the parts' length).  B16 S8192 in 16 bits, 128 jobs: 86 us
+// in 2 parts, 84 in 3, 70 in 4, 82 in 6, 76 in 8; 512 jobs that fill it
+// already, B64 S2048 in 4 bits: 26 whole, 29 in 2.  A part keeps 256 keys.
+int few_splits(int64_t jobs, int fill, int64_t keys) {
+    const int64_t most = keys / 256, least = fill / jobs;
+    if (least < 1 || jobs >= fill || most < 2) return 1;
+    int64_t best = least < most ? least : most;
+    for (int64_t s = best + 1; s <= 2 * least && s <= most; ++s)
+        if (ceil64(jobs * s, 256) * best < ceil64(jobs * best, 256) * s) best = s;
+    return (int)best;
+}
+
+// Rows and parts for jobs of many rows, by an estimate of the launch, us: a
+// 64-key step of a job of 128 rows (64) takes 1.96 (1.42) where the CU has one
+// job and 1.33 (0.86) a job where it has more; parts of a sequence write their
+// sums and read them again at 4 TB/s, in a launch of 5; a job's beginning and
+// end are four steps.  How much of the places
+// is filled is not known here: all of them are taken to be.  (D 128, both
+// widths; measured, the estimate's choice first: 1531 tokens over 9211, 8 KV
+// heads, 300 us in 128 rows and 2 parts, 292 in 4, 350 whole, 365 in 64 rows
+// and 2; 8 times 64 over 8192, 106 in 128 rows and 4 parts, 129 in 64 and 2;
+// 2011 of 4 KV heads, 53 in 64 rows, 55 in 128 and 2 parts, 68 in 128; 512 of 8
+// KV heads, 18 in 64 rows, 21 in 128, 31 and 33 in 2 parts.)
+void tile_plan(const CacheProblem& p, CachePlan* f) {
+    const int64_t rows = (int64_t)p.group * p.sq, groups = (int64_t)p.batch * p.heads_kv;
+    const double last = p.sk / 64.0;  // steps of the longest job, and of them all in the mean
+    const double mean = p.causal && p.sk > 0 ? last - (p.sq < p.sk ? p.sq : p.sk) / 128.0 : last;
+    double best = 1e300;
+    for (int split = 1; split <= 2; ++split) {
+        const int64_t jobs = groups * ceil64(rows, kAttnRows / split);
+        const double alone = split == 1 ? 1.96 : 1.42, among = split == 1 ? 1.33 : 0.86;
+        for (int parts = 1; parts <= 32 && (parts == 1 || last >= 4 * parts); ++parts) {
+            const int64_t a_cu = ceil64(jobs * parts, 256);
+            const double step = a_cu <= 1 ? alone : 2 * among;  // of a job beside another
+            double t = (a_cu <= 1 ? alone : a_cu * among) * (mean / parts + 4);
+            if ((last / parts + 4) * step > t) t = (last / parts + 4) * step;
+            if (parts > 1) t += 5 + (double)parts * groups * rows * 8.0 * (p.d > 64 ? 128 : 64) / 4e6;
+            if (t < best) {
+                best = t;
+                f->split = split;
+                f->splits = parts;
+            }
+        }
+    }
+}
+
+}  // namespace
+
 CachePlan plan_cache_attn(const CacheProblem& p) {
     CachePlan f{};
     const int64_t rows = (int64_t)p.group * p.sq, groups = (int64_t)p.batch * p.heads_kv;
     const int D = p.d > 64 ? 128 : 64;
+    if (groups >= kMaxGrid || rows >= (1ll << 30)) return f;
     // Selected pages are a query's own, and its heads few rows.
     f.token = p.count > 0 || rows <= 32;
     const int64_t at_once = p.count > 0 ? p.group : rows;
     f.row_tile = at_once <= 16 ? 16 : 32;
-    f.split = !f.token && groups * ceil_div(rows, kAttnRows) < 512 ? 2 : 1;
     f.per_query = ceil_div(p.group, f.row_tile);
+    f.split = f.splits = 1;
+    if (!f.token) tile_plan(p, &f);
     const int64_t tiles = p.count > 0 ? (int64_t)p.sq * f.per_query
                           : f.token   ? 1
                                       : ceil_div(rows, kAttnRows / f.split);
-    f.splits = 1;
     const int64_t jobs = groups * tiles;
-    // Jobs that leave the chip half empty cut the key axis, as long as a part
-    // keeps 256 keys (tiles: 512).  How many parts there are goes by the places
-    // that the pages have; a sequence's own length is cut into them on the GPU.
-    const int fill = f.token ? 256 * ((p.four || D == 64 ? 4 : 3) - f.row_tile / 16) : 512;
-    const int64_t keys = p.count > 0 ? (int64_t)p.count * p.page : p.sk;
-    const int least = f.token ? 256 : 512;
-    if (jobs > 0 && 2 * jobs <= fill && keys >= 2 * least) {
-        const int64_t want = fill / jobs, most = keys / least;
-        f.splits = (int)(want < most ? want : most);
-    }
+    if (f.token && jobs > 0)
+        f.splits = few_splits(jobs, 256 * few_waves(D, p.four, f.row_tile / 16),
+                              p.count > 0 ? (int64_t)p.count * p.page : p.sk);
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t x = at;
@@ -35,7 +83,7 @@ CachePlan plan_cache_attn(const CacheProblem& p) {
         return x;
     };
     const int64_t all = jobs * f.splits;
-    f.ok = rows < (1ll << 30) && tiles < (1ll << 30) && all < kMaxGrid && groups * rows / 4 < kMaxGrid;
+    f.ok = tiles < (1ll << 30) && all < kMaxGrid && groups * rows / 4 < kMaxGrid;
     if (!f.ok) return f;
     f.tiles = (int)tiles;
     f.jobs = (int)all;
@@ -70,7 +118,7 @@ hipError_t launch_cache_attn(const CacheProblem& p, const ShaoboFa3CacheAttnPara
     x.rows = p.group * p.sq;
     x.tiles = f.tiles;
     x.splits = f.splits;
-    x.part = 8;  // a part has at least 8 blocks of 32 keys, or 8 tiles of 64
+    x.part = f.token ? 8 : 4;  // a part's least, 256 keys: blocks of 32, or tiles of 64
     x.groups = p.batch * p.heads_kv;
     x.levels = f.tiles * f.splits;
     // (longest first, or jobs of one length group by group, as plan_attn_fwd)

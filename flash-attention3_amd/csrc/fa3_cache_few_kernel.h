@@ -176,11 +176,6 @@ struct FewCfg {
     static constexpr int kBytes = kMax + 3 * kSlot;
 };
 
-// Waves a SIMD holds: by the registers of two blocks and the rows' outputs.
-constexpr int few_waves(int D, bool four, int blocks) {
-    return (four || D == 64 ? 4 : 3) - blocks;
-}
-
 template <int D, bool kBf16, bool kCap, bool kBias, bool kFour, int kBlocks>
 __global__ __launch_bounds__(kRegThreads, few_waves(D, kFour, kBlocks)) void cache_few_kernel(CacheAttnArgs) {
     typedef CacheAttnArgs Args;

@@ -51,6 +51,12 @@ struct CachePlan {
 };
 CachePlan plan_cache_attn(const CacheProblem& p);
 
+// Workgroups of the kernel for few rows that a CU holds (waves a SIMD), by the
+// registers of two blocks of keys and of the rows' outputs.
+constexpr int few_waves(int D, bool four, int blocks) {
+    return (D == 64 ? 5 : four ? 4 : 3) - blocks;
+}
+
 // Pages that one workgroup of the scoring kernel takes, and its plan.
 struct CacheSelectPlan {
     int chunks;  // parts of a sequence's pages, scored by a workgroup each

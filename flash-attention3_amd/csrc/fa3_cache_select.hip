@@ -5,12 +5,17 @@
 // a time: the positive part of q meets the upper bound, the negative one the
 // lower.  Sums are fp64, so that two pages change places only where their
 // scores agree to its last bits; they leave as 64-bit keys of the same order.
-// Bound by reading the bounds: a wave has sixteen pages of them on their way.
+// A wave has sixteen pages of bounds on their way; q's parts wait in LDS as
+// doubles.  The sixteen sums of a lane's four pages and heads meet in steps that
+// halve them, so that a lane ends with one (105 operations, 192 for a sum of
+// each over all lanes).
 //
 // cache_pick_kernel: one workgroup per token and KV head finds the key of the
 // last page that is taken, by histograms of 1024 equal ranges between the
 // smallest and the largest key in question (one, as a rule, leaves a few keys,
-// which one wave ranks), and writes the pages at and above it in their order.
+// which one wave ranks), and writes the pages at and above it in their order.  A
+// thread has neighbouring pages, in registers unless there are more than
+// 4096.
 #include "fa3_cache_device.h"
 
 namespace fa3 {
@@ -44,25 +49,27 @@ __device__ __forceinline__ float value16(_Float16 x) {
     else return (float)x;
 }
 
-// x + the value of the lane that a DPP control selects
 template <int kCtrl>
-__device__ __forceinline__ double add_dpp(double x) {
-    typedef int i32x2v __attribute__((ext_vector_type(2)));
-    const i32x2v u = __builtin_bit_cast(i32x2v, x);
-    const i32x2v v = {__builtin_amdgcn_mov_dpp(u[0], kCtrl, 0xF, 0xF, false),
-                      __builtin_amdgcn_mov_dpp(u[1], kCtrl, 0xF, 0xF, false)};
-    return x + __builtin_bit_cast(double, v);
+__device__ __forceinline__ uint64_t dpp64(uint64_t x) {
+    const uint32_t l = __builtin_amdgcn_mov_dpp((int)(uint32_t)x, kCtrl, 0xF, 0xF, false);
+    const uint32_t h = __builtin_amdgcn_mov_dpp((int)(uint32_t)(x >> 32), kCtrl, 0xF, 0xF, false);
+    return (uint64_t)h << 32 | l;
 }
-// over 16 lanes: all of them get the sum, in one order
-__device__ __forceinline__ double sum16(double x) {
-    x = add_dpp<0x128>(x);  // row_ror:8
-    x = add_dpp<0x124>(x);
-    x = add_dpp<0x122>(x);
-    return add_dpp<0x121>(x);
+// A lane keeps the upper half of x[0 .. 2 n - 1] (up) or the lower, and adds what
+// the lane that a DPP control selects has of it.
+template <int kCtrl, int n>
+__device__ __forceinline__ void meet(double* x, bool up) {
+#pragma unroll
+    for (int i = 0; i < n; ++i) {
+        const double keep = up ? x[n + i] : x[i], give = up ? x[i] : x[n + i];
+        x[i] = keep + __builtin_bit_cast(double, dpp64<kCtrl>(__builtin_bit_cast(uint64_t, give)));
+    }
 }
+constexpr int kRor8 = 0x128, kHalfMirror = 0x141, kQuad2 = 0x4E, kQuad1 = 0xB1;  // lane ^ 8, ^ 7, ^ 2, ^ 1
 
 template <bool kBf16>
-__global__ __launch_bounds__(256) void cache_score_kernel(SelectArgs a) {
+__global__ __launch_bounds__(256, 4) void cache_score_kernel(SelectArgs a) {
+    __shared__ double2 parts[kGroupHeads][8][16];  // q's positive and negative part, channel 8 l16 + e
     const int row = fdiv(a.div_chunks, blockIdx.x), chunk = blockIdx.x - row * a.chunks;
     const int bh = fdiv(a.div_seq, row), i = row - bh * a.seqlen;
     const int b = fdiv(a.div_heads, bh), h = bh - b * a.heads_kv;
@@ -70,9 +77,9 @@ __global__ __launch_bounds__(256) void cache_score_kernel(SelectArgs a) {
     const int place = kv - n + i;
     if (i >= n || place < 0) return;  // (padding: the other kernel reads no keys)
     const int own = place >> a.c.shift;
+    if (chunk * kScorePages > own) return;
     const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = lane >> 4, w = threadIdx.x >> 6;
     const int first = chunk * kScorePages + 16 * w + g4;  // this lane's pages: every fourth
-    if (chunk * kScorePages > own) return;
     const bool in = 8 * l16 < a.d;
     int page[4];
     f16x8 lo[4], hi[4];
@@ -90,77 +97,75 @@ __global__ __launch_bounds__(256) void cache_score_kernel(SelectArgs a) {
             hi[j] = *(const f16x8*)(x + a.d);
         }
     }
-    double best[4];
-    bool past[4];  // a head's score is no number, or infinite
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        best[j] = -__builtin_inf();
-        past[j] = false;
-    }
-    const _Float16* q = a.q + b * a.q_bs + (int64_t)h * a.group * a.q_hs + i * a.q_rs + 8 * l16;
+    uint64_t best = 0;  // of page first + 4 (l16 / 4)
+    const _Float16* q = a.q + b * a.q_bs + (int64_t)h * a.group * a.q_hs + i * a.q_rs;
     for (int g0 = 0; g0 < a.group; g0 += kGroupHeads) {
-        f16x8 qv[kGroupHeads];
-#pragma unroll
-        for (int g = 0; g < kGroupHeads; ++g) {
-            qv[g] = f16x8{};
+        if (g0 > 0) __syncthreads();
+        for (int x = threadIdx.x; x < kGroupHeads * 128; x += 256) {
+            const int g = x >> 7, c = x & 127;
             // (a group's last heads again where it is no multiple of four: the same maximum)
-            if (in) qv[g] = *(const f16x8*)(q + min(g0 + g, a.group - 1) * a.q_hs);
+            const float y = c < a.d ? value16<kBf16>(q[min(g0 + g, a.group - 1) * a.q_hs + c]) : 0.f;
+            // (NaN is kept by one of the two)
+            parts[g][c & 7][c >> 3] = make_double2(y < 0.f ? 0.f : y, y < 0.f ? y : 0.f);
         }
-        double s[4][kGroupHeads] = {};
+        __syncthreads();
+        double s[4 * kGroupHeads] = {};  // [page][head]
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            double up[kGroupHeads], down[kGroupHeads];
+            wall();  // (one channel's parts at a time in registers)
+            double2 y[kGroupHeads];
 #pragma unroll
-            for (int g = 0; g < kGroupHeads; ++g) {
-                const float x = value16<kBf16>(qv[g][e]);
-                // (NaN is kept by one of the two)
-                up[g] = x < 0.f ? 0.f : x;
-                down[g] = x < 0.f ? x : 0.f;
-            }
+            for (int g = 0; g < kGroupHeads; ++g) y[g] = parts[g][e][l16];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const double l = value16<kBf16>(lo[j][e]), u = value16<kBf16>(hi[j][e]);
+                // (not unpacked before their turn)
+                uint32_t x = __builtin_bit_cast(u32x4, lo[j])[e / 2], z = __builtin_bit_cast(u32x4, hi[j])[e / 2];
+                __asm__ volatile("" : "+v"(x), "+v"(z));
+                const double l = value16<kBf16>(__builtin_bit_cast(f16x2, x)[e % 2]);
+                const double u = value16<kBf16>(__builtin_bit_cast(f16x2, z)[e % 2]);
 #pragma unroll
                 for (int g = 0; g < kGroupHeads; ++g)
-                    s[j][g] = __builtin_fma(up[g], u, __builtin_fma(down[g], l, s[j][g]));
+                    s[4 * j + g] = __builtin_fma(y[g].x, u, __builtin_fma(y[g].y, l, s[4 * j + g]));
             }
         }
-#pragma unroll
-        for (int j = 0; j < 4; ++j)
-#pragma unroll
-            for (int g = 0; g < kGroupHeads; ++g) {
-                const double x = sum16(s[j][g]);
-                past[j] |= !(__builtin_fabs(x) < __builtin_inf());
-                best[j] = x > best[j] ? x : best[j];
-            }
+        wall();
+        meet<kRor8, 8>(s, l16 & 8);        // pages 0, 1 or 2, 3
+        meet<kHalfMirror, 4>(s, l16 & 4);  // one page
+        meet<kQuad2, 2>(s, l16 & 2);
+        meet<kQuad1, 1>(s, l16 & 1);       // one head
+        uint64_t k = score_key(s[0]);
+        const uint64_t k2 = dpp64<kQuad2>(k);
+        k = k2 > k ? k2 : k;
+        const uint64_t k1 = dpp64<kQuad1>(k);
+        k = k1 > k ? k1 : k;
+        best = k > best ? k : best;
     }
-    uint64_t* keys = a.keys + (int64_t)row * a.c.width;
+    const int j = l16 >> 2, p = first + 4 * j;
+    int mine = page[0];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int p = first + 4 * j;
-        if (l16 == 0 && p <= own)
-            keys[p] = page[j] < 0 ? 0 : p == own ? kKeyOwn : past[j] ? kKeyTop : score_key(best[j]);
-    }
+    for (int x = 1; x < 4; ++x) mine = j == x ? page[x] : mine;
+    if ((l16 & 3) == 0 && p <= own)
+        a.keys[(int64_t)row * a.c.width + p] = mine < 0 ? 0 : p == own ? kKeyOwn : best;
 }
 
 constexpr int kPickThreads = 512;
 constexpr int kPickWaves = kPickThreads / 64;
 constexpr int kBins = 1024;
-constexpr int kRank = 64;         // keys that one wave ranks
-constexpr int kPickKeys = 4096;   // of a row, held in LDS; longer rows are read again
+constexpr int kRank = 64;  // keys that one wave ranks
 
 __device__ __forceinline__ uint64_t shfl_xor64(uint64_t x, int o) {
     const uint32_t l = __shfl_xor((int)(uint32_t)x, o), h = __shfl_xor((int)(uint32_t)(x >> 32), o);
     return (uint64_t)h << 32 | l;
 }
 
+// kPer: pages a thread has in registers; 0: as many as there are, read again.
+template <int kPer>
 __global__ __launch_bounds__(kPickThreads) void cache_pick_kernel(SelectArgs a) {
-    __shared__ uint64_t held[kPickKeys];
     __shared__ uint64_t few[kRank];
     __shared__ uint64_t edge[2];
     __shared__ uint32_t bins[kBins];
     __shared__ uint64_t wave_lo[kPickWaves], wave_hi[kPickWaves];
-    __shared__ int wave_n[3 * kPickWaves];
+    __shared__ int wave_n[4 * kPickWaves];
     __shared__ int found[3];  // bin, above it, in it
     __shared__ int listed;
     const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
@@ -170,22 +175,34 @@ __global__ __launch_bounds__(kPickThreads) void cache_pick_kernel(SelectArgs a) 
     const int place = kv - fresh + i;
     const int n = i < fresh && place >= 0 ? (place >> a.c.shift) + 1 : 0;
     const uint64_t* keys = a.keys + (int64_t)row * a.c.width;
-    // smallest and largest key that is neither none nor past all numbers; how many of each
+    const int per = kPer > 0 ? kPer : (n + kPickThreads - 1) / kPickThreads;
+    // this thread's pages per tid .. (0: none, also past the last)
+    uint64_t held[kPer > 0 ? kPer : 1];
+    if constexpr (kPer > 0) {
+#pragma unroll
+        for (int x = 0; x < kPer; ++x) held[x] = kPer * tid + x < n ? keys[kPer * tid + x] : 0;
+    }
+    auto each = [&](auto use) {
+        if constexpr (kPer > 0) {
+#pragma unroll
+            for (int x = 0; x < kPer; ++x) use(x, held[x]);
+        } else {
+            for (int x = 0; x < per; ++x) use(x, per * tid + x < n ? keys[per * tid + x] : 0);
+        }
+    };
+    if (tid == 0) listed = 0;
+    for (int k = tid; k < kBins; k += kPickThreads) bins[k] = 0;
+    // smallest and largest key that is neither none nor past all numbers; how
+    // many are past them, and how many there are (in one word)
     uint64_t lo = ~0ull, hi = 0;
     int past = 0, all = 0;
-    const bool held_ok = n <= kPickKeys;
-    for (int p = tid; p < n; p += kPickThreads) {
-        const uint64_t k = keys[p];
-        if (held_ok) held[p] = k;
-        if (k == 0) continue;
-        ++all;
-        if (k >= kKeyTop) {
-            ++past;
-            continue;
-        }
-        lo = k < lo ? k : lo;
-        hi = k > hi ? k : hi;
-    }
+    each([&](int, uint64_t k) {
+        all += k != 0;
+        past += k >= kKeyTop;
+        const bool number = k != 0 && k < kKeyTop;
+        lo = number && k < lo ? k : lo;
+        hi = number && k > hi ? k : hi;
+    });
     for (int o = 32; o > 0; o >>= 1) {
         const uint64_t l = shfl_xor64(lo, o), h = shfl_xor64(hi, o);
         lo = l < lo ? l : lo;
@@ -201,25 +218,22 @@ __global__ __launch_bounds__(kPickThreads) void cache_pick_kernel(SelectArgs a) 
     }
     __syncthreads();
     past = all = 0;
+#pragma unroll
     for (int k = 0; k < kPickWaves; ++k) {
         lo = wave_lo[k] < lo ? wave_lo[k] : lo;
         hi = wave_hi[k] > hi ? wave_hi[k] : hi;
         past += wave_n[k];
         all += wave_n[kPickWaves + k];
     }
-    auto key = [&](int p) { return held_ok ? held[p] : keys[p]; };
     // Taken: keys above `last`, and of those equal to it the first `equal`.
     uint64_t last = 0;
     int equal = 0;
     if (all > a.count) {
         int need = a.count;
-        if (past >= need) {  // (the own page is one, where it is there)
+        if (past >= need) {
+            // (one key is above kKeyTop, the own page's, where that is one)
             last = kKeyTop;
-            equal = need;
-            // one key above kKeyTop at most: counted here, not by the histogram
-            int own = 0;
-            if (n > 0 && key(n - 1) == kKeyOwn) own = 1;
-            equal -= own;
+            equal = need - (keys[n - 1] == kKeyOwn ? 1 : 0);
         } else {
             need -= past;
             for (;;) {  // (each round divides hi - lo by 1024)
@@ -229,13 +243,9 @@ __global__ __launch_bounds__(kPickThreads) void cache_pick_kernel(SelectArgs a) 
                     break;
                 }
                 const int bits = 64 - __builtin_clzll(hi - lo), drop = bits > 10 ? bits - 10 : 0;
-                for (int k = tid; k < kBins; k += kPickThreads) bins[k] = 0;
-                if (tid == 0) listed = 0;
-                __syncthreads();
-                for (int p = tid; p < n; p += kPickThreads) {
-                    const uint64_t k = key(p);
+                each([&](int, uint64_t k) {
                     if (k >= lo && k <= hi) atomicAdd(&bins[(k - lo) >> drop], 1u);
-                }
+                });
                 __syncthreads();
                 // thread t has bins 1023 - 2 t and 1022 - 2 t: sums from the top
                 const int c0 = bins[kBins - 1 - 2 * tid], c1 = bins[kBins - 2 - 2 * tid];
@@ -246,6 +256,7 @@ __global__ __launch_bounds__(kPickThreads) void cache_pick_kernel(SelectArgs a) 
                 }
                 if (lane == 63) wave_n[2 * kPickWaves + w] = upto;
                 __syncthreads();
+                bins[kBins - 1 - 2 * tid] = bins[kBins - 2 - 2 * tid] = 0;  // (for another round)
                 int before = upto - c0 - c1;
                 for (int k = 0; k < w; ++k) before += wave_n[2 * kPickWaves + k];
                 if (before < need && need <= before + c0) {
@@ -268,10 +279,9 @@ __global__ __launch_bounds__(kPickThreads) void cache_pick_kernel(SelectArgs a) 
                     __syncthreads();
                     continue;
                 }
-                for (int p = tid; p < n; p += kPickThreads) {
-                    const uint64_t k = key(p);
+                each([&](int, uint64_t k) {
                     if (k >= lo && k <= hi) few[atomicAdd(&listed, 1)] = k;
-                }
+                });
                 __syncthreads();
                 if (w == 0) {
                     const uint64_t mine = lane < in ? few[lane] : 0;
@@ -292,33 +302,46 @@ __global__ __launch_bounds__(kPickThreads) void cache_pick_kernel(SelectArgs a) 
             }
         }
     }
-    // In ascending order: pages before a thread's, by ballots.
-    int base = 0, same = 0;
-    for (int p0 = 0; p0 < n; p0 += kPickThreads) {
-        const int p = p0 + tid;
-        const uint64_t k = p < n ? key(p) : 0;
-        const bool above = k > last, on = last != 0 && k == last;
-        const uint64_t ma = __ballot(above), mo = __ballot(on), below = (1ull << lane) - 1;
-        __syncthreads();  // (wave_n of the round before has been read)
-        if (lane == 0) {
-            wave_n[w] = __builtin_popcountll(ma);
-            wave_n[kPickWaves + w] = __builtin_popcountll(mo);
+    // In ascending order: how many are above and equal before a thread's own.
+    int above = 0, on = 0;
+    each([&](int, uint64_t k) {
+        above += k > last;
+        on += last != 0 && k == last;
+    });
+    int above0 = above, on0 = on;
+    for (int o = 1; o < 64; o *= 2) {
+        const int x = __shfl_up(above0, o), y = __shfl_up(on0, o);
+        if (lane >= o) {
+            above0 += x;
+            on0 += y;
         }
-        __syncthreads();
-        int a0 = base, s0 = same;
-        for (int x = 0; x < kPickWaves; ++x) {
-            if (x < w) {
-                a0 += wave_n[x];
-                s0 += wave_n[kPickWaves + x];
-            }
-            base += wave_n[x];
-            same += wave_n[kPickWaves + x];
-        }
-        const int ra = a0 + __builtin_popcountll(ma & below), rs = s0 + __builtin_popcountll(mo & below);
-        const int at = ra + (rs < equal ? rs : equal);
-        if ((above || (on && rs < equal)) && at < a.count) out[at] = p;
     }
-    const int taken = base + (same < equal ? same : equal);
+    if (lane == 63) {
+        wave_n[2 * kPickWaves + w] = above0;
+        wave_n[3 * kPickWaves + w] = on0;
+    }
+    above0 -= above;
+    on0 -= on;
+    __syncthreads();
+    int above_all = 0, on_all = 0;
+#pragma unroll
+    for (int k = 0; k < kPickWaves; ++k) {
+        const int x = wave_n[2 * kPickWaves + k], y = wave_n[3 * kPickWaves + k];
+        if (k < w) {
+            above0 += x;
+            on0 += y;
+        }
+        above_all += x;
+        on_all += y;
+    }
+    each([&](int x, uint64_t k) {
+        const bool is_above = k > last, is_on = last != 0 && k == last;
+        const int at = above0 + (on0 < equal ? on0 : equal);
+        if ((is_above || (is_on && on0 < equal)) && at < a.count) out[at] = per * tid + x;
+        above0 += is_above;
+        on0 += is_on;
+    });
+    const int taken = above_all + (on_all < equal ? on_all : equal);
     for (int p = taken + tid; p < a.count; p += kPickThreads) out[p] = -1;
 }
 
@@ -362,7 +385,14 @@ hipError_t launch_cache_select(const ShaoboFa3CacheSelectParams& p, hipStream_t 
         else
             hipLaunchKernelGGL(cache_score_kernel<false>, grid, dim3(256), 0, stream, a);
     }
-    hipLaunchKernelGGL(cache_pick_kernel, dim3(rows), dim3(kPickThreads), 0, stream, a);
+    auto pick = [&](auto kernel) {
+        hipLaunchKernelGGL(kernel, dim3(rows), dim3(kPickThreads), 0, stream, a);
+    };
+    if (a.c.width <= kPickThreads) pick(cache_pick_kernel<1>);
+    else if (a.c.width <= 2 * kPickThreads) pick(cache_pick_kernel<2>);
+    else if (a.c.width <= 4 * kPickThreads) pick(cache_pick_kernel<4>);
+    else if (a.c.width <= 8 * kPickThreads) pick(cache_pick_kernel<8>);
+    else pick(cache_pick_kernel<0>);
     return hipGetLastError();
 }
 

@@ -173,7 +173,7 @@ struct FewCfg {
     static constexpr int kDB = D / 16;
     static constexpr int kSlot = kBlocks * (kDB * 1024 + 256);  // a wave's outputs and sums
     static constexpr int kMax = 4 * kBlocks * 256;              // the waves' maxima
-    static constexpr int kBytes = kMax + 3 * kSlot;
+    static constexpr int kBytes = kMax + 4 * kSlot;
 };
 
 template <int D, bool kBf16, bool kCap, bool kBias, bool kFour, int kBlocks>
@@ -329,16 +329,16 @@ __global__ __launch_bounds__(kRegThreads, few_waves(D, kFour, kBlocks)) void cac
 
     // A row without a maximum but with a sum has met NaN (FwdRows::settle).
     const auto& z = attn_args<Args>();
-    const CacheJob e = cache_job(z, blockIdx.x, 16 * kBlocks);
 #pragma unroll
     for (int q = 0; q < kBlocks; ++q) {
         sum[q] = sum_groups(sum[q]);
         const bool odd = mx[q] == kNegInf && sum[q] != 0.f;
         if (!__ballot(odd)) continue;
-        const bool some = cache_sees(z, e.row0 + 16 * q + l16, e.b, e.hkv, g4);
+        const bool some = cache_sees(z, job.row0 + 16 * q + l16, job.b, job.hkv, g4);
         if (odd && !some) sum[q] = 0.f;
     }
-    // The waves meet: sums and outputs at the largest maximum, wave 0 adds.
+    // The waves meet: sums and outputs at the largest maximum; wave w adds up
+    // and writes the channels kDB (4 g4 + w) ..
     FA3_LDS float* xm = (FA3_LDS float*)smem;
 #pragma unroll
     for (int q = 0; q < kBlocks; ++q) xm[(w * kBlocks + q) * 64 + lane] = mx[q];
@@ -354,62 +354,60 @@ __global__ __launch_bounds__(kRegThreads, few_waves(D, kFour, kBlocks)) void cac
         // (a NaN that is one: mx -inf, y 0, and the sum stays NaN)
         mx[q] = m;
         sum[q] *= y;
-        if (y == 0.f && sum[q] == 0.f) {  // (other rows' V may have been NaN)
+        const bool none = y == 0.f && sum[q] == 0.f;  // (other rows' V may have been NaN)
+        FA3_LDS char* slot = slots + w * C::kSlot + q * kDB * 1024 + lane * 16;
 #pragma unroll
-            for (int i = 0; i < kDB; ++i) o[i][q] = f32x4{};
-        } else {
+        for (int i = 0; i < kDB; ++i) {
+            f32x4 x;
 #pragma unroll
-            for (int i = 0; i < kDB; ++i) o[i][q] *= y;
+            for (int c = 0; c < 4; ++c) x[c] = none ? 0.f : o[4 * (i % (kDB / 4)) + c][q][i / (kDB / 4)] * y;
+            *(FA3_LDS f32x4*)(slot + i * 1024) = x;
         }
-    }
-    if (w > 0) {
-        FA3_LDS char* slot = slots + (w - 1) * C::kSlot;
-#pragma unroll
-        for (int q = 0; q < kBlocks; ++q) {
-#pragma unroll
-            for (int i = 0; i < kDB; ++i)
-                *(FA3_LDS f32x4*)(slot + (q * kDB + i) * 1024 + lane * 16) = o[i][q];
-            *(FA3_LDS float*)(slot + kBlocks * kDB * 1024 + q * 256 + lane * 4) = sum[q];
-        }
+        *(FA3_LDS float*)(slots + w * C::kSlot + kBlocks * kDB * 1024 + q * 256 + lane * 4) = sum[q];
     }
     wait_vm_lgkm0<0>();
     barrier();
-    if (w > 0) return;
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
-        FA3_LDS char* slot = slots + k * C::kSlot;
-#pragma unroll
-        for (int q = 0; q < kBlocks; ++q) {
-#pragma unroll
-            for (int i = 0; i < kDB; ++i)
-                o[i][q] += *(FA3_LDS f32x4*)(slot + (q * kDB + i) * 1024 + lane * 16);
-            sum[q] += *(FA3_LDS float*)(slot + kBlocks * kDB * 1024 + q * 256 + lane * 4);
-        }
-    }
 #pragma unroll
     for (int q = 0; q < kBlocks; ++q) {
-        const int row = e.row0 + 16 * q + l16;
-        if (row >= e.end) continue;
-        const bool none = mx[q] == kNegInf && sum[q] == 0.f;
-        const float inv = none ? 0.f : 1.f / sum[q];
-        const float lse2 = none ? kNegInf : mx[q] + __builtin_amdgcn_logf(sum[q]);
-        float y[4 * kDB];  // channels 4 kDB g4 ..
+        f32x4 y[kDB / 4] = {};
+        float total = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4 * kDB; ++i) y[i] = none ? 0.f : o[i % kDB][q][i / kDB] * inv;
+        for (int k = 0; k < 4; ++k) {
+            FA3_LDS char* slot = slots + k * C::kSlot;
+#pragma unroll
+            for (int i = 0; i < kDB / 4; ++i)
+                y[i] += *(FA3_LDS f32x4*)(slot + (q * kDB + w * (kDB / 4) + i) * 1024 + lane * 16);
+            total += *(FA3_LDS float*)(slot + kBlocks * kDB * 1024 + q * 256 + lane * 4);
+        }
+        const int row = job.row0 + 16 * q + l16;
+        if (row >= job.end) continue;
+        const bool none = mx[q] == kNegInf && total == 0.f;
+        const float inv = none ? 0.f : 1.f / total;
+        const float lse2 = none ? kNegInf : mx[q] + __builtin_amdgcn_logf(total);
+        float out[kDB];
+#pragma unroll
+        for (int i = 0; i < kDB; ++i) out[i] = none ? 0.f : y[i / 4][i % 4] * inv;
+        const int c = kDB * (4 * g4 + w);
+        const bool first = g4 == 0 && w == 0;
         if (z.splits > 1) {
-            const int64_t at = ((int64_t)e.split * z.groups + e.grp) * z.rows + row;
-            if (g4 == 0) z.part_l[at] = lse2;
-            float* p = z.part_o + at * D + 4 * kDB * g4;
+            const int64_t at = ((int64_t)job.split * z.groups + job.grp) * z.rows + row;
+            if (first) z.part_l[at] = lse2;
 #pragma unroll
-            for (int i = 0; i < kDB; ++i) *(f32x4*)(p + 4 * i) = *(const f32x4*)(y + 4 * i);
+            for (int i = 0; i < kDB / 4; ++i) *(f32x4*)(z.part_o + at * D + c + 4 * i) = *(const f32x4*)(out + 4 * i);
             continue;
         }
-        const AttnRow r = attn_row(row, e.end, e.hkv, z.group, z.div_group);
-        if (g4 == 0) z.lse[((int64_t)e.b * z.heads_q + r.h) * z.sq + r.i] = lse2 * 0.69314718055994531f;
-        _Float16* p = z.out.p + e.b * z.out.bs + r.h * z.out.hs + r.i * z.out.rs + 4 * kDB * g4;
+        const AttnRow r = attn_row(row, job.end, job.hkv, z.group, z.div_group);
+        if (first) z.lse[((int64_t)job.b * z.heads_q + r.h) * z.sq + r.i] = lse2 * 0.69314718055994531f;
+        if (c >= z.d) continue;
+        _Float16* p = z.out.p + job.b * z.out.bs + r.h * z.out.hs + r.i * z.out.rs + c;
+        if constexpr (kDB == 8) {
+            *(f16x8*)p = pack8<kBf16>(out);
+        } else {
+            f16x4 x;
 #pragma unroll
-        for (int i = 0; i < kDB / 2; ++i)
-            if (4 * kDB * g4 + 8 * i < z.d) *(f16x8*)(p + 8 * i) = pack8<kBf16>(y + 8 * i);
+            for (int i = 0; i < 4; ++i) x[i] = to16<kBf16>(out[i]);
+            *(f16x4*)p = x;
+        }
     }
 }
 

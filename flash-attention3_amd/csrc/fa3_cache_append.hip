@@ -197,18 +197,18 @@ __device__ __forceinline__ void append_v(const AppendRun& r) {
     }
 }
 
-// Keys of 16-bit values that order as unsigned integers, NaN below all (kHigh:
-// above all).
-template <bool kBf16, bool kHigh>
-__device__ __forceinline__ uint32_t order_of(_Float16 x) {
-    const uint32_t b = __builtin_bit_cast(uint16_t, x);
-    if ((b & 0x7FFFu) > (kBf16 ? 0x7F80u : 0x7C00u)) return kHigh ? 0xFFFFu : 0u;
-    return (b & 0x8000u ? ~b : b | 0x8000u) & 0xFFFFu;
-}
-__device__ __forceinline__ uint16_t of_order(uint32_t k) {
-    return (uint16_t)(k & 0x8000u ? k & 0x7FFFu : ~k);
-}
+// Two 16-bit values as unsigned integers of the same order (a NaN beyond the
+// infinity of its sign), and back.
 typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+typedef int16_t i16x2 __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ uint32_t order_of(uint32_t x) {
+    const uint32_t sign = __builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, x) >> (i16x2)15);
+    return x ^ (sign | 0x80008000u);
+}
+__device__ __forceinline__ uint32_t of_order(uint32_t k) {
+    const uint32_t sign = __builtin_bit_cast(uint32_t, __builtin_bit_cast(i16x2, k) >> (i16x2)15);
+    return k ^ (~sign | 0x80008000u);
+}
 template <bool kHigh>
 __device__ __forceinline__ uint32_t edge16(uint32_t x, uint32_t y) {
     const u16x2 u = __builtin_bit_cast(u16x2, x), v = __builtin_bit_cast(u16x2, y);
@@ -216,7 +216,6 @@ __device__ __forceinline__ uint32_t edge16(uint32_t x, uint32_t y) {
                                               : __builtin_elementwise_min(u, v));
 }
 // A lane's smallest and largest keys of its 8 channels.
-template <bool kBf16>
 struct Edges {
     uint32_t low[4], high[4];  // channels 2 i, 2 i + 1
     __device__ __forceinline__ void none() {
@@ -224,12 +223,11 @@ struct Edges {
         for (int i = 0; i < 4; ++i) low[i] = 0xFFFFFFFFu, high[i] = 0u;
     }
     __device__ __forceinline__ void take(const f16x8& x) {
+        const u32x4 k = __builtin_bit_cast(u32x4, x);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            low[i] = edge16<false>(low[i], order_of<kBf16, false>(x[2 * i]) |
-                                               order_of<kBf16, false>(x[2 * i + 1]) << 16);
-            high[i] = edge16<true>(high[i], order_of<kBf16, true>(x[2 * i]) |
-                                                order_of<kBf16, true>(x[2 * i + 1]) << 16);
+            low[i] = edge16<false>(low[i], order_of(k[i]));
+            high[i] = edge16<true>(high[i], order_of(k[i]));
         }
     }
     __device__ __forceinline__ void meet(int lanes) {  // those `lanes` apart
@@ -255,23 +253,15 @@ struct Edges {
     // as 16-bit values, with those that the page has (unless it starts anew)
     __device__ __forceinline__ void store(char* bounds, int c, int d, const f16x8& old_low,
                                           const f16x8& old_high, bool anew) {
-        f16x8 l, h;
-        if (!anew) {
+        const u32x4 x = __builtin_bit_cast(u32x4, old_low), y = __builtin_bit_cast(u32x4, old_high);
+        u32x4 l, h;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                low[i] = edge16<false>(low[i], order_of<kBf16, false>(old_low[2 * i]) |
-                                                   order_of<kBf16, false>(old_low[2 * i + 1]) << 16);
-                high[i] = edge16<true>(high[i], order_of<kBf16, true>(old_high[2 * i]) |
-                                                    order_of<kBf16, true>(old_high[2 * i + 1]) << 16);
-            }
+        for (int i = 0; i < 4; ++i) {
+            l[i] = of_order(anew ? low[i] : edge16<false>(low[i], order_of(x[i])));
+            h[i] = of_order(anew ? high[i] : edge16<true>(high[i], order_of(y[i])));
         }
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            l[i] = __builtin_bit_cast(_Float16, of_order(low[i / 2] >> (i % 2 * 16) & 0xFFFFu));
-            h[i] = __builtin_bit_cast(_Float16, of_order(high[i / 2] >> (i % 2 * 16) & 0xFFFFu));
-        }
-        *(f16x8*)(bounds + 16 * c) = l;
-        *(f16x8*)(bounds + 2 * d + 16 * c) = h;
+        *(u32x4*)(bounds + 16 * c) = l;
+        *(u32x4*)(bounds + 2 * d + 16 * c) = h;
     }
 };
 
@@ -289,7 +279,7 @@ __device__ __forceinline__ void append_turned(const AppendRun& r, uint32_t* edge
     const int c0 = turns ? u : pairs / 4 + u - turned, c1 = pairs / 8 + u;
     constexpr int kN = kInterleaved ? 4 : 8;
     // the page's bounds, read long before they are needed
-    Edges<kBf16> e0, e1;
+    Edges e0, e1;
     f16x8 old[4] = {};
     char* bounds = nullptr;
     const bool anew = ((r.place0 + r.i0) & ((1 << a.c.shift) - 1)) == 0;

@@ -248,6 +248,11 @@ __global__ __launch_bounds__(kRegThreads, few_waves(D, kFour, kBlocks)) void cac
             }
         }
         // log2-domain scores
+        float far[kBlocks];
+        if constexpr (kBias) {
+#pragma unroll
+            for (int q = 0; q < kBlocks; ++q) far[q] = (float)(place[q] - (j0 + 4 * g4));
+        }
 #pragma unroll
         for (int q = 0; q < kBlocks; ++q)
 #pragma unroll
@@ -259,8 +264,8 @@ __global__ __launch_bounds__(kRegThreads, few_waves(D, kFour, kBlocks)) void cac
                         x = (fine ? attn_tanh_fine(x, k1) : attn_tanh(x, k1)) * cap2;
                     else
                         x *= c;
-                    if constexpr (kBias)
-                        x = __builtin_fmaf(-slope[q], __builtin_fabsf((float)(place[q] - (j0 + 16 * t + 4 * g4 + e))), x);
+                    if constexpr (kBias)  // (exact: a difference of places, then fp32)
+                        x = __builtin_fmaf(-slope[q], __builtin_fabsf(far[q] - (float)(16 * t + e)), x);
                     s[t][q][e] = x;
                 }
         if (j0 + 32 > lim_min) {

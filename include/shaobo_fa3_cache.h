@@ -28,7 +28,8 @@
  * Bounds: [pages, num_heads_kv, 2, head_dim] in dtype, contiguous: for each
  * channel the smallest and the largest key (before it becomes 4 bits) that
  * appends have written to the page; a row at a page's first place starts them
- * anew.  Rows written over otherwise leave them as wide as they were.
+ * anew.  Rows written over otherwise leave them as wide as they were.  A NaN is
+ * beyond the infinity of its sign.
  *
  * Streams, launches and workspaces are as in shaobo_fa3_attn.h.
  */

@@ -11,26 +11,21 @@ namespace {
 // Tokens of sequence b with the call's, and how many rows of the call are tokens.
 template <typename C>
 __device__ __forceinline__ int cache_kv(const C& c, int b) {
-    const int kv = scalar_load(c.kv_lens + b), most = c.width << c.shift;
-    return kv < 0 ? 0 : kv < most ? kv : most;
+    return cache_length(scalar_load(c.kv_lens + b), c.width << c.shift);
 }
 template <typename C>
 __device__ __forceinline__ int cache_new(const C& c, int b, int seqlen) {
-    if (c.new_lens == nullptr) return seqlen;
-    const int n = scalar_load(c.new_lens + b);
-    return n < 0 ? 0 : n < seqlen ? n : seqlen;
+    return c.new_lens == nullptr ? seqlen : cache_length(scalar_load(c.new_lens + b), seqlen);
 }
 // The page of positions [n << shift, (n + 1) << shift), 0 <= n < width; -1 for none.
 template <typename C>
 __device__ __forceinline__ int cache_page(const C& c, int b, int n) {
-    const int p = c.table[b * c.table_s + n];
-    return (unsigned)p < (unsigned)c.pages ? p : -1;
+    return cache_page_of(c.table[b * c.table_s + n], c.pages);
 }
 // The same where b and n are one for all lanes.
 template <typename C>
 __device__ __forceinline__ int cache_page_scalar(const C& c, int b, int n) {
-    const int p = scalar_load(c.table + b * c.table_s + n);
-    return (unsigned)p < (unsigned)c.pages ? p : -1;
+    return cache_page_of(scalar_load(c.table + b * c.table_s + n), c.pages);
 }
 
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));

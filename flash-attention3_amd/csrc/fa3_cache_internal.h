@@ -7,6 +7,13 @@
 
 namespace fa3 {
 
+// What a page table holds and what a caller's lengths say, made safe: a page's
+// number or -1, a length within 0 .. most.
+__host__ __device__ inline int cache_page_of(int entry, int pages) {
+    return (unsigned)entry < (unsigned)pages ? entry : -1;
+}
+__host__ __device__ inline int cache_length(int n, int most) { return n < 0 ? 0 : n < most ? n : most; }
+
 // A cache as the kernels take it; strides in bytes.
 struct CacheView {
     char *k, *v;

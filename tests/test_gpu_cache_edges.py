@@ -1,0 +1,506 @@
+"""The paged cache where it can go wrong: what lies behind sequences and in
+other pages, NaN that is seen and NaN that is not, strides and far offsets,
+streams, graphs, a served sequence against the whole prompt, refusals."""
+import ctypes
+import math
+
+import pytest
+
+import attn_oracle as A
+import cache_oracle as O
+import shaobo_fa3 as F
+from test_gpu_attn import i32, refused, within
+from test_gpu_cache import append_case, attn_case, check_append, check_attn, gen_of, make_cache, rows, where
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+BF, HF = torch.bfloat16, torch.float16
+
+
+@pytest.fixture(scope="module")
+def T():
+    if not torch.cuda.is_available():
+        pytest.skip("no GPU")
+    F.load()
+    import shaobo_fa3_torch
+    assert shaobo_fa3_torch._ATTN, "lib/_fa3_torch_attn.so is not built"
+    return shaobo_fa3_torch
+
+
+def spoiled(cache):
+    """The cache with NaN and infinities (4 bits: any bytes, NaN for scales)
+    wherever no sequence has a row, and pages of others behind the sequences."""
+    used = torch.zeros(cache["k"].shape[0], cache["page_size"], dtype=torch.bool, device="cuda")
+    table, ps = cache["table"].clone(), cache["page_size"]
+    for b in range(table.shape[0]):
+        ok, page, row = O.there(cache, b)
+        used[page[ok], row[ok]] = True
+        n = -(-O.clipped(cache, b)[0] // ps)
+        table[b, n:] = torch.arange(table.shape[1] - n, device="cuda", dtype=torch.int32) % used.shape[0]
+    out = dict(cache, table=table)
+    for n in ("k", "v"):
+        x = cache[n].clone()
+        if cache["bits"] == 16:
+            junk = torch.tensor([math.nan, math.inf, -math.inf], device="cuda", dtype=x.dtype)
+            x = torch.where(used[:, None, :, None], x, junk[torch.randint(0, 3, x.shape, device="cuda",
+                                                                           generator=gen_of(2))])
+        else:
+            code, scale = O.parts(x)
+            noise = torch.randint(0, 16, code.shape, device="cuda", generator=gen_of(3), dtype=torch.int32)
+            code = torch.where(used[:, None, :, None], code, noise)
+            scale = torch.where(used[:, None, :], scale, torch.full_like(scale, math.nan))
+            x = O.pack(code, scale)
+        out[n] = x
+    return out
+
+
+EDGE = [dict(kv=[1, 33, 70], Hq=4), dict(kv=[130, 257], Hq=8, D=128), dict(kv=[61, 3000], D=128, ps=128),
+        dict(kv=[90, 200], S=70, D=128), dict(kv=[101, 333], S=130, Hq=4, ps=32), dict(kv=[45, 3], new=[9, 2], S=12),
+        dict(kv=[200], S=3, holes=[1], Hq=4, D=128), dict(kv=[200, 90], slopes=1, S=2), dict(kv=[200, 90], S=80, softcap=5.0)]
+
+
+@pytest.mark.parametrize("bits,dtype", [(16, BF), (4, BF), (16, HF), (4, HF)])
+@pytest.mark.parametrize("case", EDGE, ids=str)
+def test_other_rows_may_hold_anything(T, case, bits, dtype):
+    """Behind the sequences and in pages of nobody: bit for bit the same.  Padding
+    rows of q too."""
+    cache, q, o = attn_case(case, bits, dtype)
+    want = check_attn(T, cache, q, o)
+    for b, n in enumerate(cache["new"]):
+        q[b, :, n:] = math.nan
+    bad = spoiled(cache)
+    kw = dict(causal=o["causal"], softmax_scale=o["scale"], softcap=o["softcap"], slopes=o.get("slopes"), return_lse=True)
+    got = T.cache_attention(q, bad["k"], bad["v"], **where(bad), **kw)
+    torch.cuda.synchronize()
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    N = cache["table"].shape[1]
+    every = torch.arange(N, device="cuda", dtype=torch.int32).expand(*q.shape[:1], cache["k"].shape[1], q.shape[2], N)
+    a = T.cache_attention(q, cache["k"], cache["v"], selected=every.contiguous(), **where(cache), **kw)
+    b = T.cache_attention(q, bad["k"], bad["v"], selected=every.contiguous(), **where(bad), **kw)
+    torch.cuda.synchronize()
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+    x = T.cache_read(cache["k"], cache["v"], page_table=cache["table"], kv_lens=i32(cache["kv"]), seqlen=400, dtype=dtype)
+    y = T.cache_read(bad["k"], bad["v"], page_table=bad["table"], kv_lens=i32(cache["kv"]), seqlen=400, dtype=dtype)
+    assert all(torch.equal(c, d) for c, d in zip(x, y))
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("case", [dict(kv=[1]), dict(kv=[200], Hq=8, D=128), dict(kv=[3000], D=128), dict(kv=[300], S=150),
+                                  dict(kv=[300], S=150, D=128, softcap=5.0), dict(kv=[100], S=5, slopes=1)], ids=str)
+def test_visible_nan_shows(T, case, bits):
+    """A row whose q is NaN, or that sees a key that is, has NaN for output and
+    log-sum-exp; rows of other heads of another KV head do not."""
+    cache, q, o = attn_case(case, bits, BF)
+    kw = dict(causal=o["causal"], softcap=o["softcap"], slopes=o.get("slopes"), return_lse=True)
+    q2 = q.clone()
+    q2[0, 0, -1] = math.nan
+    out, lse = T.cache_attention(q2, cache["k"], cache["v"], **where(cache), **kw)
+    assert torch.isnan(out[0, 0, -1]).all() and torch.isnan(lse[0, 0, -1])
+    assert torch.isfinite(out[0, q.shape[1] // 2:]).all()
+    # a key, the last of the sequence: seen by the last row alone
+    kv, ps = case["kv"][0], cache["page_size"]
+    page, row = int(cache["table"][0, (kv - 1) // ps]), (kv - 1) % ps
+    if bits == 16:
+        cache["k"][page, 0, row, 3] = math.nan
+    else:
+        code, scale = O.parts(cache["k"])
+        scale[page, 0, row] = math.nan
+        cache["k"] = O.pack(code, scale)
+    out, lse = T.cache_attention(q, cache["k"], cache["v"], **where(cache), **kw)
+    G = q.shape[1] // cache["k"].shape[1]
+    assert torch.isnan(out[0, :G, -1]).all() and torch.isnan(lse[0, :G, -1]).all()
+    assert torch.isfinite(out[0, G:]).all() and torch.isfinite(lse[0, G:]).all()
+
+
+def test_rows_that_see_nothing_beside_nan(T):
+    """Non-causal rows without keys (every page is none) and padding rows are
+    zeros whatever q holds."""
+    for bits in (16, 4):
+        for S in (3, 100):
+            cache, q, o = attn_case(dict(kv=[150, 90], new=[S - 1, S], S=S, Hq=4, D=128, causal=False), bits, BF)
+            cache["table"][1] = -1
+            q[1], q[0, :, -1] = math.nan, math.inf
+            out, lse = T.cache_attention(q, cache["k"], cache["v"], causal=False, return_lse=True, **where(cache))
+            assert (out[1] == 0).all() and (lse[1] == -math.inf).all()
+            assert (out[0, :, -1] == 0).all() and (lse[0, :, -1] == -math.inf).all()
+            assert torch.isfinite(out[0, :, :-1]).all()
+
+
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("S", [1, 5, 90])
+def test_strides(T, bits, S):
+    """Pages of k and v in one pool, 16-bit rows of all heads of a place side by
+    side, a table that is part of a wider one, rows that are views."""
+    cache, q, o = attn_case(dict(kv=[200, 77], S=S, Hq=8, Hkv=4, D=128, ps=32), bits, BF)
+    want = check_attn(T, cache, q, o)
+    n, H, ps, row = cache["k"].shape
+    pool = torch.zeros(n, 2, H, ps, row, dtype=cache["k"].dtype, device="cuda")
+    if bits == 16:
+        pool = torch.zeros(n, ps, 2, H, row, dtype=BF, device="cuda").permute(0, 2, 3, 1, 4)
+    views = dict(cache, k=pool[:, 0], v=pool[:, 1])
+    views["k"].copy_(cache["k"])
+    views["v"].copy_(cache["v"])
+    wide = torch.full((2, cache["table"].shape[1] + 5), 12345, dtype=torch.int32, device="cuda")
+    wide[:, 2:2 + cache["table"].shape[1]] = cache["table"]
+    views["table"] = wide[:, 2:2 + cache["table"].shape[1]]
+    big = torch.zeros(2, S + 3, 8 + 2, 128 + 8, dtype=BF, device="cuda")
+    qv = big[:, 1:S + 1, 1:9, :128].transpose(1, 2)
+    qv.copy_(q)
+    out, lse = T.cache_attention(qv, views["k"], views["v"], return_lse=True, **where(views))
+    assert torch.equal(out, want[0]) and torch.equal(lse, want[1])
+    # the same rows appended through both
+    gen = gen_of(5)
+    k, v = (rows(gen, 2, 4, S, 128, BF, True) for _ in range(2))
+    bounds = [torch.zeros(n, H, 2, 128, dtype=BF, device="cuda") for _ in range(2)]
+    fr = T.rotary_freqs([64], device="cuda")
+    got = [T.cache_append(k, v, c["k"], c["v"], q=x, freqs=fr, bounds=b, **where(c))
+           for c, x, b in ((cache, q, bounds[0]), (views, qv, bounds[1]))]
+    assert torch.equal(got[0], got[1]) and torch.equal(*bounds)
+    assert torch.equal(cache["k"], views["k"].contiguous()) and torch.equal(cache["v"], views["v"].contiguous())
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_offsets_past_32_bits(T, bits):
+    """Pages more than 2^32 bytes into their tensor."""
+    H, ps, D = 8, 128, 128
+    pages = 2 ** 32 // (H * ps * (2 * D if bits == 16 else D // 2 + 4)) + 40
+    k, v, bounds = T.cache_pages(pages, H, ps, D, BF, bits=bits, bounds=True)
+    table = i32([[pages - 1, pages - 7, pages - 3], [pages - 2, 5, pages - 20]])
+    cache = dict(k=k, v=v, bits=bits, table=table, kv=[300, 270], new=[300, 200], page_size=ps, D=D, dtype=BF)
+    gen = gen_of(4)
+    x, y = (rows(gen, 2, H, 300, D, BF) for _ in range(2))
+    q = rows(gen, 2, H, 300, D, BF)
+    T.cache_append(x, y, k, v, bounds=bounds, **where(cache))
+    got = T.cache_read(k, v, page_table=table, kv_lens=i32([300, 270]), seqlen=300, dtype=BF)
+    if bits == 16:
+        assert torch.equal(got[0][0], x[0]) and torch.equal(got[1][0], y[0])
+        assert torch.equal(got[0][1, :, 70:270], x[1, :, :200])
+    small = dict(cache, k=k[-40:].clone(), v=v[-40:].clone(), table=(table - (pages - 40)).clamp(min=-1))
+    assert int(bounds[pages - 1].float().abs().sum()) > 0
+    for S in (1, 100):
+        c = dict(cache, new=[S, S])
+        s = dict(small, new=[S, S])
+        c["table"] = table.clone()
+        c["table"][1, 1] = -1  # (page 5 is not among the small ones)
+        a = T.cache_attention(q[:, :, :S].contiguous(), k, v, return_lse=True, **where(c))
+        b = T.cache_attention(q[:, :, :S].contiguous(), s["k"], s["v"], return_lse=True, **where(s))
+        assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+        check_attn(T, s, q[:, :, :S].contiguous(), dict(causal=True, softcap=0.0, scale=None))
+    sel = T.cache_select(q[:, :, :1].contiguous(), bounds, page_table=table, kv_lens=i32([300, 270]), page_size=ps, count=2)
+    assert torch.equal(sel, O.select(q[:, :, :1], bounds, dict(cache, new=[1, 1]), 2))
+
+
+def test_turned_in_place_and_beside(T):
+    """The C entry: q's output may be q, and nothing around its rows is written."""
+    lib = F.load()
+    B, Hq, Hkv, S, D, ps = 2, 6, 2, 21, 64, 32
+    gen = gen_of(7)
+    k, v = (rows(gen, B, Hkv, S, D, BF) for _ in range(2))
+    room = torch.full((B, Hq, S + 2, D + 16), 7.0, dtype=BF, device="cuda")
+    q = room[:, :, 1:S + 1, 8:8 + D]
+    q.copy_(rows(gen, B, Hq, S, D, BF))
+    cache = make_cache(gen, [40, 21], [S, S], Hkv, D, ps)
+    fr = T.rotary_freqs([32], device="cuda")
+    want = T.cache_append(k, v, cache["k"], cache["v"], q=q, freqs=fr, **where(cache))
+    lens, new = i32([40, 21]), i32([S, S])
+    p = F.CacheAppendParams()
+    lib.shaobo_fa3_cache_append_params_init(ctypes.byref(p))
+    p.seqlen, p.num_heads_q, p.pairs, p.freqs = S, Hq, 32, fr.data_ptr()
+    c = p.cache
+    c.batch, c.num_heads_kv, c.head_dim, c.dtype = B, Hkv, D, F.DTYPE_BF16
+    c.pages, c.page_size, c.width = cache["k"].shape[0], ps, cache["table"].shape[1]
+    for n in ("k", "v"):
+        t = getattr(c, n)
+        t.data, (t.page_stride, t.head_stride, t.row_stride, _) = cache[n].data_ptr(), cache[n].stride()
+    c.page_table, c.page_table_stride = cache["table"].data_ptr(), cache["table"].stride(0)
+    c.kv_lens, c.new_lens = lens.data_ptr(), new.data_ptr()
+    for n, t in (("k", k), ("v", v), ("q", q), ("q_out", q)):
+        x = getattr(p, n)
+        x.data, (x.batch_stride, x.head_stride, x.row_stride, _) = t.data_ptr(), t.stride()
+    before = cache["k"].clone()
+    assert lib.shaobo_fa3_cache_append(ctypes.byref(p), torch.cuda.current_stream().cuda_stream) == F.SUCCESS
+    torch.cuda.synchronize()
+    assert torch.equal(q, want) and torch.equal(cache["k"], before)
+    edge = room.clone()
+    edge[:, :, 1:S + 1, 8:8 + D] = 7.0
+    assert (edge == 7.0).all()
+
+
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("D,ps", [(64, 32), (128, 64)])
+def test_one_by_one_equals_at_once(T, bits, D, ps):
+    """Tokens appended singly, in parts and together: the same pages and bounds."""
+    gen = gen_of(3)
+    k, v, q = (rows(gen, 2, h, 150, D, BF) for h in (2, 2, 4))
+    table = torch.randperm(10, generator=gen, device="cuda").int().view(2, 5)
+    fr = T.rotary_freqs([D // 2], device="cuda")
+    results = []
+    for cuts in ([150], [1] * 150, [70, 1, 1, 40, 38]):
+        kp, vp, bounds = T.cache_pages(10, 2, ps, D, BF, bits=bits, bounds=True)
+        at, qs = 0, []
+        for n in cuts:
+            at += n
+            qs.append(T.cache_append(*(x[:, :, at - n:at].contiguous() for x in (k, v)), kp, vp,
+                                     q=q[:, :, at - n:at].contiguous(), freqs=fr, bounds=bounds,
+                                     page_table=table, kv_lens=i32([at, at])))
+        results.append((kp, vp, bounds, torch.cat(qs, 2)))
+    for r in results[1:]:
+        for a, b in zip(results[0], r):
+            assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+
+
+@pytest.mark.parametrize("cap", [0.0, 8.0])
+def test_serving_equals_the_prompt(T, cap):
+    """rotary + score_attention over a whole sequence against a prompt appended
+    in two parts and tokens one by one, with and without selection of all pages."""
+    B, Hq, Hkv, S, D, ps = 2, 8, 2, 170, 128, 32
+    gen = gen_of(11)
+    q, k, v = (rows(gen, B, h, S, D, BF, True) for h in (Hq, Hkv, Hkv))
+    fr = T.rotary_freqs([D // 2], device="cuda")
+    pos = torch.arange(S, device="cuda").expand(1, B, S)
+    kp, vp, bounds = T.cache_pages(20, Hkv, ps, D, BF, bounds=True)
+    table = torch.randperm(20, generator=gen, device="cuda").int().view(B, 10)
+    outs, cuts = [], [100, 58] + [1] * 12
+    at, qs, lses = 0, [], []
+    for n in cuts:
+        at += n
+        part = [x[:, :, at - n:at] for x in (q, k, v)]
+        where_ = dict(page_table=table, kv_lens=i32([at, at]))
+        qt = T.cache_append(part[1], part[2], kp, vp, q=part[0], freqs=fr, bounds=bounds, **where_)
+        out, lse = T.cache_attention(qt, kp, vp, softcap=cap, return_lse=True, **where_)
+        if n == 1:
+            sel = T.cache_select(qt, bounds, page_size=ps, count=10, **where_)
+            o2, l2 = T.cache_attention(qt, kp, vp, softcap=cap, selected=sel, return_lse=True, **where_)
+            assert (out.double() - o2.double()).abs().max() <= 2.0 ** -7 * out.double().abs().max()
+            assert (lse - l2).abs().max() <= 1e-4
+        outs.append(out), qs.append(qt), lses.append(lse)
+    kt, vt = T.cache_read(kp, vp, page_table=table, kv_lens=i32([S, S]), seqlen=S, dtype=BF)
+    assert torch.equal(vt, v)
+    # the layer's own rotation differs by fp32's rounding before the one to 16 bits
+    qr, kr = T.rotary(q, k, positions=pos, freqs=fr)
+    step = 2.0 ** -7
+    assert ((kr - kt).abs() <= step * kr.abs() + 1e-6).all()
+    want, wlse, off, lse_off = A.forward(torch.cat(qs, 2), kt, vt, True, softcap=cap)
+    within("lse", torch.cat(lses, 2), wlse, lse_off)
+    within("out", torch.cat(outs, 2), want, off)
+    dense, dlse = T.score_attention(torch.cat(qs, 2), kt, vt, softcap=cap, return_lse=True)
+    within("dense", dense, want, off)
+    within("dense lse", dlse, wlse, lse_off)
+
+
+def step(T, s):
+    """One decoding step of a state: append, select, attend twice."""
+    w = dict(page_table=s["table"], kv_lens=s["lens"])
+    qt = T.cache_append(s["k"], s["v"], s["kp"], s["vp"], q=s["q"], freqs=s["fr"], bounds=s["bounds"], **w)
+    sel = T.cache_select(qt, s["bounds"], page_size=s["ps"], count=4, **w)
+    return (qt, sel, *T.cache_attention(qt, s["kp"], s["vp"], return_lse=True, **w),
+            *T.cache_attention(qt, s["kp"], s["vp"], selected=sel, return_lse=True, **w))
+
+
+def step_state(T, bits, S=1, seed=1, old=900):
+    gen = gen_of(seed)
+    B, Hq, Hkv, D, ps = 3, 8, 2, 128, 64
+    kp, vp, bounds = T.cache_pages(60, Hkv, ps, D, BF, bits=bits, bounds=True)
+    s = dict(kp=kp, vp=vp, bounds=bounds, ps=ps, fr=T.rotary_freqs([D // 2], device="cuda"))
+    s["table"] = torch.randperm(60, generator=gen, device="cuda").int().view(B, 20)
+    w = dict(page_table=s["table"], kv_lens=i32([old] * B))
+    k, v = (rows(gen, B, Hkv, old, D, BF) for _ in range(2))
+    T.cache_append(k, v, kp, vp, freqs=s["fr"], bounds=bounds, **w)
+    for n, h in (("q", Hq), ("k", Hkv), ("v", Hkv)):
+        s[n] = rows(gen, B, h, S, D, BF)
+    s["lens"] = i32([old + S, old // 2 + S, S])
+    return s
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_on_another_stream_and_on_two(T, bits):
+    states = [step_state(T, bits, seed=n) for n in (1, 2)]
+    want = [step(T, s) for s in states]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [None, None]
+    for _ in range(5):
+        for i in range(2):
+            with torch.cuda.stream(streams[i]):
+                got[i] = step(T, states[i])
+    torch.cuda.synchronize()
+    for a, b in zip(want, got):
+        assert all(torch.equal(x, y) for x, y in zip(a, b))
+
+
+@pytest.mark.parametrize("bits,S", [(16, 1), (4, 1), (4, 5), (16, 90)])
+def test_graph_capture(T, bits, S):
+    """A step captured twice and replayed with other tokens and lengths, eager
+    work between; every replay against the eager step on a copy of the cache."""
+    s = step_state(T, bits, S)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(T, s)
+    torch.cuda.current_stream().wait_stream(side)
+    graphs, outs = [], []
+    for _ in range(2):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(step(T, s))
+    for n in range(4):
+        other = step_state(T, bits, S, seed=20 + n)
+        for name in ("q", "k", "v"):
+            s[name].copy_(other[name])
+        s["lens"] += i32([1, 30, 3])
+        copy = dict(s, **{x: s[x].clone() for x in ("kp", "vp", "bounds")})
+        want = [x.clone() for x in step(T, copy)]
+        torch.cuda.synchronize()
+        for g, out in zip(graphs, outs):
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(want, out))
+            assert all(torch.equal(copy[x].view(torch.uint8), s[x].view(torch.uint8)) for x in ("kp", "vp", "bounds"))
+
+
+def test_results_are_reproducible(T):
+    for bits in (16, 4):
+        for kv, S in (([5000, 3000], 1), ([3000, 900], 70)):
+            cache, q, o = attn_case(dict(kv=kv, S=S, Hq=8, D=128), bits, BF)
+            a, b = (T.cache_attention(q, cache["k"], cache["v"], return_lse=True, **where(cache)) for _ in range(2))
+            assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_pages_with_nan_are_selected(T):
+    """A key that is NaN makes its page's bounds NaN on one side, and the page
+    comes first."""
+    s = step_state(T, 16, old=640)
+    k = rows(gen_of(9), 1, 2, 640, 128, BF)
+    k[0, :, 5 * 64 + 9, 7] = math.nan
+    k[0, :, 2 * 64 + 1, 100] = -math.inf
+    w = dict(page_table=s["table"][:1].contiguous(), kv_lens=i32([640]))
+    T.cache_append(k, k, s["kp"], s["vp"], bounds=s["bounds"], **w)
+    sel = T.cache_select(s["q"][:1], s["bounds"], page_size=64, count=3, **w)
+    assert (sel == i32([2, 5, 9])).all()
+
+
+def test_nothing_to_do(T):
+    """Empty batches, no rows, no pages, a table of no width."""
+    kp, vp, bounds = T.cache_pages(4, 2, 32, 64, BF, bounds=True)
+    fr = T.rotary_freqs([32], device="cuda")
+    for B, S, width in ((0, 3, 2), (2, 0, 2), (2, 3, 0)):
+        k = torch.zeros(B, 2, S, 64, dtype=BF, device="cuda")
+        w = dict(page_table=torch.zeros(B, width, dtype=torch.int32, device="cuda"),
+                 kv_lens=torch.full((B,), 3, dtype=torch.int32, device="cuda"))
+        pos = torch.zeros(1, B, S, dtype=torch.int32, device="cuda")
+        assert T.cache_append(k, k, kp, vp, q=k, freqs=fr, bounds=bounds, **w).shape == k.shape
+        assert T.cache_append(k, k, kp, vp, q=k, freqs=fr, positions=pos, **w).shape == k.shape
+        assert T.cache_append(k, k, kp, vp, **w) is None
+        sel = T.cache_select(k, bounds, page_size=32, count=2, **w)
+        assert sel.shape == (B, 2, S, 2) and (width or (sel == -1).all())
+        for s in (None, sel):
+            out, lse = T.cache_attention(k, kp, vp, selected=s, return_lse=True, **w)
+            assert out.shape == k.shape and (width or ((out == 0).all() and (lse == -math.inf).all()))
+        x, y = T.cache_read(kp, vp, seqlen=S, dtype=BF, **w)
+        assert x.shape == (B, 2, S, 64) and (x == 0).all()
+    torch.cuda.synchronize()
+    assert (kp == 0).all() and (bounds == 0).all()
+
+
+def test_lengths_out_of_range_are_taken_into_it(T):
+    """Lengths below 0, past the pages and past the rows."""
+    for bits in (16, 4):
+        cache, q, o = attn_case(dict(kv=[128, 128, 128], S=4, Hq=4), bits, BF)
+        for kv, new in (([-5, 1 << 30, 2147483647], [4, 4, 4]), ([128, 100, 3], [-7, 9, 2147483647])):
+            lens, fresh = i32(kv), i32(new)
+            out, lse = T.cache_attention(q, cache["k"], cache["v"], page_table=cache["table"], kv_lens=lens,
+                                         new_lens=fresh, return_lse=True)
+            c = dict(cache, kv=[max(0, min(128, n)) for n in kv], new=[max(0, min(4, n)) for n in new])
+            want, wlse, off, lse_off = O.attend(q, c)
+            within("out", out, want, off)
+            within("lse", lse, wlse, lse_off)
+            k = rows(gen_of(1), 3, 2, 4, 64, BF)
+            T.cache_append(k, k, cache["k"], cache["v"], page_table=cache["table"], kv_lens=lens, new_lens=fresh)
+            b = torch.zeros(cache["k"].shape[0], 2, 2, 64, dtype=BF, device="cuda")
+            sel = T.cache_select(q, b, page_table=cache["table"], kv_lens=lens, new_lens=fresh, page_size=64, count=2)
+            assert torch.equal(sel, O.select(q, b, c, 2))
+            T.cache_read(cache["k"], cache["v"], page_table=cache["table"], kv_lens=lens, seqlen=200, dtype=BF)
+    torch.cuda.synchronize()
+
+
+def test_library_checks(T):
+    """Schemas and fake implementations agree with what the operators do."""
+    checks = ("test_schema", "test_faketensor")
+    ops = torch.ops.shaobo_fa3
+    for bits in (16, 4):
+        s = step_state(T, bits, 2)
+        w = (s["table"], s["lens"])
+        for op, args in (
+                ("cache_append", (s["k"], s["v"], s["kp"], s["vp"], *w, None, s["q"], None, s["fr"], False, s["bounds"])),
+                ("cache_append", (s["k"], s["v"], s["kp"], s["vp"], *w)),
+                ("cache_attn", (s["q"], s["kp"], s["vp"], *w)),
+                ("cache_select", (s["q"], s["bounds"], *w, 64, 3)),
+                ("cache_read", (s["kp"], s["vp"], *w, 100, BF))):
+            torch.library.opcheck(getattr(ops, op).default, args, test_utils=checks)
+
+
+def test_refusals(T):
+    s = step_state(T, 16, 2)
+    ops = torch.ops.shaobo_fa3
+    q, k, v, kp, vp, t, n = (s[x] for x in ("q", "k", "v", "kp", "vp", "table", "lens"))
+    four = T.cache_pages(60, 2, 64, 128, BF, bits=4)[0]
+    a = ops.cache_attn
+    refused("must be \\[batch", lambda: a(q[0], kp, vp, t, n))
+    refused("fp16 or bf16", lambda: a(q.float(), kp, vp, t, n))
+    refused("type", lambda: a(q.half(), kp, vp, t, n))
+    refused("alike", lambda: a(q, kp, vp[:, :, :32], t, n))
+    refused("alike", lambda: a(q, kp, four, t, n))
+    refused("same GPU", lambda: a(q, kp, vp.cpu(), t, n))
+    refused("head_dim 128, rows of 64", lambda: a(q[..., :64], kp, vp, t, n))
+    refused("page_size", lambda: a(q, kp[:, :, :16], vp[:, :, :16], t, n))
+    refused("page_size", lambda: a(q, kp[:, :, :48], vp[:, :, :48], t, n))
+    refused("int32 \\[batch, width\\]", lambda: a(q, kp, vp, t.long(), n))
+    refused("int32 \\[batch, width\\]", lambda: a(q, kp, vp, t.cpu(), n))
+    refused("rows must be contiguous", lambda: a(q, kp, vp, t.t().contiguous().t(), n))
+    refused("batch", lambda: a(q, kp, vp, t[:2], n[:2]))
+    refused("kv_lens", lambda: a(q, kp, vp, t, n.long()))
+    refused("kv_lens", lambda: a(q, kp, vp, t, n[:2]))
+    refused("new_lens", lambda: a(q, kp, vp, t, n, n[:1]))
+    refused("heads", lambda: a(q[:, :3], kp, vp, t, n))
+    refused("16 bytes", lambda: a(q, torch.zeros(60, 2, 64, 132, dtype=BF, device="cuda")[..., :128], vp, t, n))
+    refused("two axes", lambda: a(q, torch.zeros(60, 2, 64, 80, dtype=torch.uint8, device="cuda")[..., :68], four, t, n))
+    refused("64 or 128", lambda: a(q[..., :96], *(torch.zeros(60, 2, 64, 52, dtype=torch.uint8, device="cuda"),) * 2, t, n))
+    refused("needs causal", lambda: a(q, kp, vp, t, n, None, False, None, 0.0, None, n))
+    refused("softcap", lambda: a(q, kp, vp, t, n, None, True, None, -1.0))
+    refused("finite", lambda: a(q, kp, vp, t, n, None, True, math.nan))
+    refused("slopes", lambda: a(q, kp, vp, t, n, None, True, None, 0.0, torch.ones(3, device="cuda")))
+    sel = torch.zeros(3, 2, 2, 4, dtype=torch.int32, device="cuda")
+    refused("selected", lambda: a(q, kp, vp, t, n, None, True, None, 0.0, None, None, sel.long()))
+    refused("selected", lambda: a(q, kp, vp, t, n, None, True, None, 0.0, None, None, sel[:, :1].contiguous()))
+    refused("selected", lambda: a(q, kp, vp, t, n, None, True, None, 0.0, None, None, sel[..., :2]))
+    refused("selected", lambda: a(q, kp, vp, t, n, None, True, None, 0.0, None, None, sel[..., :0]))
+    p = ops.cache_append
+    refused("heads", lambda: p(k[:, :1], v[:, :1], kp, vp, t, n))
+    refused("other rows", lambda: p(k, v[:, :, :1], kp, vp, t, n))
+    refused("other rows", lambda: p(k, v, kp, vp, t, n, None, q[:, :, :1]))
+    refused("several axes", lambda: p(k, v, kp, vp, t, n, None, q, None, T.rotary_freqs([32, 32], device="cuda")))
+    refused("need freqs", lambda: p(k, v, kp, vp, t, n, None, q, torch.zeros(1, 3, 2, device="cuda")))
+    refused("positions", lambda: p(k, v, kp, vp, t, n, None, q, torch.zeros(1, 3, 1, device="cuda"), s["fr"]))
+    refused("positions", lambda: p(k, v, kp, vp, t, n, None, q, torch.zeros(1, 3, 2, device="cuda").short(), s["fr"]))
+    refused("pairs", lambda: p(k, v, kp, vp, t, n, None, q, None, s["fr"][:, :12].contiguous()))
+    refused("bounds", lambda: p(k, v, kp, vp, t, n, bounds=s["bounds"][:-1]))
+    refused("bounds", lambda: p(k, v, kp, vp, t, n, bounds=s["bounds"].half()))
+    c = ops.cache_select
+    refused("count", lambda: c(q, s["bounds"], t, n, 64, 0))
+    refused("page_size", lambda: c(q, s["bounds"], t, n, 100, 3))
+    refused("bounds", lambda: c(q, s["bounds"].float(), t, n, 64, 3))
+    refused("heads", lambda: c(q[:, :3], s["bounds"], t, n, 64, 3))
+    r = ops.cache_read
+    refused("fp16 or bf16", lambda: r(kp, vp, t, n, 10, torch.float32))
+    refused("type", lambda: r(kp, vp, t, n, 10, HF))
+    refused("seqlen", lambda: r(kp, vp, t, n, -1, BF))
+    refused("seqlen", lambda: r(kp, vp, t, n, 1 << 25, BF))
+    # (under grad mode: no gradient)
+    refused("no gradient", lambda: T.cache_attention(q.clone().requires_grad_(), kp, vp, page_table=t, kv_lens=n))
+    refused("no gradient", lambda: T.cache_append(k.clone().requires_grad_(), v, kp, vp, page_table=t, kv_lens=n))
+    with torch.no_grad():
+        T.cache_attention(q.clone().requires_grad_(), kp, vp, page_table=t, kv_lens=n)
+    torch.cuda.synchronize()

@@ -21,6 +21,14 @@ struct FwdCfg {
     static constexpr int kKs = D / 32, kDB = D / 16;
 };
 
+// The rest of 8 values that their bf16 parts leave.
+__device__ __forceinline__ f16x8 pack8_rest(const float* x, const f16x8& hi) {
+    float y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = x[i] - (float)__builtin_bit_cast(__bf16, (_Float16)hi[i]);
+    return pack8<true>(y);
+}
+
 // A wave's 32 rows: what they see, and their running softmax and output.
 //
 // The vector units bound the tile loop, so an element's score stays as it
@@ -41,7 +49,8 @@ struct FwdCfg {
 // V's in bf16, and step() takes the rows' scales; a score is scaled and then
 // masked, where others are masked in their product's seed (a scale of zero
 // would make a NaN of it), and P is scaled before it is rounded, to bf16, whose
-// range holds any scale.
+// range holds any scale; for fp16 rows to two bf16 terms, 16 bits of it, and
+// two products.
 template <int D, bool kBf16, bool kCap, bool kBias, typename Args_ = AttnFwdArgs, bool kFour = false>
 struct FwdRows {
     typedef Args_ Args;
@@ -265,7 +274,7 @@ struct FwdRows {
         for (int n = 0; n < 2; ++n) be[n] -= mx[n] == kNegInf ? 0.f : mx[n];
 #pragma unroll
         for (int r = 0; r < M / 2; ++r) {
-            f16x8 bp[2];
+            f16x8 bp[2], rest[2];
             f32x4 vs[2];
             if constexpr (kFour) {
                 const FA3_LDS f32x4* x =
@@ -283,8 +292,13 @@ struct FwdRows {
                     if constexpr (kFour) p[j] *= vs[j >> 2][j & 3];
                 }
                 bp[n] = pack8<kBf16 || kFour>(p);
+                if constexpr (kFour && !kBf16) rest[n] = pack8_rest(p, bp[n]);
             }
-            reg_grads<D, kBf16 || kFour, false>(rd, tv, tv, m0 / 2 + r, bp, bp, o, o);
+            // (two terms: fewer operands on their way, for their registers)
+            typedef typename std::conditional<kFour && !kBf16, AttnAhead<D, true>, RegCfg<D>>::type Ahead;
+            reg_grads<D, kBf16 || kFour, false, Ahead>(rd, tv, tv, m0 / 2 + r, bp, bp, o, o);
+            if constexpr (kFour && !kBf16)
+                reg_grads<D, true, false, Ahead>(rd, tv, tv, m0 / 2 + r, rest, rest, o, o);
         }
     }
 

@@ -14,7 +14,7 @@
 //       makes two levels of;
 //   4 bits: the scales of those rows, K's and V's.  Levels are exact, the
 //       scale of K meets the fp32 score, that of V meets P before its rounding
-//       to bf16.
+//       to bf16 (fp16 rows: to two bf16 terms, FwdRows).
 // Two blocks' loads are out at a time; there is no barrier before the waves meet.
 #pragma once
 
@@ -303,7 +303,7 @@ __global__ __launch_bounds__(kRegThreads, few_waves(D, kFour, kBlocks)) void cac
                 for (int i = 0; i < kDB; ++i) o[i][q] *= y;
             }
         }
-        f16x8 bp[kBlocks];
+        f16x8 bp[kBlocks], rest[kBlocks];
 #pragma unroll
         for (int q = 0; q < kBlocks; ++q) {
             const float m = mx[q] == kNegInf ? 0.f : mx[q];
@@ -315,10 +315,14 @@ __global__ __launch_bounds__(kRegThreads, few_waves(D, kFour, kBlocks)) void cac
                 if constexpr (kFour) p[j] *= f.vs[j >> 2][j & 3];
             }
             bp[q] = pack8<kBf16 || kFour>(p);
+            if constexpr (kFour && !kBf16) rest[q] = pack8_rest(p, bp[q]);
         }
         f.values([&](int i, f16x8 x) {
 #pragma unroll
-            for (int q = 0; q < kBlocks; ++q) o[i][q] = mfma_16x16x32<kBf16 || kFour>(x, bp[q], o[i][q]);
+            for (int q = 0; q < kBlocks; ++q) {
+                o[i][q] = mfma_16x16x32<kBf16 || kFour>(x, bp[q], o[i][q]);
+                if constexpr (kFour && !kBf16) o[i][q] = mfma_16x16x32<true>(x, rest[q], o[i][q]);
+            }
         });
     };
     for (int x = 0; x < n; x += 2) {

@@ -103,7 +103,8 @@ int shaobo_fa3_cache_append(const ShaoboFa3CacheAppendParams* params, void* stre
  *
  * 4 bits: scores are of what the codes stand for, in fp32 (levels are exact in
  * 16 bits, the scale is applied to the product); P times a value's scale is
- * rounded to bf16 for its product with the levels. */
+ * rounded for its product with the levels, to bf16, or to 16 bits (two bf16
+ * terms) in fp16. */
 typedef struct ShaoboFa3CacheAttnParams {
     uint32_t struct_size;
     int32_t seqlen;

@@ -101,8 +101,10 @@ def attend(q, cache, causal=True, scale=None, softcap=0.0, slopes=None, prefix=N
     G = Hq // Hkv
     scale = D ** -0.5 if scale is None else scale
     u, dev = torch.finfo(q.dtype).eps / 2, q.device
-    # (4 bits: P times a value's scale in bf16)
-    up = u if cache["bits"] == 16 else torch.finfo(torch.bfloat16).eps / 2
+    # (4 bits in fp16: P times a value's scale as two bf16 terms, the second off
+    # by half a step of what the first leaves, 2^-8 of 2^-8; below 2^-126 it is
+    # flushed, and with it nothing of fp16's size)
+    up = u if cache["bits"] == 16 or q.dtype == torch.bfloat16 else (torch.finfo(torch.bfloat16).eps / 2) ** 2
     out = torch.zeros(B, Hq, S, D, dtype=torch.float64, device=dev)
     lse = torch.full((B, Hq, S), -math.inf, dtype=torch.float64, device=dev)
     out_off, lse_off = torch.zeros_like(out), torch.zeros_like(lse)

@@ -29,6 +29,29 @@ __device__ __forceinline__ f16x8 pack8_rest(const float* x, const f16x8& hi) {
     return pack8<true>(y);
 }
 
+// g[db][n] += X^T (B + C) over the 32 streamed rows 32 r .., bf16: reg_grads
+// with two terms for an operand.
+template <int D>
+__device__ __forceinline__ void two_terms(const RegReader<D>& rd, const FA3_LDS char* x, int r,
+                                          const f16x8 (&b)[2], const f16x8 (&c)[2],
+                                          f32x4 (&g)[D / 16][2]) {
+    constexpr int kN = D / 16, kA = 2;
+    f16x8 f[kN];
+#pragma unroll
+    for (int i = 0; i < kA; ++i) f[i] = rd.tr(x, r, i);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+        wall();
+        if (i + kA < kN) f[i + kA] = rd.tr(x, r, i + kA);
+        wall();
+#pragma unroll
+        for (int n = 0; n < 2; ++n) g[i][n] = mfma_16x16x32<true>(f[i], b[n], g[i][n]);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) g[i][n] = mfma_16x16x32<true>(f[i], c[n], g[i][n]);
+    }
+    wall();
+}
+
 // A wave's 32 rows: what they see, and their running softmax and output.
 //
 // The vector units bound the tile loop, so an element's score stays as it
@@ -294,11 +317,8 @@ struct FwdRows {
                 bp[n] = pack8<kBf16 || kFour>(p);
                 if constexpr (kFour && !kBf16) rest[n] = pack8_rest(p, bp[n]);
             }
-            // (two terms: fewer operands on their way, for their registers)
-            typedef typename std::conditional<kFour && !kBf16, AttnAhead<D, true>, RegCfg<D>>::type Ahead;
-            reg_grads<D, kBf16 || kFour, false, Ahead>(rd, tv, tv, m0 / 2 + r, bp, bp, o, o);
-            if constexpr (kFour && !kBf16)
-                reg_grads<D, true, false, Ahead>(rd, tv, tv, m0 / 2 + r, rest, rest, o, o);
+            if constexpr (kFour && !kBf16) two_terms<D>(rd, tv, m0 / 2 + r, bp, rest, o);
+            else reg_grads<D, kBf16, false>(rd, tv, tv, m0 / 2 + r, bp, bp, o, o);
         }
     }
 

@@ -125,6 +125,15 @@ __global__ __launch_bounds__(kRegThreads, D == 64 ? 3 : 2) void attn_fwd_kernel(
 // Bound by reading the cache: 5.4 TB/s for 16 caches of 8192 keys (Hkv 8, D
 // 128, 99 us, the rate of a large copy), 4.9 where they are filled to
 // different lengths (64-69 us).
+template <int D>
+struct TokenCfg {
+    static constexpr int kBlock = 32 * D * 2;   // 32 rows of K or V
+    static constexpr int kStage = 2 * kBlock;
+    static constexpr int kBytes = kRegWaves * 2 * kStage;
+    static constexpr int kLd = kBlock / 1024;   // loads per wave, block and tensor
+    static_assert(2048 + 3 * (D / 16 * 2048 + 512) <= kBytes, "the meeting fits the stages");
+};
+
 template <int D, bool kBf16, bool kCap, bool kBias>
 __global__ __launch_bounds__(kRegThreads, D == 64 ? 2 : 1) void attn_token_kernel(AttnFwdArgs) {
     typedef AttnFwdArgs Args;

@@ -465,16 +465,6 @@ __device__ __forceinline__ FwdJob fwd_job(const A& a, int id) {
     return j;
 }
 
-// LDS of the kernels for few rows: two stages of 32 keys a wave.
-template <int D>
-struct TokenCfg {
-    static constexpr int kBlock = 32 * D * 2;   // 32 rows of K or V
-    static constexpr int kStage = 2 * kBlock;
-    static constexpr int kBytes = kRegWaves * 2 * kStage;
-    static constexpr int kLd = kBlock / 1024;   // loads per wave, block and tensor
-    static_assert(2048 + 3 * (D / 16 * 2048 + 512) <= kBytes, "the meeting fits the stages");
-};
-
 // Joins the parts of a split key axis: with w_s = exp2(l_s - max l), out =
 // sum w_s o_s / sum w_s.  D / 8 lanes hold a row, 8 columns each.  kWays
 // groups of them take every kWays-th part of it, whose sums meet at the end:

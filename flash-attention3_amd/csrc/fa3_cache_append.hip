@@ -15,6 +15,14 @@
 // and a level's border by a few of their bits, so an fp32 turn's last bits
 // would now and then decide a level.  (A double becomes 16 bits by way of fp32,
 // as a cast does.)
+//
+// Bound by HBM where there is much to move: 8192 tokens of 32 + 8 heads of 128
+// channels 46 us, 4.4 TB/s; the fp64 work shows in 4 bits with bounds, where
+// each head's run forms its own angles (2 x 2048 such tokens: 29 us, their bytes
+// 17).  One token 4.4 us in the kernel, 2 of them its angles.
+//
+// read: a thread per 8 channels; 2 x 4096 places of 8 heads from 4 bits 10 us,
+// 4.3 TB/s.
 #include "fa3_cache_device.h"
 #include "fa3_rotary_angle.h"
 
@@ -536,7 +544,9 @@ AppendGrid append_grid(const ShaoboFa3CacheAppendParams& p) {
     // A token's cosines are formed by every workgroup that turns some of its
     // heads, at a cost of about 8 of them: as many heads each as leave a
     // thousand workgroups to q (k and v: 512), and no fewer than its groups take
-    // at once.
+    // at once.  (8192 tokens of 32 + 8 heads 43.9 us, with half as many
+    // workgroups 42.6, with twice as many 51.5; 2 x 2048 in 4 bits and read back
+    // 38.2, 39.5, 43.6.)
     const int at_once = side / run;
     auto share = [&](int heads, int runs, int want) {
         int64_t x = (int64_t)heads * c.batch * runs / want;

@@ -16,6 +16,12 @@
 //       scale of K meets the fp32 score, that of V meets P before its rounding
 //       to bf16 (fp16 rows: to two bf16 terms, FwdRows).
 // Two blocks' loads are out at a time; there is no barrier before the waves meet.
+//
+// Bound by HBM: 16 sequences of up to 8192 in 16 bits 65 us, 5.0 TB/s; 48 of up
+// to 16384 in 4 bits 113 us, 4.8 TB/s (the codes make 44 % of the SIMDs' cycles
+// vector instructions, matrix ones 14 %).  Where few keys are left to a wave,
+// its chain of loads, products and exponentials: 8 x 5 tokens over 6001 in 4
+// bits 16 us, one token over 129 5.5.
 #pragma once
 
 #include "fa3_cache_attn_kernel.h"

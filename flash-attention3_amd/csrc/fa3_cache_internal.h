@@ -64,7 +64,6 @@ constexpr int few_waves(int D, bool four, int blocks) {
     return (D == 64 ? 5 : four ? 4 : 3) - blocks;
 }
 
-// Pages that one workgroup of the scoring kernel takes, and its plan.
 struct CacheSelectPlan {
     int chunks;  // parts of a sequence's pages, scored by a workgroup each
     size_t total;

@@ -8,14 +8,16 @@
 // A wave has sixteen pages of bounds on their way; q's parts wait in LDS as
 // doubles.  The sixteen sums of a lane's four pages and heads meet in steps that
 // halve them, so that a lane ends with one (105 operations, 192 for a sum of
-// each over all lanes).
+// each over all lanes).  16 sequences of 512 pages, 8 KV heads: 12 us, 23 MB of
+// bounds; 2048 pages of one sequence 5.7, latency.
 //
 // cache_pick_kernel: one workgroup per token and KV head finds the key of the
 // last page that is taken, by histograms of 1024 equal ranges between the
 // smallest and the largest key in question (one, as a rule, leaves a few keys,
 // which one wave ranks), and writes the pages at and above it in their order.  A
 // thread has neighbouring pages, in registers unless there are more than
-// 4096.
+// 4096.  48 of 512 pages, 128 rows: 5.8 us; 64 of 2048, 8 rows: 6.5; the chain
+// of its steps, whose barriers wait for one workgroup's eight waves.
 #include "fa3_cache_device.h"
 
 namespace fa3 {

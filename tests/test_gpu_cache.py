@@ -329,7 +329,7 @@ def test_codes_at_the_levels_borders(T, dtype):
         assert torch.equal(scale[0, 0, :16].nan_to_num(nan=-1.0), s[0, 0].nan_to_num(nan=-1.0))
         assert (scale[0, 0, 16:] == 0).all() and torch.isnan(scale[0, 0, 13:15]).all()
     a, b = T.cache_read(k, v, page_table=i32([[0]]), kv_lens=i32([16]), seqlen=16, dtype=dtype)
-    # a level is off by half of the widest gap (2 of 6), a twelfth... of 2 / 6 / 2 of the largest
+    # (the widest gap between levels is 2 of 6, a value off by half of it: a sixth of the largest)
     top = x.double().abs().amax(-1, keepdim=True)
     fine = torch.isfinite(top[..., 0])
     assert ((a.double() - x.double()).abs()[fine] <= (top / 6 * 1.001 + 2.0 ** -24)[fine]).all()

@@ -21,6 +21,23 @@ int few_splits(int64_t jobs, int fill, int64_t keys) {
     return (int)best;
 }
 
+// Slots of a KV head for parts of several sequences, dealt on the GPU by their
+// lengths (cache_deal); 0: every sequence in as many parts (few_splits), which
+// costs a launch less where those are one.  As many slots as fill the chip, and
+// half as many at least beyond one a sequence: a part is then no longer than
+// twice what an even share would be.  16 bits, 8 KV heads, D 128: 32768 keys
+// beside 63 times 512 54 us, whole sequences 359; 4 of 32768 beside 124 of 1024
+// 206 and 518; 16 of up to 8192 70.4, in four parts each 71.9; but 64 of 512 under
+// a table of 32768 27.8 and 24.9, hence not where no sequence can be long.  As
+// many slots again as fill the chip: 64 of 4096 to 32768 896 for 950, 64 of
+// 2048 118 for 109.
+int few_slots(const CacheProblem& p, int64_t jobs, int fill) {
+    if (p.batch < 2 || p.batch > kDealBatch || p.sk < 512) return 0;
+    if ((int64_t)p.batch * (p.sk / 32) >= (1ll << 31) || (jobs >= fill && p.sk < 8192)) return 0;
+    const int per = fill / p.heads_kv, half = per > 2 ? per / 2 : 1;
+    return per > p.batch + half ? per : p.batch + half;
+}
+
 // Rows and parts for jobs of many rows, by an estimate of the launch, us: a
 // 64-key step of a job of 128 rows (64) takes 1.96 (1.42) where the CU has one
 // job and 1.33 (0.86) a job where it has more; parts of a sequence write their
@@ -73,24 +90,29 @@ CachePlan plan_cache_attn(const CacheProblem& p) {
                           : f.token   ? 1
                                       : ceil_div(rows, kAttnRows / f.split);
     const int64_t jobs = groups * tiles;
-    if (f.token && jobs > 0)
-        f.splits = few_splits(jobs, 256 * few_waves(D, p.four, f.row_tile / 16),
-                              p.count > 0 ? (int64_t)p.count * p.page : p.sk);
+    if (f.token && jobs > 0) {
+        const int fill = 256 * few_waves(D, p.four, f.row_tile / 16);
+        f.slots = p.count > 0 ? 0 : few_slots(p, jobs, fill);
+        if (f.slots == 0)
+            f.splits = few_splits(jobs, fill, p.count > 0 ? (int64_t)p.count * p.page : p.sk);
+    }
     size_t at = 0;
     auto take = [&](size_t n) {
         const size_t x = at;
         at += (n + 255) / 256 * 256;
         return x;
     };
-    const int64_t all = jobs * f.splits;
+    const int64_t all = f.slots > 0 ? (int64_t)f.slots * p.heads_kv : jobs * f.splits;
     f.ok = tiles < (1ll << 30) && all < kMaxGrid && groups * rows / 4 < kMaxGrid;
     if (!f.ok) return f;
     f.tiles = (int)tiles;
     f.jobs = (int)all;
-    if (f.splits > 1) {
-        f.po_off = take((size_t)f.splits * groups * rows * D * 4);
-        f.pl_off = take((size_t)f.splits * groups * rows * 4);
+    if (f.splits > 1 || f.slots > 0) {
+        const size_t parts = f.slots > 0 ? (size_t)f.slots * p.heads_kv : (size_t)f.splits * groups;
+        f.po_off = take(parts * rows * D * 4);
+        f.pl_off = take(parts * rows * 4);
     }
+    if (f.slots > 0) f.deal_off = take((size_t)p.batch * 8);
     f.total = at;
     return f;
 }
@@ -142,6 +164,9 @@ hipError_t launch_cache_attn(const CacheProblem& p, const ShaoboFa3CacheAttnPara
     x.x.count = p.count;
     x.x.per_query = f.per_query;
     x.x.div_per_query = make_fastdiv(f.per_query);
+    x.x.slots = f.slots;
+    x.x.batch = p.batch;
+    x.x.deal = (int2*)(ws + f.deal_off);
     if (p.d > 64) p.four ? launch_cache_d128_4(x, p, f, stream) : launch_cache_d128_16(x, p, f, stream);
     else p.four ? launch_cache_d64_4(x, p, f, stream) : launch_cache_d64_16(x, p, f, stream);
     return hipGetLastError();

@@ -47,8 +47,7 @@ struct CacheJob {
     int kv, off, prefix, lim;  // lim: keys that any of its rows sees
 };
 template <typename A>
-__device__ __forceinline__ CacheJob cache_job(const A& a, int id, int row_tile) {
-    const FwdJob f = fwd_job(a, id);
+__device__ __forceinline__ CacheJob cache_job_of(const A& a, const FwdJob& f, int row_tile) {
     CacheJob j;
     j.b = f.b;
     j.hkv = f.hkv;
@@ -73,6 +72,84 @@ __device__ __forceinline__ CacheJob cache_job(const A& a, int id, int row_tile) 
         j.lim = attn_limit(fdiv(a.div_group, last), j.off, j.kv, a.m.causal, j.prefix);
     }
     return j;
+}
+
+template <typename A>
+__device__ __forceinline__ CacheJob cache_job(const A& a, int id, int row_tile) {
+    return cache_job_of(a, fwd_job(a, id), row_tile);
+}
+
+// Parts of the sequences dealt to the slots of a KV head: slot `slot` has part
+// `split` of the `parts` of sequence b, which lie in the slots from first on;
+// each is `part` blocks of 32 keys (deal_part).  b -1: nothing is left for the
+// slot.  All lanes of all waves come to the same; a lane counts for every 64th
+// sequence.
+struct CacheDeal {
+    int b, split, first, parts, part;
+};
+__device__ __forceinline__ uint32_t sum_lanes(uint32_t x) {
+    x += (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x128, 0xF, 0xF, false);  // lane ^ 8
+    x += (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x141, 0xF, 0xF, false);  // ^ 7
+    x += (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0x4E, 0xF, 0xF, false);   // ^ 2
+    x += (uint32_t)__builtin_amdgcn_mov_dpp((int)x, 0xB1, 0xF, 0xF, false);   // ^ 1
+    auto r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    x = r[0] + r[1];
+    r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    return __builtin_amdgcn_readfirstlane(r[0] + r[1]);
+}
+template <typename A>
+__device__ __forceinline__ CacheDeal cache_deal(const A& a, int slot) {
+    constexpr int kChunks = kDealBatch / 64;
+    const int lane = threadIdx.x & 63, B = a.x.batch;
+    const auto& c = a.x.cv;
+    uint32_t n[kChunks], mine[kChunks];
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k) {
+        const int b = 64 * k + lane;
+        n[k] = mine[k] = 0;
+        if (b < B) {
+            const int kv = cache_length(c.kv_lens[b], c.width << c.shift);
+            const int fresh = c.new_lens == nullptr ? a.sq : cache_length(c.new_lens[b], a.sq);
+            n[k] = fresh > 0 ? (kv + 31) >> 5 : 0;
+        }
+    }
+    uint32_t total = 0;
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k) total += n[k];
+    total = sum_lanes(total);
+    auto count = [&](uint32_t part) {
+        uint32_t s = 0;
+#pragma unroll
+        for (int k = 0; k < kChunks; ++k)
+            if (64 * k < B) {
+                mine[k] = 64 * k + lane < B ? max(1u, (n[k] + part - 1) / part) : 0u;
+                s += mine[k];
+            }
+        return sum_lanes(s);
+    };
+    CacheDeal d{-1, 0, 0, 0, (int)(4 * deal_part(total, a.x.slots, B, a.part / 4, count))};
+    count(d.part);
+    int base = 0;
+#pragma unroll
+    for (int k = 0; k < kChunks; ++k) {
+        if (64 * k >= B) continue;
+        int upto = (int)mine[k];
+#pragma unroll
+        for (int o = 1; o < 64; o *= 2) {
+            const int x = __shfl_up(upto, o);
+            if (lane >= o) upto += x;
+        }
+        const uint64_t past = __ballot(slot < base + upto);
+        if (d.b < 0 && past != 0) {
+            const int l = __builtin_ctzll(past);
+            d.b = 64 * k + l;
+            d.parts = __builtin_amdgcn_readlane((int)mine[k], l);
+            d.first = base + __builtin_amdgcn_readlane(upto, l) - d.parts;
+            d.split = slot - d.first;
+        }
+        base += __builtin_amdgcn_readlane(upto, 63);
+    }
+    return d;
 }
 
 // Blocks of 32 keys that a job of few rows walks: [begin, end) of a sequence's

@@ -28,6 +28,11 @@ void launch_cache(const CacheAttnArgs& x, const CacheProblem& p, const CachePlan
     using F = std::false_type;
     if (p.softcap > 0.f) p.bias ? kinds(T{}, T{}) : kinds(T{}, F{});
     else p.bias ? kinds(F{}, T{}) : kinds(F{}, F{});
+    if (f.slots > 0) {
+        hipLaunchKernelGGL((cache_join_kernel<D, kBf16>), dim3(ceil_div((int64_t)x.groups * x.rows, 4)),
+                           dim3(256), 0, stream, x);
+        return;
+    }
     if (f.splits <= 1) return;
     auto join = [&](auto ways) {
         constexpr int kW = decltype(ways)::value;

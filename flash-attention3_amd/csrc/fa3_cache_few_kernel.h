@@ -193,8 +193,30 @@ __global__ __launch_bounds__(kRegThreads, few_waves(D, kFour, kBlocks)) void cac
     FA3_LDS char* smem = (FA3_LDS char*)smem_raw;
     const int lane = threadIdx.x & 63, l16 = lane & 15, g4 = lane >> 4;
     const int w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const CacheJob job = cache_job(a, blockIdx.x, 16 * kBlocks);
-    const CacheSpan span = cache_span(a, job);
+    CacheJob job;
+    CacheSpan span;
+    int slot = 0, parts = a.splits;
+    if (a.x.slots > 0) {
+        slot = fdiv(a.div_hkv, blockIdx.x);
+        const CacheDeal d = cache_deal(a, slot);
+        if (d.b < 0) return;
+        const int hkv = blockIdx.x - slot * a.heads_kv;
+        FwdJob f;
+        f.b = d.b;
+        f.hkv = hkv;
+        f.grp = d.b * a.heads_kv + hkv;
+        f.split = d.split;
+        f.tile = 0;
+        job = cache_job_of(a, f, 16 * kBlocks);
+        const int n = (job.lim + 31) >> 5;
+        span.begin = min(d.split * d.part, n);
+        span.end = min(span.begin + d.part, n);
+        parts = d.parts;
+        if (hkv == 0 && d.split == 0 && threadIdx.x == 0) a.x.deal[d.b] = make_int2(d.first, d.parts);
+    } else {
+        job = cache_job(a, blockIdx.x, 16 * kBlocks);
+        span = cache_span(a, job);
+    }
     const int first = span.begin + w, end = span.end;
     const int n = end > first ? (end - first + 3) >> 2 : 0;
     const FewPages at{a.x.cv.k + job.hkv * a.x.cv.k_hs, a.x.cv.v + job.hkv * a.x.cv.v_hs,
@@ -404,8 +426,9 @@ __global__ __launch_bounds__(kRegThreads, few_waves(D, kFour, kBlocks)) void cac
         for (int i = 0; i < kDB; ++i) out[i] = none ? 0.f : y[i / 4][i % 4] * inv;
         const int c = kDB * (4 * g4 + w);
         const bool first = g4 == 0 && w == 0;
-        if (z.splits > 1) {
-            const int64_t at = ((int64_t)job.split * z.groups + job.grp) * z.rows + row;
+        if (parts > 1) {
+            const int64_t at = z.x.slots > 0 ? ((int64_t)slot * z.heads_kv + job.hkv) * z.rows + row
+                                             : ((int64_t)job.split * z.groups + job.grp) * z.rows + row;
             if (first) z.part_l[at] = lse2;
 #pragma unroll
             for (int i = 0; i < kDB / 4; ++i) *(f32x4*)(z.part_o + at * D + c + 4 * i) = *(const f32x4*)(out + 4 * i);
@@ -424,6 +447,59 @@ __global__ __launch_bounds__(kRegThreads, few_waves(D, kFour, kBlocks)) void cac
             *(f16x4*)p = x;
         }
     }
+}
+
+// Joins the parts of the sequences that were dealt several, as attn_join_kernel
+// does: a wave has a row, D / 8 lanes of it 8 channels each of every 512 / D-th
+// part.
+template <int D, bool kBf16>
+__global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnArgs a) {
+    constexpr int kLanes = D / 8, kWays = 512 / D;
+    const int lane = threadIdx.x & 63;
+    const int64_t rg = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (rg >= (int64_t)a.groups * a.rows) return;
+    const int grp = (int)(rg / a.rows), r = (int)(rg - (int64_t)grp * a.rows);
+    const int b = fdiv(a.div_hkv, grp), hkv = grp - b * a.heads_kv;
+    const int2 deal = a.x.deal[b];
+    if (deal.y <= 1) return;  // (its only part wrote the outputs)
+    auto at = [&](int s) { return ((int64_t)(deal.x + s) * a.heads_kv + hkv) * a.rows + r; };
+    float top = kNegInf;
+    for (int s = lane; s < deal.y; s += 64) top = __builtin_fmaxf(top, a.part_l[at(s)]);
+#pragma unroll
+    for (int o = 32; o > 0; o >>= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o));
+    const int col = (lane % kLanes) * 8;
+    float z = 0.f, acc[8] = {};
+#pragma unroll 4
+    for (int s = lane / kLanes; s < deal.y; s += kWays) {
+        const float l = a.part_l[at(s)];
+        const float* p = a.part_o + at(s) * D + col;
+        const f32x4 x = *(const f32x4*)p, y = *(const f32x4*)(p + 4);
+        const bool none = l == kNegInf;
+        const float f = none ? 0.f : fast_exp2(l - top);
+        z += f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            acc[e] = __builtin_fmaf(f, none ? 0.f : x[e], acc[e]);
+            acc[4 + e] = __builtin_fmaf(f, none ? 0.f : y[e], acc[4 + e]);
+        }
+    }
+#pragma unroll
+    for (int o = 32; o >= kLanes; o >>= 1) {
+        z += __shfl_xor(z, o);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) acc[e] += __shfl_xor(acc[e], o);
+    }
+    const AttnRow x = attn_row(r, a.rows, hkv, a.group, a.div_group);
+    const bool none = z == 0.f;  // (NaN is not)
+    const float inv = none ? 0.f : 1.f / z;
+    if (lane == 0)
+        a.lse[((int64_t)b * a.heads_q + x.h) * a.sq + x.i] =
+            none ? kNegInf : (top + __builtin_amdgcn_logf(z)) * 0.69314718055994531f;
+    if (lane >= kLanes || col >= a.d) return;
+    f16x8 v;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = to16<kBf16>(acc[e] * inv);
+    *(f16x8*)(a.out.p + b * a.out.bs + x.h * a.out.hs + x.i * a.out.rs + col) = v;
 }
 
 }  // namespace

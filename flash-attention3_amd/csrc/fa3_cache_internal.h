@@ -39,7 +39,30 @@ struct CacheAttnExtra {
     const int* selected;  // [batch * heads_kv][sq][count], or null
     int count, per_query;
     FastDiv div_per_query;
+    // slots > 0: the kernel for few rows deals parts of all sequences to as many
+    // slots of each KV head; deal[b]: the first of sequence b's, and how many
+    int slots, batch;
+    int2* deal;
 };
+constexpr int kDealBatch = 256;  // sequences at most, four a lane
+// The least part, in fours of blocks, for which count(blocks a part), the parts
+// that `batch` sequences of `total` blocks make (an empty one too), are no more
+// than the slots.  With P slots, B sequences and n blocks in all, parts of
+// n / (P - B) blocks are at most n / (n / (P - B)) + B.
+template <typename F>
+__host__ __device__ inline uint32_t deal_part(uint32_t total, uint32_t slots, uint32_t batch, uint32_t least,
+                                              F count) {
+    const uint32_t spare = slots - batch;
+    uint32_t lo = (total + 4 * slots - 1) / (4 * slots), hi = (total + 4 * spare - 1) / (4 * spare);
+    lo = lo < least ? least : lo;
+    hi = hi < lo ? lo : hi;
+    while (lo < hi) {
+        const uint32_t mid = (lo + hi) >> 1;
+        if (count(4 * mid) <= slots) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
 struct CacheAttnArgs : AttnFwdArgs {
     static constexpr bool kPaged = true;
     CacheAttnExtra x;
@@ -52,8 +75,9 @@ struct CachePlan {
     int tiles;    // row tiles of a KV head (selected pages: of all its queries)
     int per_query;  // selected pages: row tiles of one query's heads
     int splits;   // parts of the key axis
+    int slots;    // or, where it is cut by the sequences' lengths: slots of a KV head
     int jobs;
-    size_t po_off, pl_off, total;
+    size_t po_off, pl_off, deal_off, total;
     bool ok;
 };
 CachePlan plan_cache_attn(const CacheProblem& p);

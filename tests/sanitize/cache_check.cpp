@@ -8,6 +8,7 @@
 #include <cstdio>
 #include <cstdlib>
 #include <random>
+#include <vector>
 
 #include "fa3_cache_internal.h"
 
@@ -97,7 +98,7 @@ int main(int argc, char** argv) {
             if (p != (e >= 0 && e < pages ? e : -1)) return fail("page");
             if (n < 0 || n > pages || (e >= 0 && e <= pages && n != e)) return fail("length");
         }
-    int seen[3] = {};
+    int seen[3] = {}, dealt = 0;
     for (int it = 0; it < iters; ++it) {
         const bool plausible = rng() % 4 != 0;
         ShaoboFa3CacheAttnParams a;
@@ -134,6 +135,27 @@ int main(int argc, char** argv) {
             p.causal = a.causal != 0;
             const fa3::CachePlan f = fa3::plan_cache_attn(p);
             if (!f.ok || f.splits < 1) return fail("plan");
+            if (f.slots > 0) {
+                if (f.slots <= p.batch || p.batch > fa3::kDealBatch || f.splits > 1 ||
+                    f.jobs != f.slots * p.heads_kv)
+                    return fail("slots");
+                uint32_t total = 0;
+                std::vector<uint32_t> n(p.batch);
+                const int shape = (int)(rng() % 3);
+                for (uint32_t& x : n) {
+                    const uint32_t most = p.sk / 32 + 1;
+                    x = (uint32_t)(rng() % (shape == 0 || (shape == 1 && rng() % 8 == 0) ? most : most < 16 ? most : 16));
+                    total += x;
+                }
+                auto count = [&](uint32_t part) {
+                    uint32_t s = 0;
+                    for (uint32_t x : n) s += std::max(1u, (x + part - 1) / part);
+                    return s;
+                };
+                const uint32_t part = fa3::deal_part(total, f.slots, p.batch, 2, count);
+                if (part < 2 || count(4 * part) > (uint32_t)f.slots) return fail("a part without a slot");
+                ++dealt;
+            }
             const int64_t rows = (int64_t)p.group * p.sq;
             if (p.count > 0 ? f.tiles < (int64_t)p.sq || f.per_query * f.row_tile < p.group
                             : (int64_t)f.tiles * (f.token ? f.row_tile : 128 / f.split) < rows)
@@ -175,5 +197,5 @@ int main(int argc, char** argv) {
         if (!status_ok(shaobo_fa3_cache_read(&r, nullptr))) return fail("read");
     }
     std::printf("ok %d %d %d\n", seen[0], seen[1], seen[2]);
-    return seen[0] > iters / 20 && seen[1] > 0 && seen[2] > 0 ? 0 : fail("the fuzz is one-sided");
+    return seen[0] > iters / 20 && seen[1] > 0 && seen[2] > 0 && dealt > iters / 500 ? 0 : fail("the fuzz is one-sided");
 }

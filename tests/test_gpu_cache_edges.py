@@ -291,6 +291,23 @@ def test_serving_equals_the_prompt(T, cap):
     within("dense lse", dlse, wlse, lse_off)
 
 
+DEALT = [
+    # (the kernel for few rows cuts several sequences by their lengths)
+    dict(kv=[9000] + [40] * 9, Hq=8), dict(kv=[1, 700, 0, 5000, 33], D=128, Hq=8),
+    dict(kv=[200 + 37 * n for n in range(70)], Hq=4), dict(kv=[0] * 65 + [3000, 1], Hq=4, D=128),
+    dict(kv=[300, 2500, 90], new=[3, 0, 2], S=4, Hq=8, D=128), dict(kv=[5000, 10], S=3, Hq=2, Hkv=1, softcap=9.0, std=3.0),
+    dict(kv=[10] * 255 + [4000]), dict(kv=[4000] + [10] * 256), dict(kv=[600, 4100, 700], S=2, slopes=1, Hq=8, ps=32),
+    dict(kv=[3000, 2900], holes=[0, 5, 20], Hq=4, D=128), dict(kv=[16000] + [100] * 90, Hq=16, Hkv=8, D=128),
+    dict(kv=[2600, 700], D=128, Hq=32, Hkv=1), dict(kv=[400] * 40 + [9000], Hq=32, Hkv=16, D=64, prefix=[500] * 41, S=2),
+]
+
+
+@pytest.mark.parametrize("bits,dtype", [(16, BF), (4, HF)])
+@pytest.mark.parametrize("case", DEALT, ids=lambda c: f"{len(c['kv'])}-{max(c['kv'])}-{c.get('S', 1)}")
+def test_sequences_of_very_different_lengths(T, case, bits, dtype):
+    check_attn(T, *attn_case(case, bits, dtype))
+
+
 def step(T, s):
     """One decoding step of a state: append, select, attend twice."""
     w = dict(page_table=s["table"], kv_lens=s["lens"])

@@ -9,7 +9,8 @@ int64_t ceil64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
 // Parts of the key axis for jobs of few rows: as many as fill the chip once,
 // and then up to twice as many where those leave the CUs less uneven (the most
-// jobs a CU has, by the parts' length).  B16 S8192 in 16 bits, 128 jobs: 86 us
+// jobs a CU has, by the parts' length).  16 sequences of up to 8192 in 16 bits,
+// each in as many parts, 128 jobs: 86 us
 // in 2 parts, 84 in 3, 70 in 4, 82 in 6, 76 in 8; 512 jobs that fill it
 // already, B64 S2048 in 4 bits: 26 whole, 29 in 2.  A part keeps 256 keys.
 int few_splits(int64_t jobs, int fill, int64_t keys) {

@@ -17,8 +17,8 @@
 //       to bf16 (fp16 rows: to two bf16 terms, FwdRows).
 // Two blocks' loads are out at a time; there is no barrier before the waves meet.
 //
-// Bound by HBM: 16 sequences of up to 8192 in 16 bits 65 us, 5.0 TB/s; 48 of up
-// to 16384 in 4 bits 113 us, 4.8 TB/s (the codes make 44 % of the SIMDs' cycles
+// Bound by HBM: 16 sequences of up to 8192 in 16 bits 62.6 us, 5.1 TB/s; 48 of up
+// to 16384 in 4 bits 108.6 us, 5.0 TB/s (the codes make 44 % of the SIMDs' cycles
 // vector instructions, matrix ones 14 %).  Where few keys are left to a wave,
 // its chain of loads, products and exponentials: 8 x 5 tokens over 6001 in 4
 // bits 16 us, one token over 129 5.5.
@@ -451,7 +451,8 @@ __global__ __launch_bounds__(kRegThreads, few_waves(D, kFour, kBlocks)) void cac
 
 // Joins the parts of the sequences that were dealt several, as attn_join_kernel
 // does: a wave has a row, D / 8 lanes of it 8 channels each of every 512 / D-th
-// part.
+// part.  Latency: 4.7 us for 512 rows as for 6144, what the launch of the other
+// join takes.
 template <int D, bool kBf16>
 __global__ __launch_bounds__(256) void cache_join_kernel(CacheAttnArgs a) {
     constexpr int kLanes = D / 8, kWays = 512 / D;

@@ -16,8 +16,12 @@ void launch_cache(const CacheAttnArgs& x, const CacheProblem& p, const CachePlan
     auto kinds = [&](auto cz, auto bi) {
         constexpr bool kC = decltype(cz)::value, kBi = decltype(bi)::value;
         if (f.token) {
-            f.row_tile == 16 ? go(cache_few_kernel<D, kBf16, kC, kBi, kFour, 1>)
-                             : go(cache_few_kernel<D, kBf16, kC, kBi, kFour, 2>);
+            auto few = [&](auto dealt) {
+                constexpr bool kDealt = decltype(dealt)::value;
+                f.row_tile == 16 ? go(cache_few_kernel<D, kBf16, kC, kBi, kFour, 1, kDealt>)
+                                 : go(cache_few_kernel<D, kBf16, kC, kBi, kFour, 2, kDealt>);
+            };
+            f.slots > 0 ? few(std::true_type{}) : few(std::false_type{});
         } else if (f.split == 2) {
             go(cache_tile_kernel<D, kBf16, kC, kBi, kFour, 2>);
         } else {

@@ -221,11 +221,11 @@ def test_kernels_share_a_cu():
     assert bad == []
     few = [k for k in kernels if "cache_few_kernel" in k[".name"]]
     tile = [k for k in kernels if "cache_tile_kernel" in k[".name"]]
-    assert len(few) == 64 and len(tile) == 64 and os.path.exists(gate.LIB_PATH)
+    assert len(few) == 128 and len(tile) == 64 and os.path.exists(gate.LIB_PATH)
     for k in few:
-        # template arguments: D, type, cap, bias, four, 16-row blocks
+        # template arguments: D, type, cap, bias, four, 16-row blocks, dealt
         args = k[".name"].split("cache_few_kernelI")[1].split("EEE")[0]
-        d, four, blocks = 64 if "Li64E" in args else 128, args.split("E")[4] == "Lb1", int(args[-1])
+        d, four, blocks = 64 if "Li64E" in args else 128, args.split("E")[4] == "Lb1", int(args.split("E")[5][2:])
         n = (5 if d == 64 else 4 if four else 3) - blocks
         assert k[".vgpr_count"] <= 512 // n // 8 * 8, k[".name"]
         assert n * k[".group_segment_fixed_size"] <= gate.LDS_BYTES, k[".name"]

@@ -353,7 +353,8 @@ CacheSelectPlan plan_cache_select(const ShaoboFa3CacheSelectParams& p) {
     CacheSelectPlan f{};
     const int64_t rows = (int64_t)p.cache.batch * p.cache.num_heads_kv * p.seqlen;
     f.chunks = ceil_div(p.cache.width, kScorePages);
-    f.ok = rows < kMaxGrid && rows * f.chunks < kMaxGrid;
+    // (kMaxGrid is of workgroups of 256 threads)
+    f.ok = rows * (kPickThreads / 256) < kMaxGrid && rows * f.chunks < kMaxGrid;
     f.total = f.ok ? (size_t)rows * p.cache.width * 8 : 0;
     f.total = (f.total + 255) / 256 * 256;
     return f;

@@ -162,6 +162,23 @@ def test_workspaces(lib):
     assert need("attn", seqlen=1, cache__width=512, selected=PTR, count=8) < n
 
 
+@pytest.mark.parametrize("heads,seqlen,status", [
+    (8, 1 << 20, F.UNSUPPORTED), (1, (1 << 23) + 1, F.UNSUPPORTED), (8, (1 << 20) - 1, F.SUCCESS),
+    (1, (1 << 23) - 1, F.SUCCESS), (1 << 16, 128, F.UNSUPPORTED), (1 << 16, 127, F.SUCCESS),
+])
+@pytest.mark.parametrize("width", [0, 1, 64])
+def test_selection_of_more_rows_than_a_launch_takes(lib, heads, seqlen, status, width):
+    """Picking has a workgroup of 512 threads for every token and KV head, and a launch
+    fewer than 2^32 threads: refused at 2^23 rows, before anything is launched."""
+    p = make(lib, "select", cache__batch=1, cache__num_heads_kv=heads, num_heads_q=heads, seqlen=seqlen,
+             cache__width=width)
+    assert lib.shaobo_fa3_cache_select_validate(ctypes.byref(p)) == status
+    n = lib.shaobo_fa3_cache_select_workspace_bytes(ctypes.byref(p))
+    assert n == (-(-heads * seqlen * width * 8 // 256) * 256 if status == F.SUCCESS else 0)
+    if status != F.SUCCESS:
+        assert call(lib, "select", p) == status
+
+
 # ---------------------------------------------------------------------------
 @pytest.fixture(scope="module")
 def T():

@@ -4,6 +4,11 @@
 #include "fa3_torch_common.h"
 #include "shaobo_fa3_cache.h"
 
+#include <ATen/core/grad_mode.h>
+#include <c10/core/AutogradState.h>
+
+#include <initializer_list>
+
 namespace {
 
 int32_t dtype_of(at::ScalarType t) {
@@ -12,6 +17,16 @@ int32_t dtype_of(at::ScalarType t) {
 
 void check_type(at::ScalarType t, const char* name) {
     TORCH_CHECK_VALUE(t == at::kHalf || t == at::kBFloat16, name, " must be fp16 or bf16");
+}
+
+// No operator here has a gradient: a call that would leave one out is refused.
+void no_gradient(std::initializer_list<optional<Tensor>> tensors) {
+    const bool backward = at::GradMode::is_enabled();
+    const bool forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
+    for (const optional<Tensor>& t : tensors)
+        TORCH_CHECK_VALUE(!t.has_value() || !((backward && t->requires_grad()) ||
+                                              (forward && t->_fw_grad(0).defined())),
+                          "the cache's operators have no gradient: pass detached tensors");
 }
 
 // [B] lengths
@@ -115,6 +130,7 @@ std::vector<Tensor> cache_append(const Tensor& k, const Tensor& v, Tensor k_page
                                  const optional<Tensor>& new_lens, const optional<Tensor>& q,
                                  const optional<Tensor>& positions, const optional<Tensor>& freqs,
                                  bool interleaved, const optional<Tensor>& bounds) {
+    no_gradient({k, v, k_pages, v_pages, q, positions, freqs, bounds});
     TORCH_CHECK_VALUE(k.dim() == 4, "k must be [batch, heads, sequence, head_dim]");
     check_type(k.scalar_type(), "k");
     ShaoboFa3CacheAppendParams p;
@@ -189,6 +205,7 @@ std::tuple<Tensor, Tensor> cache_attn(const Tensor& q, const Tensor& k_pages, co
                                       const optional<Tensor>& slopes,
                                       const optional<Tensor>& prefix_lens,
                                       const optional<Tensor>& selected) {
+    no_gradient({q, k_pages, v_pages, slopes});
     TORCH_CHECK_VALUE(q.dim() == 4, "q must be [batch, heads, sequence, head_dim]");
     check_type(q.scalar_type(), "q");
     ShaoboFa3CacheAttnParams p;
@@ -242,6 +259,7 @@ std::tuple<Tensor, Tensor> cache_attn(const Tensor& q, const Tensor& k_pages, co
 Tensor cache_select(const Tensor& q, const Tensor& bounds, const Tensor& page_table,
                     const Tensor& kv_lens, int64_t page_size, int64_t count,
                     const optional<Tensor>& new_lens) {
+    no_gradient({q, bounds});
     TORCH_CHECK_VALUE(q.dim() == 4 && q.is_cuda(), "q must be [batch, heads, sequence, head_dim] on a GPU");
     check_type(q.scalar_type(), "q");
     TORCH_CHECK_VALUE(bounds.dim() == 4, "bounds must be [pages, heads_kv, 2, head_dim]");
@@ -292,6 +310,7 @@ Tensor cache_select(const Tensor& q, const Tensor& bounds, const Tensor& page_ta
 std::tuple<Tensor, Tensor> cache_read(const Tensor& k_pages, const Tensor& v_pages,
                                       const Tensor& page_table, const Tensor& kv_lens, int64_t seqlen,
                                       at::ScalarType dtype) {
+    no_gradient({k_pages, v_pages});
     check_type(dtype, "dtype");
     ShaoboFa3CacheReadParams p;
     shaobo_fa3_cache_read_params_init(&p);

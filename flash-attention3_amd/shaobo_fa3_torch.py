@@ -447,7 +447,7 @@ def cache_append(k, v, k_pages, v_pages, *, page_table, kv_lens, new_lens=None, 
     bounds       follow the keys written, for cache_select
 
     Written pages must belong to one sequence each."""
-    _no_gradient(k, v, q)
+    _no_gradient(k, v, k_pages, v_pages, q, positions, freqs, bounds)
     out = torch.ops.shaobo_fa3.cache_append(k, v, k_pages, v_pages, page_table, kv_lens, new_lens, q,
                                             positions, freqs, interleaved, bounds)
     return out[0] if out else None
@@ -465,7 +465,7 @@ def cache_attention(q, k_pages, v_pages, *, page_table, kv_lens, new_lens=None, 
 
     Padding rows give zeros, and -inf in the log-sum-exp that return_lse=True
     also returns (fp32 [B, Hq, S])."""
-    _no_gradient(q, slopes)
+    _no_gradient(q, k_pages, v_pages, slopes)
     out, lse = torch.ops.shaobo_fa3.cache_attn(q, k_pages, v_pages, page_table, kv_lens, new_lens,
                                                causal, softmax_scale, softcap, slopes, prefix_lens,
                                                selected)
@@ -478,7 +478,7 @@ def cache_select(q, bounds, *, page_table, kv_lens, page_size, count, new_lens=N
     those before it the ones whose bounds allow the largest score of any head of
     the group (for a positive softmax scale).  bounds as cache_append keeps them
     (q turned as it returns it)."""
-    _no_gradient(q)
+    _no_gradient(q, bounds)
     return torch.ops.shaobo_fa3.cache_select(q, bounds, page_table, kv_lens, page_size, count,
                                              new_lens)
 
@@ -487,5 +487,5 @@ def cache_read(k_pages, v_pages, *, page_table, kv_lens, seqlen, dtype=torch.bfl
     """k and v [B, Hkv, seqlen, D] in dtype: the first seqlen places of every
     sequence as the cache holds them, zeros at and behind kv_lens and where
     there is no page."""
-    _no_gradient()
+    _no_gradient(k_pages, v_pages)
     return torch.ops.shaobo_fa3.cache_read(k_pages, v_pages, page_table, kv_lens, seqlen, dtype)

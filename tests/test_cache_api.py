@@ -221,6 +221,36 @@ def test_refusals_without_a_gpu(T):
         T.cache_pages(1, 1, 32, 64, bits=8, device="cpu")
 
 
+def test_no_tensor_of_a_call_loses_its_gradient(T):
+    """Whichever tensor requires one, the call is refused (under no_grad it goes on, to
+    an operator that has no CPU kernel)."""
+    def tensors():
+        x = {n: torch.zeros(1, 1, 32, 64, dtype=torch.bfloat16) for n in ("q", "k", "v", "k_pages", "v_pages")}
+        x["bounds"] = torch.zeros(1, 1, 2, 64, dtype=torch.bfloat16)
+        x["slopes"], x["freqs"], x["positions"] = torch.zeros(1), torch.zeros(1, 8), torch.zeros(1, 1, 32)
+        return x
+
+    t = torch.zeros(1, 1, dtype=torch.int32)
+    w = dict(page_table=t, kv_lens=t[0])
+    calls = {
+        T.cache_append: lambda x: T.cache_append(x["k"], x["v"], x["k_pages"], x["v_pages"], q=x["q"], freqs=x["freqs"],
+                                                 positions=x["positions"], bounds=x["bounds"], **w),
+        T.cache_attention: lambda x: T.cache_attention(x["q"], x["k_pages"], x["v_pages"], slopes=x["slopes"], **w),
+        T.cache_select: lambda x: T.cache_select(x["q"], x["bounds"], page_size=32, count=1, **w),
+        T.cache_read: lambda x: T.cache_read(x["k_pages"], x["v_pages"], seqlen=1, **w),
+    }
+    takes = {T.cache_append: "k v k_pages v_pages q freqs positions bounds", T.cache_attention: "q k_pages v_pages slopes",
+             T.cache_select: "q bounds", T.cache_read: "k_pages v_pages"}
+    for f, call_ in calls.items():
+        for name in takes[f].split():
+            x = tensors()
+            x[name].requires_grad_()
+            with pytest.raises(ValueError, match="no gradient"):
+                call_(x)
+            with torch.no_grad(), pytest.raises(NotImplementedError):
+                call_(x)
+
+
 def test_a_missing_library_is_said(T, monkeypatch):
     monkeypatch.setattr(T, "_ATTN", False)
     q = torch.zeros(1, 1, 4, 64, dtype=torch.bfloat16)

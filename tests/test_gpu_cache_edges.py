@@ -521,3 +521,37 @@ def test_refusals(T):
     with torch.no_grad():
         T.cache_attention(q.clone().requires_grad_(), kp, vp, page_table=t, kv_lens=n)
     torch.cuda.synchronize()
+
+
+def test_no_gradient_is_dropped(T):
+    """Whichever tensor requires a gradient or has a tangent, functions and operators
+    refuse the call; under no_grad, and for tensors without, they run."""
+    import torch.autograd.forward_ad as fw
+    s = step_state(T, 16, 2)
+    x = dict(s, slopes=torch.rand(8, device="cuda"), pos=torch.zeros(1, 3, 2, device="cuda"))
+    ops, w = torch.ops.shaobo_fa3, (s["table"], s["lens"])
+    names = dict(page_table=s["table"], kv_lens=s["lens"])
+    calls = [
+        ("k v kp vp q pos fr bounds", lambda y: ops.cache_append(y["k"], y["v"], y["kp"], y["vp"], *w, None, y["q"], y["pos"],
+                                                                 y["fr"], False, y["bounds"])),
+        ("k v kp vp q pos fr bounds", lambda y: T.cache_append(y["k"], y["v"], y["kp"], y["vp"], q=y["q"], positions=y["pos"],
+                                                               freqs=y["fr"], bounds=y["bounds"], **names)),
+        ("q kp vp slopes", lambda y: ops.cache_attn(y["q"], y["kp"], y["vp"], *w, None, True, None, 0.0, y["slopes"])),
+        ("q kp vp slopes", lambda y: T.cache_attention(y["q"], y["kp"], y["vp"], slopes=y["slopes"], **names)),
+        ("q bounds", lambda y: ops.cache_select(y["q"], y["bounds"], *w, 64, 3)),
+        ("q bounds", lambda y: T.cache_select(y["q"], y["bounds"], page_size=64, count=3, **names)),
+        ("kp vp", lambda y: ops.cache_read(y["kp"], y["vp"], *w, 10, BF)),
+        ("kp vp", lambda y: T.cache_read(y["kp"], y["vp"], seqlen=10, **names)),
+    ]
+    for takes, call in calls:
+        call(x)
+        for name in takes.split():
+            y = dict(x)
+            y[name] = x[name].clone().requires_grad_()
+            refused("no gradient", lambda: call(y))
+            with torch.no_grad():
+                call(y)
+            with fw.dual_level():
+                y[name] = fw.make_dual(x[name].clone(), torch.ones_like(x[name]))
+                refused("no gradient", lambda: call(y))
+    torch.cuda.synchronize()

@@ -29,6 +29,12 @@ void no_gradient(std::initializer_list<optional<Tensor>> tensors) {
                           "the cache's operators have no gradient: pass detached tensors");
 }
 
+// Counts a write as autograd does, so that a backward that saved t misses its
+// values.  (Tensors made under inference mode have no counter.)
+void written(const Tensor& t) {
+    if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+
 // [B] lengths
 const int32_t* lens_of(const Tensor& t, int64_t B, const Tensor& like, const char* name) {
     check_int32(t, {B}, like, name);
@@ -195,6 +201,9 @@ std::vector<Tensor> cache_append(const Tensor& k, const Tensor& v, Tensor k_page
         p.q_out = view(out[0], "q's output");
     }
     check_status(shaobo_fa3_cache_append(&p, stream_of(k)), "shaobo_fa3_cache_append");
+    written(k_pages);
+    written(v_pages);
+    if (bounds.has_value()) written(*bounds);
     return out;
 }
 

@@ -555,3 +555,22 @@ def test_no_gradient_is_dropped(T):
                 y[name] = fw.make_dual(x[name].clone(), torch.ones_like(x[name]))
                 refused("no gradient", lambda: call(y))
     torch.cuda.synchronize()
+
+
+def test_appends_count_as_writes(T):
+    """Autograd's version counters of what an append writes: a value that a backward
+    has yet to read is missed.  Tensors without counters are written too."""
+    s = step_state(T, 16, 2)
+    w = dict(page_table=s["table"], kv_lens=s["lens"])
+    x = torch.ones((), device="cuda", requires_grad=True)
+    y = (s["kp"].float().sum() + (s["vp"] * x).float().sum())  # (x's gradient needs the values)
+    before = [s[n]._version for n in ("kp", "vp", "bounds")]
+    T.cache_append(s["k"], s["v"], s["kp"], s["vp"], bounds=s["bounds"], **w)
+    assert all(s[n]._version > v for n, v in zip(("kp", "vp", "bounds"), before))
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.backward()
+    with torch.inference_mode():
+        kp, vp, bounds = T.cache_pages(60, 2, 64, 128, BF, bounds=True)
+        T.cache_append(s["k"], s["v"], kp, vp, bounds=bounds, **w)
+        assert kp.abs().sum() > 0 and bounds.abs().sum() > 0
+    torch.cuda.synchronize()

@@ -1,6 +1,6 @@
-// PyTorch operators of the paged cache: shaobo_fa3::cache_append, ::cache_attn,
-// ::cache_select and ::cache_read (shaobo_fa3_torch.py adds their fake
-// implementations).  Built into the attention layer's library.
+// PyTorch operators of the paged cache: shaobo_fa3::cache_append (and
+// ::cache_append_into), ::cache_attn, ::cache_select and ::cache_read
+// (shaobo_fa3_torch.py adds their fake implementations).  Built into the attention layer's library.
 #include "fa3_torch_common.h"
 #include "shaobo_fa3_cache.h"
 
@@ -131,12 +131,14 @@ void check_rows(const Tensor& x, const Tensor& first, const Tensor& page_table, 
                       "page table's batch and GPU");
 }
 
-std::vector<Tensor> cache_append(const Tensor& k, const Tensor& v, Tensor k_pages, Tensor v_pages,
-                                 const Tensor& page_table, const Tensor& kv_lens,
-                                 const optional<Tensor>& new_lens, const optional<Tensor>& q,
-                                 const optional<Tensor>& positions, const optional<Tensor>& freqs,
-                                 bool interleaved, const optional<Tensor>& bounds) {
-    no_gradient({k, v, k_pages, v_pages, q, positions, freqs, bounds});
+// The append; turned q goes to q_out, or (fresh) to a tensor made here.
+optional<Tensor> append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages,
+                        const Tensor& page_table, const Tensor& kv_lens,
+                        const optional<Tensor>& new_lens, const optional<Tensor>& q,
+                        const optional<Tensor>& positions, const optional<Tensor>& freqs,
+                        bool interleaved, const optional<Tensor>& bounds, optional<Tensor> q_out,
+                        bool fresh) {
+    no_gradient({k, v, k_pages, v_pages, q, positions, freqs, bounds, q_out});
     TORCH_CHECK_VALUE(k.dim() == 4, "k must be [batch, heads, sequence, head_dim]");
     check_type(k.scalar_type(), "k");
     ShaoboFa3CacheAppendParams p;
@@ -195,16 +197,40 @@ std::vector<Tensor> cache_append(const Tensor& k, const Tensor& v, Tensor k_page
         p.cache.bounds = bounds->data_ptr();
     }
     const Guard guard(k.device());
-    std::vector<Tensor> out;
+    if (fresh && q.has_value()) q_out = like(*q);
+    TORCH_CHECK_VALUE(q.has_value() == q_out.has_value(), "q and q_out: both or neither");
     if (q.has_value()) {
-        out.push_back(like(*q));
-        p.q_out = view(out[0], "q's output");
+        check_rows(*q_out, k, page_table, "q_out");
+        TORCH_CHECK_VALUE(q_out->size(1) == q->size(1), "q_out must have q's heads");
+        p.q_out = view(*q_out, "q_out");
     }
     check_status(shaobo_fa3_cache_append(&p, stream_of(k)), "shaobo_fa3_cache_append");
     written(k_pages);
     written(v_pages);
     if (bounds.has_value()) written(*bounds);
-    return out;
+    if (!fresh && q_out.has_value()) written(*q_out);
+    return q_out;
+}
+
+std::vector<Tensor> cache_append(const Tensor& k, const Tensor& v, Tensor k_pages, Tensor v_pages,
+                                 const Tensor& page_table, const Tensor& kv_lens,
+                                 const optional<Tensor>& new_lens, const optional<Tensor>& q,
+                                 const optional<Tensor>& positions, const optional<Tensor>& freqs,
+                                 bool interleaved, const optional<Tensor>& bounds) {
+    const optional<Tensor> out = append(k, v, k_pages, v_pages, page_table, kv_lens, new_lens, q, positions,
+                                        freqs, interleaved, bounds, c10::nullopt, true);
+    return out.has_value() ? std::vector<Tensor>{*out} : std::vector<Tensor>{};
+}
+
+// The same with q's output given and nothing returned: the form that a traced
+// graph holds (functionalization knows no operator that writes and returns a list).
+void cache_append_into(const Tensor& k, const Tensor& v, Tensor k_pages, Tensor v_pages,
+                       const Tensor& page_table, const Tensor& kv_lens,
+                       const optional<Tensor>& new_lens, const optional<Tensor>& q,
+                       const optional<Tensor>& positions, const optional<Tensor>& freqs,
+                       bool interleaved, const optional<Tensor>& bounds, const optional<Tensor>& q_out) {
+    append(k, v, k_pages, v_pages, page_table, kv_lens, new_lens, q, positions, freqs, interleaved, bounds,
+           q_out, false);
 }
 
 std::tuple<Tensor, Tensor> cache_attn(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages,
@@ -345,6 +371,11 @@ TORCH_LIBRARY_FRAGMENT(shaobo_fa3, m) {
         "Tensor kv_lens, Tensor? new_lens=None, Tensor? q=None, Tensor? positions=None, "
         "Tensor? freqs=None, bool interleaved=False, Tensor(c!)? bounds=None) -> Tensor[]");
     m.def(
+        "cache_append_into(Tensor k, Tensor v, Tensor(a!) k_pages, Tensor(b!) v_pages, Tensor page_table, "
+        "Tensor kv_lens, Tensor? new_lens=None, Tensor? q=None, Tensor? positions=None, "
+        "Tensor? freqs=None, bool interleaved=False, Tensor(c!)? bounds=None, Tensor(d!)? q_out=None) "
+        "-> ()");
+    m.def(
         "cache_attn(Tensor q, Tensor k_pages, Tensor v_pages, Tensor page_table, Tensor kv_lens, "
         "Tensor? new_lens=None, bool causal=True, float? softmax_scale=None, float softcap=0.0, "
         "Tensor? slopes=None, Tensor? prefix_lens=None, Tensor? selected=None) -> (Tensor, Tensor)");
@@ -358,6 +389,7 @@ TORCH_LIBRARY_FRAGMENT(shaobo_fa3, m) {
 
 TORCH_LIBRARY_IMPL(shaobo_fa3, CUDA, m) {
     m.impl("cache_append", &cache_append);
+    m.impl("cache_append_into", &cache_append_into);
     m.impl("cache_attn", &cache_attn);
     m.impl("cache_select", &cache_select);
     m.impl("cache_read", &cache_read);

@@ -221,6 +221,8 @@ def attention(q, k, v, causal=True, softmax_scale=None):
 #
 #   torch.ops.shaobo_fa3.cache_append(k, v, k_pages!, v_pages!, page_table, kv_lens,
 #       new_lens, q, positions, freqs, interleaved, bounds!) -> [turned q] or []
+#   torch.ops.shaobo_fa3.cache_append_into(the same, q_out!) -> nothing; what
+#       cache_append becomes in a traced graph
 #   torch.ops.shaobo_fa3.cache_attn(q, k_pages, v_pages, page_table, kv_lens, new_lens,
 #       causal, softmax_scale, softcap, slopes, prefix_lens, selected) -> out, lse
 #   torch.ops.shaobo_fa3.cache_select(q, bounds, page_table, kv_lens, page_size, count,
@@ -274,6 +276,22 @@ if _ATTN:
     def _(k, v, k_pages, v_pages, page_table, kv_lens, new_lens=None, q=None, positions=None,
           freqs=None, interleaved=False, bounds=None):
         return [] if q is None else [torch.empty_like(q)]
+
+    @torch.library.register_fake("shaobo_fa3::cache_append_into")
+    def _(k, v, k_pages, v_pages, page_table, kv_lens, new_lens=None, q=None, positions=None,
+          freqs=None, interleaved=False, bounds=None, q_out=None):
+        return None
+
+    # Functionalization takes no operator that writes to arguments and returns a
+    # list, so a traced cache_append becomes cache_append_into.
+    @torch.ops.shaobo_fa3.cache_append.default.py_impl(
+        torch._C.DispatchKey.CompositeImplicitAutograd)
+    def _(k, v, k_pages, v_pages, page_table, kv_lens, new_lens=None, q=None, positions=None,
+          freqs=None, interleaved=False, bounds=None):
+        q_out = None if q is None else torch.empty_like(q)
+        torch.ops.shaobo_fa3.cache_append_into(k, v, k_pages, v_pages, page_table, kv_lens, new_lens,
+                                               q, positions, freqs, interleaved, bounds, q_out)
+        return [] if q is None else [q_out]
 
     @torch.library.register_fake("shaobo_fa3::cache_attn")
     def _(q, k_pages, v_pages, page_table, kv_lens, new_lens=None, causal=True, softmax_scale=None,

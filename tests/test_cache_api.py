@@ -208,6 +208,42 @@ def test_fake_implementations(T):
         assert sel.shape == (2, 4, 33, 5) and sel.dtype == torch.int32
 
 
+def test_appends_are_functionalized(T):
+    """A program that appends, with and without queries and bounds, becomes one graph
+    that returns what it wrote."""
+    from torch._functorch.aot_autograd import aot_export_module
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    class Step(torch.nn.Module):
+        def __init__(self, f):
+            super().__init__()
+            self.f = f
+
+        def forward(self, *tensors):
+            return self.f(*tensors)
+
+    def functions(k, v, kp, vp, t, n, q, b):
+        qt = T.cache_append(k, v, kp, vp, page_table=t, kv_lens=n, q=q, bounds=b)
+        assert T.cache_append(k, v, kp, vp, page_table=t, kv_lens=n) is None
+        return qt, T.cache_attention(qt, kp, vp, page_table=t, kv_lens=n)
+
+    def operators(k, v, kp, vp, t, n, q, b):
+        qt, = torch.ops.shaobo_fa3.cache_append(k, v, kp, vp, t, n, None, q, bounds=b)
+        assert torch.ops.shaobo_fa3.cache_append(k, v, kp, vp, t, n) == []
+        return qt, *torch.ops.shaobo_fa3.cache_attn(qt, kp, vp, t, n)
+
+    for f, outs in ((functions, 2), (operators, 3)):
+        with FakeTensorMode(), torch.no_grad():
+            k = torch.empty(2, 4, 33, 64, dtype=torch.bfloat16, device="cuda")
+            q = torch.empty(2, 33, 8, 64, dtype=torch.bfloat16, device="cuda").transpose(1, 2)
+            t = torch.empty(2, 9, dtype=torch.int32, device="cuda")
+            kp, vp, b = T.cache_pages(7, 4, 32, 64, torch.bfloat16, bounds=True)
+            graph, signature = aot_export_module(Step(f), (k, k, kp, vp, t, t[:, 0], q, b), trace_joint=False)
+        assert sorted(signature.user_inputs_to_mutate.values()) == sorted(signature.user_inputs[n] for n in (2, 3, 7))
+        assert len(signature.user_outputs) == outs
+        assert str(graph.graph).count("cache_append_into") == 2
+
+
 def test_refusals_without_a_gpu(T):
     q = torch.zeros(1, 1, 4, 64, dtype=torch.bfloat16)
     t = torch.zeros(1, 1, dtype=torch.int32)

@@ -574,3 +574,68 @@ def test_appends_count_as_writes(T):
         T.cache_append(s["k"], s["v"], kp, vp, bounds=bounds, **w)
         assert kp.abs().sum() > 0 and bounds.abs().sum() > 0
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("S,direct", [(1, False), (5, False), (3, True)])
+def test_a_step_is_traced(T, bits, S, direct):
+    """A step as one traced and functionalized graph: outputs and cache as the eager
+    step's, call after call; with and without queries and bounds."""
+    ops = torch.ops.shaobo_fa3
+
+    def run(k, v, kp, vp, q, fr, bounds, table, lens):
+        w = dict(page_table=table, kv_lens=lens)
+        if direct:
+            qt, = ops.cache_append(k, v, kp, vp, table, lens, None, q, None, fr, False, bounds)
+            assert ops.cache_append(k, v, kp, vp, table, lens, None, None, None, fr) == []
+        else:
+            qt = T.cache_append(k, v, kp, vp, q=q, freqs=fr, bounds=bounds, **w)
+            assert T.cache_append(k, v, kp, vp, freqs=fr, **w) is None
+        sel = T.cache_select(qt, bounds, page_size=64, count=4, **w)
+        return (qt, sel, *T.cache_attention(qt, kp, vp, return_lse=True, **w),
+                T.cache_attention(qt, kp, vp, selected=sel, **w))
+
+    names = ("k", "v", "kp", "vp", "q", "fr", "bounds", "table", "lens")
+    torch._dynamo.reset()
+    traced = torch.compile(run, backend="aot_eager", fullgraph=True)
+    s = step_state(T, bits, S)
+    with torch.no_grad():
+        for n in range(3):
+            other = step_state(T, bits, S, seed=30 + n)
+            for name in ("q", "k", "v"):
+                s[name].copy_(other[name])
+            s["lens"] += S
+            copy = dict(s, **{x: s[x].clone() for x in ("kp", "vp", "bounds")})
+            want = run(*(copy[x] for x in names))
+            got = traced(*(s[x] for x in names))
+            torch.cuda.synchronize()
+            assert all(torch.equal(x, y) for x, y in zip(want, got))
+            assert all(torch.equal(copy[x].view(torch.uint8), s[x].view(torch.uint8)) for x in ("kp", "vp", "bounds"))
+
+
+def test_an_append_into_a_tensor(T):
+    """cache_append_into: a tensor beside q, q itself, no q; what does not fit."""
+    s = step_state(T, 16, 5)
+    op, w = torch.ops.shaobo_fa3.cache_append_into, (s["table"], s["lens"], None)
+    kp, vp, bounds = (s[n].clone() for n in ("kp", "vp", "bounds"))
+    want = T.cache_append(s["k"], s["v"], kp, vp, q=s["q"], freqs=s["fr"], bounds=bounds, page_table=s["table"],
+                          kv_lens=s["lens"])
+    room = torch.full((3, 5, 8, 144), 7.0, dtype=BF, device="cuda")
+    for out in (room[..., 8:136].transpose(1, 2), torch.zeros_like(s["q"])):
+        assert op(s["k"], s["v"], s["kp"], s["vp"], *w, s["q"], None, s["fr"], False, s["bounds"], out) is None
+        assert torch.equal(out, want) and torch.equal(kp, s["kp"]) and torch.equal(vp, s["vp"])
+        assert torch.equal(bounds, s["bounds"])
+    assert (room[..., :8] == 7.0).all() and (room[..., 136:] == 7.0).all()
+    q = s["q"].clone()
+    op(s["k"], s["v"], s["kp"], s["vp"], *w, q, None, s["fr"], False, None, q)
+    assert torch.equal(q, want)
+    op(s["k"], s["v"], s["kp"], s["vp"], *w, None, None, s["fr"])
+    assert torch.equal(kp, s["kp"])
+    for q_out in (None, want[:, :4], want[:, :, :4], want.half(), want.cpu(), want[:2]):
+        refused("q_out", lambda: op(s["k"], s["v"], s["kp"], s["vp"], *w, s["q"], None, s["fr"], False, None, q_out))
+    refused("q_out", lambda: op(s["k"], s["v"], s["kp"], s["vp"], *w, None, None, s["fr"], False, None, want))
+    refused("no gradient", lambda: op(s["k"], s["v"], s["kp"], s["vp"], *w, s["q"], None, s["fr"], False, None,
+                                      want.clone().requires_grad_()))
+    args = (s["k"], s["v"], s["kp"], s["vp"], *w, s["q"], None, s["fr"], False, s["bounds"], torch.empty_like(s["q"]))
+    torch.library.opcheck(op.default, args, test_utils=("test_schema", "test_faketensor"))
+    torch.cuda.synchronize()

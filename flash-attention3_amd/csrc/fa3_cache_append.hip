@@ -52,6 +52,9 @@ struct AppendArgs {
     FastDiv div_segments, div_segments_k, div_row, div_hv;
 };
 
+// Lengths that an append follows: past any table by more rows than a call has.
+constexpr int kAppendPlaces = (1 << 30) + kMaxGrid;
+
 constexpr int kAppendThreads = 256;
 constexpr int kAppendWaves = kAppendThreads / 64;
 
@@ -424,16 +427,21 @@ __global__ __launch_bounds__(kAppendThreads) void cache_append_kernel(AppendArgs
     r.b = fdiv(is_k ? a.div_segments_k : a.div_segments, blockIdx.x);
     if (r.b >= a.batch) return;  // (k's runs may be longer, and fewer)
     const int seg = blockIdx.x - r.b * (is_k ? a.segments_k : a.segments), run = is_k ? a.run_k : a.run;
-    const int kv = cache_kv(a.c, r.b), fresh = cache_new(a.c, r.b, a.seqlen);
+    // (not taken into the table's places: a token past them is not written, one
+    // that is moved back would be, over another)
+    const int kv = cache_length(scalar_load(a.c.kv_lens + r.b), kAppendPlaces);
+    const int fresh = cache_new(a.c, r.b, a.seqlen);
     // rows i0 .. i1 - 1 of the call, at places place0 + i
     r.place0 = kv - fresh;
     const int run0 = ((r.place0 >> run) + seg) << run;
     r.i0 = max(run0 - r.place0, 0);
     r.i1 = min(run0 + (1 << run) - r.place0, a.seqlen);
     if (r.i0 >= r.i1) return;
-    // tokens among them: i0 .. t1 - 1 (a place below 0 or a page that is none: not written)
+    // tokens among them: i0 .. t1 - 1 (a place below 0 or past the table, or a page
+    // that is none: not written)
     r.page = -1;
-    if (run0 >= 0 && r.i0 < fresh) r.page = cache_page_scalar(a.c, r.b, (r.place0 + r.i0) >> a.c.shift);
+    if (run0 >= 0 && r.i0 < fresh && run0 < a.c.width << a.c.shift)
+        r.page = cache_page_scalar(a.c, r.b, (r.place0 + r.i0) >> a.c.shift);
     r.t1 = r.page >= 0 ? min(r.i1, fresh) : r.i0;
     const int per = is_q ? a.hq : is_k ? a.hk : a.hv;
     r.h0 = part * per;

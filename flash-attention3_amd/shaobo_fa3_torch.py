@@ -458,6 +458,7 @@ def cache_append(k, v, k_pages, v_pages, *, page_table, kv_lens, new_lens=None, 
                  [n * page_size, (n + 1) * page_size); a number that is no page:
                  nothing is written there
     kv_lens      int32 [B]: tokens of each sequence, the new ones included
+                 (those past the table's places are not written)
     new_lens     int32 [B]: how many of the S rows are tokens (default: all),
                  the rest is padding; token i is at place kv_lens - new_lens + i
     freqs        fp32 [axes, pairs] as rotary takes them; None: nothing is turned

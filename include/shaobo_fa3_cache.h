@@ -14,6 +14,8 @@
  * (taken into 0 .. width page_size).  Of the seqlen rows of q, k and v the
  * first new_lens[b] (taken into 0 .. seqlen; all, where there are none) are
  * tokens, the rest padding: token i is at place kv_lens[b] - new_lens[b] + i.
+ * An append alone follows lengths past the table, up to 2^30 + 2^24: it writes
+ * no token whose place is not in the table, and none over an earlier one.
  *
  * 16 bits: k and v are [pages, num_heads_kv, page_size, head_dim] in dtype.
  *

@@ -639,3 +639,33 @@ def test_an_append_into_a_tensor(T):
     args = (s["k"], s["v"], s["kp"], s["vp"], *w, s["q"], None, s["fr"], False, s["bounds"], torch.empty_like(s["q"]))
     torch.library.opcheck(op.default, args, test_utils=("test_schema", "test_faketensor"))
     torch.cuda.synchronize()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+@pytest.mark.parametrize("S,new", [(1, None), (4, None), (40, None), (9, [5, 0, 9, 2, 7, 1])])
+def test_tokens_past_the_table_are_not_written(T, bits, S, new):
+    """Lengths past the table's places: nothing held is written over, tokens that are
+    in the table go to their places, keys and queries turn by theirs -- as under a
+    wider table whose further pages are none."""
+    ps, width, B, D = 32, 2, 6, 64
+    gen = gen_of(6)
+    k, v, q = (rows(gen, B, h, S, D, BF) for h in (2, 2, 4))
+    fr = T.rotary_freqs([D // 2], device="cuda")
+    lens = i32([64, 65, 66, 64 + S, 64 + S // 2, 1 << 20])
+    table = torch.randperm(B * width, generator=gen, device="cuda").int().view(B, width)
+    results = []
+    for t in (table, torch.cat((table, torch.full((B, 1 << 15), -1, device="cuda").int()), 1)):
+        kp, vp, bounds = T.cache_pages(B * width, 2, ps, D, BF, bits=bits, bounds=True)
+        old = rows(gen_of(7), B, 2, 64, D, BF)
+        T.cache_append(old, old, kp, vp, page_table=table, kv_lens=i32([64] * B), bounds=bounds)
+        qt = T.cache_append(k, v, kp, vp, q=q, freqs=fr, bounds=bounds, page_table=t, kv_lens=lens,
+                            new_lens=None if new is None else i32(new))
+        results.append((kp.view(torch.uint8), vp.view(torch.uint8), bounds, qt))
+    for a, b in zip(*results):
+        assert torch.equal(a, b)
+    # lengths that no table has
+    kp, vp, bounds = (x.clone() for x in (kp, vp, bounds))
+    T.cache_append(k, v, kp, vp, q=q, freqs=fr, bounds=bounds, page_table=table, kv_lens=i32([2147483647] * B))
+    torch.cuda.synchronize()
+    assert torch.equal(kp.view(torch.uint8), results[0][0]) and torch.equal(vp.view(torch.uint8), results[0][1])
+    assert torch.equal(bounds, results[0][2])

@@ -4,6 +4,7 @@
 #include "fa3_torch_common.h"
 #include "shaobo_fa3_cache.h"
 
+#include <ATen/MemoryOverlap.h>
 #include <ATen/core/grad_mode.h>
 #include <c10/core/AutogradState.h>
 
@@ -27,6 +28,17 @@ void no_gradient(std::initializer_list<optional<Tensor>> tensors) {
         TORCH_CHECK_VALUE(!t.has_value() || !((backward && t->requires_grad()) ||
                                               (forward && t->_fw_grad(0).defined())),
                           "the cache's operators have no gradient: pass detached tensors");
+}
+
+// Two elements of what an append writes must not share memory: the call would
+// leave either one's value there.
+void check_written(const Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(at::has_internal_overlap(t) != at::MemOverlap::Yes, name,
+                      ": written to, it must not overlap itself");
+}
+bool apart(const Tensor& a, const Tensor& b) {
+    const at::MemOverlapStatus s = at::get_overlap_status(a, b);
+    return s != at::MemOverlapStatus::Full && s != at::MemOverlapStatus::Partial;
 }
 
 // Counts a write as autograd does, so that a backward that saved t misses its
@@ -144,6 +156,9 @@ optional<Tensor> append(const Tensor& k, const Tensor& v, const Tensor& k_pages,
     ShaoboFa3CacheAppendParams p;
     shaobo_fa3_cache_append_params_init(&p);
     p.cache = cache_of(k_pages, v_pages, page_table, kv_lens, new_lens, k.scalar_type(), k.size(3));
+    check_written(k_pages, "k_pages");
+    check_written(v_pages, "v_pages");
+    TORCH_CHECK_VALUE(apart(k_pages, v_pages), "k_pages and v_pages must not overlap");
     const int64_t B = k.size(0), S = k.size(2);
     check_rows(k, k, page_table, "k");
     check_rows(v, k, page_table, "v");
@@ -202,6 +217,9 @@ optional<Tensor> append(const Tensor& k, const Tensor& v, const Tensor& k_pages,
     if (q.has_value()) {
         check_rows(*q_out, k, page_table, "q_out");
         TORCH_CHECK_VALUE(q_out->size(1) == q->size(1), "q_out must have q's heads");
+        check_written(*q_out, "q_out");
+        TORCH_CHECK_VALUE(at::get_overlap_status(*q_out, *q) != at::MemOverlapStatus::Partial,
+                          "q_out must be q or lie apart from it");
         p.q_out = view(*q_out, "q_out");
     }
     check_status(shaobo_fa3_cache_append(&p, stream_of(k)), "shaobo_fa3_cache_append");

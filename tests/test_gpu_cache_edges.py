@@ -669,3 +669,25 @@ def test_tokens_past_the_table_are_not_written(T, bits, S, new):
     torch.cuda.synchronize()
     assert torch.equal(kp.view(torch.uint8), results[0][0]) and torch.equal(vp.view(torch.uint8), results[0][1])
     assert torch.equal(bounds, results[0][2])
+
+
+def test_written_tensors_that_overlap_are_refused(T):
+    """Pages that are one memory, by a stride of zero or k's and v's the same, are
+    read but not written; likewise q's output."""
+    for bits in (16, 4):
+        s = step_state(T, bits, 2)
+        w = dict(page_table=s["table"], kv_lens=s["lens"])
+        kp, vp = s["kp"], s["vp"]
+        for k_pages, v_pages in ((kp[:1].expand(60, -1, -1, -1), vp), (kp, vp[:, :1].expand(-1, 2, -1, -1)), (kp, kp),
+                                 (kp[:50], kp[10:])):
+            refused("overlap", lambda: T.cache_append(s["k"], s["v"], k_pages, v_pages, **w))
+            if k_pages.shape == v_pages.shape:
+                T.cache_attention(s["q"], k_pages, v_pages, **w)
+                T.cache_read(k_pages, v_pages, seqlen=10, dtype=BF, **w)
+        op, a = torch.ops.shaobo_fa3.cache_append_into, (s["k"], s["v"], kp, vp, s["table"], s["lens"], None)
+        room = torch.zeros(5, 8, 2, 128, dtype=BF, device="cuda")
+        room[1:4] = s["q"]
+        for q, q_out in ((s["q"], s["q"][:1].expand(3, -1, -1, -1)), (room[1:4], room[:3]), (room[1:4], room[2:])):
+            refused("overlap|apart", lambda: op(*a, q, None, s["fr"], False, None, q_out))
+        op(*a, room[1:4], None, s["fr"], False, None, room[1:4])
+    torch.cuda.synchronize()

@@ -495,8 +495,8 @@ def cache_select(q, bounds, *, page_table, kv_lens, page_size, count, new_lens=N
     """The `count` pages that each new token and KV head is to look at, int32
     [B, Hkv, S, count], ascending, -1 behind them: the token's own page, and of
     those before it the ones whose bounds allow the largest score of any head of
-    the group (for a positive softmax scale).  bounds as cache_append keeps them
-    (q turned as it returns it)."""
+    the group (for a positive softmax scale); pages that are none are left out.
+    bounds as cache_append keeps them (q turned as it returns it)."""
     _no_gradient(q, bounds)
     return torch.ops.shaobo_fa3.cache_select(q, bounds, page_table, kv_lens, page_size, count,
                                              new_lens)

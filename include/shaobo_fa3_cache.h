@@ -140,8 +140,9 @@ int shaobo_fa3_cache_attn(const ShaoboFa3CacheAttnParams* params, void* stream);
  *           sum_c max(q_c low_c, q_c high_c),    in fp64
  * (equal scores: the lower page; a page and head with a bound or a score that
  * is not finite comes before all that are).
- * Page numbers of the sequence, ascending, -1 behind them; all -1 for padding
- * and for a token whose own page is none, pages that are none are left out.
+ * Page numbers of the sequence, ascending, -1 behind them; pages that are none,
+ * the token's own among them, are left out, the others still listed.  All -1
+ * for padding and for a token whose place is below 0.
  * For a positive softmax scale; the cache's k and v are not looked at. */
 typedef struct ShaoboFa3CacheSelectParams {
     uint32_t struct_size;

@@ -691,3 +691,19 @@ def test_written_tensors_that_overlap_are_refused(T):
             refused("overlap|apart", lambda: op(*a, q, None, s["fr"], False, None, q_out))
         op(*a, room[1:4], None, s["fr"], False, None, room[1:4])
     torch.cuda.synchronize()
+
+
+def test_a_token_whose_own_page_is_none(T):
+    """Its own page is left out of the list as any absent page is; the others stay."""
+    s = step_state(T, 16)
+    table = s["table"].clone()
+    s["lens"] = i32([901, 451, 1])
+    table[0, 14], table[0, 2], table[1, 7], table[2, 0] = -1, 60, -5, 1 << 30
+    w = dict(page_table=table, kv_lens=s["lens"])
+    sel = T.cache_select(s["q"], s["bounds"], page_size=64, count=20, **w)
+    want = [[n for n in range(14) if n != 2], list(range(7)), []]
+    for b, pages in enumerate(want):
+        assert (sel[b, :, 0] == i32(pages + [-1] * (20 - len(pages)))).all()
+    few = T.cache_select(s["q"], s["bounds"], page_size=64, count=3, **w)
+    cache = dict(table=table, kv=[901, 451, 1], new=[1] * 3, page_size=64)
+    assert torch.equal(few, O.select(s["q"], s["bounds"], cache, 3)) and (few[0] >= 0).all()

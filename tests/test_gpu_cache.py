@@ -298,6 +298,25 @@ def test_append_other_head_dims(T, D):
     check_append(T, cache, k, v, q, dict(freqs=f, positions=None, interleaved=False), bounds)
 
 
+@pytest.mark.parametrize("bits,dtype", [(16, BF), (4, HF)])
+@pytest.mark.parametrize("kind", [torch.int32, torch.int64, torch.float32])
+@pytest.mark.parametrize("case", [
+    dict(kv=[33, 65], D=128, Hq=4, axes=1), dict(kv=[129], S=100, axes=2, D=128, Hq=4), dict(kv=[70, 60], S=9, axes=3, inter=True, Hq=2),
+    dict(kv=[10000], S=3, place="far", axes=1, D=128, Hq=2), dict(kv=[40, 90], new=[3, 5], S=7, axes=2),
+], ids=ids)
+def test_append_takes_positions_of_any_type(T, case, kind, bits, dtype):
+    """int32, int64 and fp32 (with quarters), below 0 too; as they lie, or a row of
+    positions that the batch shares and reads with strides."""
+    cache, k, v, q, o = append_case(case, bits, dtype)
+    x = (o["positions"] - 250).to(kind)
+    if kind == torch.float32:
+        x = x + 0.25 * torch.randint(0, 4, x.shape, generator=gen_of(3), device="cuda")
+    check_append(T, cache, k, v, q, dict(o, positions=x))
+    shared = x[:, :1].transpose(0, 2).contiguous().transpose(0, 2).expand_as(x)
+    bounds = torch.zeros(cache["k"].shape[0], k.shape[1], 2, k.shape[3], dtype=dtype, device="cuda")
+    check_append(T, cache, k, v, q, dict(o, positions=shared), bounds)
+
+
 def special_rows(dtype):
     """Rows at the levels' borders and of odd sizes: [n, 64]."""
     x = torch.zeros(16, 64)
@@ -398,3 +417,27 @@ def test_select(T, case, kind, dtype):
                          count=c["count"])
     torch.cuda.synchronize()
     assert torch.equal(got, O.select(q, x, cache, c["count"]))
+
+
+@pytest.mark.parametrize("kind", ["random", "equal", "coarse", "wild"])
+@pytest.mark.parametrize("count", [1, 64, 600])
+@pytest.mark.parametrize("width", [511, 512, 513, 1023, 1024, 1025, 2048, 2049, 4096, 4097])
+def test_select_at_the_pick_kernels_widths(T, width, count, kind):
+    """Tables as wide as a thread of the pick kernels has pages for, in registers or
+    not, and one more or less: all of it used, and half."""
+    gen, ps, D = gen_of(width), 32, 64
+    pages = width + 2
+    x = torch.randn(pages, 1, 2, D, generator=gen, device="cuda")
+    if kind == "equal":
+        x = x[:1].expand_as(x)
+    elif kind == "coarse":
+        x = x[torch.randint(0, 5, (pages,), generator=gen, device="cuda")]
+    x = x.sort(2)[0].to(BF).contiguous()
+    if kind == "wild":
+        x[::3, :, 1, 5], x[1::5, :, :, 0], x[2::7, :, 0, 3] = math.inf, math.nan, -math.inf
+    q = rows(gen, 1, 2, 1, D, BF)
+    table = torch.randperm(pages, generator=gen, device="cuda")[None, :width].int().contiguous()
+    for kv in (ps * width, ps * (width // 2) + 5):
+        got = T.cache_select(q, x, page_table=table, kv_lens=i32([kv]), page_size=ps, count=count)
+        torch.cuda.synchronize()
+        assert torch.equal(got, O.select(q, x, dict(table=table, kv=[kv], new=[1], page_size=ps), count))

@@ -72,8 +72,9 @@ __device__ __forceinline__ void two_terms(const RegReader<D>& rd, const FA3_LDS 
 // V's in bf16, and step() takes the rows' scales; a score is scaled and then
 // masked, where others are masked in their product's seed (a scale of zero
 // would make a NaN of it), and P is scaled before it is rounded, to bf16, whose
-// range holds any scale; for fp16 rows to two bf16 terms, 16 bits of it, and
-// two products.
+// range is fp32's (p is up to 2^kLazy, a scale a sixth of a row's largest value:
+// finite up to values of 2^120); for fp16 rows to two bf16 terms, 16 bits of it,
+// and two products.
 template <int D, bool kBf16, bool kCap, bool kBias, typename Args_ = AttnFwdArgs, bool kFour = false>
 struct FwdRows {
     typedef Args_ Args;

@@ -24,6 +24,9 @@
  * fp32; P and dS are rounded to the tensors' type before their products with
  * V, dO, Q and K, and the outputs once more (in fp16 a dS below 2^-14 loses
  * bits as gradients do: scale the loss).  Results are bitwise reproducible.
+ * The forward's sums of V are fp32, of weights up to 2^8 that are divided by
+ * their sum at the end: finite where |v| times 2^8 times the visible keys is
+ * below 2^127; larger values of bf16 may give infinities or NaN.
  *
  * Keys at kv and behind, and keys with a negative document, take no part
  * whatever their K and V hold (NaN included), and neither do queries that

@@ -103,6 +103,8 @@ int shaobo_fa3_cache_append(const ShaoboFa3CacheAppendParams* params, void* stre
  * j < prefix).  With `selected` only keys of the pages listed for (b, KV head,
  * i) are looked at: page numbers of the sequence, those outside [0, width) left
  * out, one that is listed twice counted twice.  Padding rows give zeros and -inf.
+ * As there, sums of V are finite where |v| times 2^8 times the visible keys is
+ * below 2^127.
  *
  * 4 bits: scores are of what the codes stand for, in fp32 (levels are exact in
  * 16 bits, the scale is applied to the product); P times a value's scale is

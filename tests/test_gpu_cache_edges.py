@@ -707,3 +707,23 @@ def test_a_token_whose_own_page_is_none(T):
     few = T.cache_select(s["q"], s["bounds"], page_size=64, count=3, **w)
     cache = dict(table=table, kv=[901, 451, 1], new=[1] * 3, page_size=64)
     assert torch.equal(few, O.select(s["q"], s["bounds"], cache, 3)) and (few[0] >= 0).all()
+
+
+@pytest.mark.parametrize("bits,dtype", [(16, BF), (4, BF), (4, HF)])
+@pytest.mark.parametrize("S", [1, 3, 100])
+def test_large_values(T, S, bits, dtype):
+    """V up to the size that the header promises: |v| times 2^8 times the keys below 2^127
+    (in fp16 the type's own largest)."""
+    kv = 500  # < 2^9
+    cache, q, o = attn_case(dict(kv=[kv, 70], S=S, Hq=8, D=128), bits, dtype)
+    top = 2.0 ** 110 if dtype == BF else 65504.0
+    x = O.rows_of(cache["v"], bits)
+    factor = top / float(x.abs().max())
+    if bits == 16:
+        cache["v"] = (cache["v"].double() * factor).to(dtype)
+    else:
+        code, scale = O.parts(cache["v"])
+        cache["v"] = O.pack(code, (scale.double() * factor).float())
+    assert float(O.rows_of(cache["v"], bits).abs().max()) > 0.99 * top
+    out, _ = check_attn(T, cache, q, o)
+    assert torch.isfinite(out).all()

@@ -21,14 +21,17 @@ void check_type(at::ScalarType t, const char* name) {
 }
 
 // No operator here has a gradient: a call that would leave one out is refused.
-void no_gradient(std::initializer_list<optional<Tensor>> tensors) {
-    const bool backward = at::GradMode::is_enabled();
-    const bool forward = c10::AutogradState::get_tls_state().get_fw_grad_mode();
-    for (const optional<Tensor>& t : tensors)
-        TORCH_CHECK_VALUE(!t.has_value() || !((backward && t->requires_grad()) ||
-                                              (forward && t->_fw_grad(0).defined())),
-                          "the cache's operators have no gradient: pass detached tensors");
+// (Looked at first: what autograd knows nothing of, nearly every tensor here.)
+void no_gradient(std::initializer_list<const Tensor*> tensors) {
+    for (const Tensor* t : tensors) {
+        if (t == nullptr || t->unsafeGetTensorImpl()->autograd_meta() == nullptr) continue;
+        const bool wanted =
+            (at::GradMode::is_enabled() && t->requires_grad()) ||
+            (c10::AutogradState::get_tls_state().get_fw_grad_mode() && t->_fw_grad(0).defined());
+        TORCH_CHECK_VALUE(!wanted, "the cache's operators have no gradient: pass detached tensors");
+    }
 }
+const Tensor* given(const optional<Tensor>& t) { return t.has_value() ? &*t : nullptr; }
 
 // Two elements of what an append writes must not share memory: the call would
 // leave either one's value there.
@@ -143,14 +146,13 @@ void check_rows(const Tensor& x, const Tensor& first, const Tensor& page_table, 
                       "page table's batch and GPU");
 }
 
-// The append; turned q goes to q_out, or (fresh) to a tensor made here.
-optional<Tensor> append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages,
-                        const Tensor& page_table, const Tensor& kv_lens,
-                        const optional<Tensor>& new_lens, const optional<Tensor>& q,
-                        const optional<Tensor>& positions, const optional<Tensor>& freqs,
-                        bool interleaved, const optional<Tensor>& bounds, optional<Tensor> q_out,
-                        bool fresh) {
-    no_gradient({k, v, k_pages, v_pages, q, positions, freqs, bounds, q_out});
+// The append; turned q goes to q_out, or (fresh) to a tensor made there.
+void append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tensor& v_pages,
+            const Tensor& page_table, const Tensor& kv_lens, const optional<Tensor>& new_lens,
+            const optional<Tensor>& q, const optional<Tensor>& positions, const optional<Tensor>& freqs,
+            bool interleaved, const optional<Tensor>& bounds, Tensor& q_out, bool fresh) {
+    no_gradient({&k, &v, &k_pages, &v_pages, given(q), given(positions), given(freqs), given(bounds),
+                 q_out.defined() ? &q_out : nullptr});
     TORCH_CHECK_VALUE(k.dim() == 4, "k must be [batch, heads, sequence, head_dim]");
     check_type(k.scalar_type(), "k");
     ShaoboFa3CacheAppendParams p;
@@ -213,21 +215,20 @@ optional<Tensor> append(const Tensor& k, const Tensor& v, const Tensor& k_pages,
     }
     const Guard guard(k.device());
     if (fresh && q.has_value()) q_out = like(*q);
-    TORCH_CHECK_VALUE(q.has_value() == q_out.has_value(), "q and q_out: both or neither");
-    if (q.has_value()) {
-        check_rows(*q_out, k, page_table, "q_out");
-        TORCH_CHECK_VALUE(q_out->size(1) == q->size(1), "q_out must have q's heads");
-        check_written(*q_out, "q_out");
-        TORCH_CHECK_VALUE(at::get_overlap_status(*q_out, *q) != at::MemOverlapStatus::Partial,
+    TORCH_CHECK_VALUE(q.has_value() == q_out.defined(), "q and q_out: both or neither");
+    if (!fresh && q.has_value()) {
+        check_rows(q_out, k, page_table, "q_out");
+        TORCH_CHECK_VALUE(q_out.size(1) == q->size(1), "q_out must have q's heads");
+        check_written(q_out, "q_out");
+        TORCH_CHECK_VALUE(at::get_overlap_status(q_out, *q) != at::MemOverlapStatus::Partial,
                           "q_out must be q or lie apart from it");
-        p.q_out = view(*q_out, "q_out");
     }
+    if (q.has_value()) p.q_out = view(q_out, "q_out");
     check_status(shaobo_fa3_cache_append(&p, stream_of(k)), "shaobo_fa3_cache_append");
     written(k_pages);
     written(v_pages);
     if (bounds.has_value()) written(*bounds);
-    if (!fresh && q_out.has_value()) written(*q_out);
-    return q_out;
+    if (!fresh && q.has_value()) written(q_out);
 }
 
 std::vector<Tensor> cache_append(const Tensor& k, const Tensor& v, Tensor k_pages, Tensor v_pages,
@@ -235,9 +236,11 @@ std::vector<Tensor> cache_append(const Tensor& k, const Tensor& v, Tensor k_page
                                  const optional<Tensor>& new_lens, const optional<Tensor>& q,
                                  const optional<Tensor>& positions, const optional<Tensor>& freqs,
                                  bool interleaved, const optional<Tensor>& bounds) {
-    const optional<Tensor> out = append(k, v, k_pages, v_pages, page_table, kv_lens, new_lens, q, positions,
-                                        freqs, interleaved, bounds, c10::nullopt, true);
-    return out.has_value() ? std::vector<Tensor>{*out} : std::vector<Tensor>{};
+    std::vector<Tensor> out(q.has_value() ? 1 : 0);
+    Tensor none;
+    append(k, v, k_pages, v_pages, page_table, kv_lens, new_lens, q, positions, freqs, interleaved, bounds,
+           out.empty() ? none : out[0], true);
+    return out;
 }
 
 // The same with q's output given and nothing returned: the form that a traced
@@ -247,8 +250,9 @@ void cache_append_into(const Tensor& k, const Tensor& v, Tensor k_pages, Tensor 
                        const optional<Tensor>& new_lens, const optional<Tensor>& q,
                        const optional<Tensor>& positions, const optional<Tensor>& freqs,
                        bool interleaved, const optional<Tensor>& bounds, const optional<Tensor>& q_out) {
-    append(k, v, k_pages, v_pages, page_table, kv_lens, new_lens, q, positions, freqs, interleaved, bounds,
-           q_out, false);
+    Tensor to = q_out.has_value() ? *q_out : Tensor();
+    append(k, v, k_pages, v_pages, page_table, kv_lens, new_lens, q, positions, freqs, interleaved, bounds, to,
+           false);
 }
 
 std::tuple<Tensor, Tensor> cache_attn(const Tensor& q, const Tensor& k_pages, const Tensor& v_pages,
@@ -258,7 +262,7 @@ std::tuple<Tensor, Tensor> cache_attn(const Tensor& q, const Tensor& k_pages, co
                                       const optional<Tensor>& slopes,
                                       const optional<Tensor>& prefix_lens,
                                       const optional<Tensor>& selected) {
-    no_gradient({q, k_pages, v_pages, slopes});
+    no_gradient({&q, &k_pages, &v_pages, given(slopes)});
     TORCH_CHECK_VALUE(q.dim() == 4, "q must be [batch, heads, sequence, head_dim]");
     check_type(q.scalar_type(), "q");
     ShaoboFa3CacheAttnParams p;
@@ -312,7 +316,7 @@ std::tuple<Tensor, Tensor> cache_attn(const Tensor& q, const Tensor& k_pages, co
 Tensor cache_select(const Tensor& q, const Tensor& bounds, const Tensor& page_table,
                     const Tensor& kv_lens, int64_t page_size, int64_t count,
                     const optional<Tensor>& new_lens) {
-    no_gradient({q, bounds});
+    no_gradient({&q, &bounds});
     TORCH_CHECK_VALUE(q.dim() == 4 && q.is_cuda(), "q must be [batch, heads, sequence, head_dim] on a GPU");
     check_type(q.scalar_type(), "q");
     TORCH_CHECK_VALUE(bounds.dim() == 4, "bounds must be [pages, heads_kv, 2, head_dim]");
@@ -363,7 +367,7 @@ Tensor cache_select(const Tensor& q, const Tensor& bounds, const Tensor& page_ta
 std::tuple<Tensor, Tensor> cache_read(const Tensor& k_pages, const Tensor& v_pages,
                                       const Tensor& page_table, const Tensor& kv_lens, int64_t seqlen,
                                       at::ScalarType dtype) {
-    no_gradient({k_pages, v_pages});
+    no_gradient({&k_pages, &v_pages});
     check_type(dtype, "dtype");
     ShaoboFa3CacheReadParams p;
     shaobo_fa3_cache_read_params_init(&p);

@@ -19,7 +19,8 @@
 // Bound by HBM where there is much to move: 8192 tokens of 32 + 8 heads of 128
 // channels 46 us, 4.4 TB/s; the fp64 work shows in 4 bits with bounds, where
 // each head's run forms its own angles (2 x 2048 such tokens: 29 us, their bytes
-// 17).  One token 4.4 us in the kernel, 2 of them its angles.
+// 17).  One token 4.3 us a call in a captured graph (4.8 in a kernel trace), 2 of
+// them its angles.
 //
 // read: a thread per 8 channels; 2 x 4096 places of 8 heads from 4 bits 10 us,
 // 4.3 TB/s.

@@ -7,12 +7,17 @@ namespace {
 
 int64_t ceil64(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Parts of the key axis for jobs of few rows: as many as fill the chip once,
-// and then up to twice as many where those leave the CUs less uneven (the most
-// jobs a CU has, by the parts' length).  16 sequences of up to 8192 in 16 bits,
-// each in as many parts, 128 jobs: 86 us
-// in 2 parts, 84 in 3, 70 in 4, 82 in 6, 76 in 8; 512 jobs that fill it
-// already, B64 S2048 in 4 bits: 26 whole, 29 in 2.  A part keeps 256 keys.
+// Parts of the key axis for jobs of few rows that are not dealt (few_slots says
+// which are): one sequence, more than 256, selected pages.  As many as fill the
+// chip once, and then up to twice as many where those leave the CUs less uneven
+// (the most jobs a CU has, by the parts' length); one where the jobs fill it
+// already.  A part keeps 256 keys.  Whole calls, us, the rule's choice first, D
+// 128.  One token and 8 KV heads, over 2048 keys in 16 bits: 10.3 in 8 parts, 13.2
+// in 4, 23.3 whole; over 16384: 21.7 in 64, 20.2 in 32, 22.0 in 16, 170 whole; over
+// 131072: 100 in 64, 105 in 128, 100 in 32; the same in 4 bits: 36.6 in 96, 41.0
+// in 128, 35.5 in 64, 44.5 in 32.  64 pages of 2048 in 4 bits: 21.7 in 16, 24.0 in
+// 8, 45.7 whole; 48 pages, 16 sequences: 63.2 in 4, 64.0 in 2, 65.7 in 6.  300
+// sequences of one KV head, over 8192: 246 in 2, 270 whole, 223 in 4.
 int few_splits(int64_t jobs, int fill, int64_t keys) {
     const int64_t most = keys / 256, least = fill / jobs;
     if (least < 1 || jobs >= fill || most < 2) return 1;
@@ -44,12 +49,13 @@ int few_slots(const CacheProblem& p, int64_t jobs, int fill) {
 // job and 1.33 (0.86) a job where it has more; parts of a sequence write their
 // sums and read them again at 4 TB/s, in a launch of 5; a job's beginning and
 // end are four steps.  How much of the places
-// is filled is not known here: all of them are taken to be.  (D 128, both
-// widths; measured, the estimate's choice first: 1531 tokens over 9211, 8 KV
-// heads, 300 us in 128 rows and 2 parts, 292 in 4, 350 whole, 365 in 64 rows
-// and 2; 8 times 64 over 8192, 106 in 128 rows and 4 parts, 129 in 64 and 2;
-// 2011 of 4 KV heads, 53 in 64 rows, 55 in 128 and 2 parts, 68 in 128; 512 of 8
-// KV heads, 18 in 64 rows, 21 in 128, 31 and 33 in 2 parts.)
+// is filled is not known here: all of them are taken to be.  (D 128; measured,
+// the estimate's choice first: 1531 tokens over 9211, 8 KV heads, in 4 bits 300
+// us in 128 rows and 2 parts, 293 in 4, 350 whole, 366 in 64 rows and 2, in 16 bits
+// 280, 270, 310, 315; 8 times 64 over 8192, 110 in 128 rows and 4 parts, 128 in 64
+// and 2; 2011 of 4 KV heads, 50 in 64 rows, 52 in 128 and 2 parts, 67 in 128; 512
+// of 8 KV heads, 18 in 64 rows, 21 in 128, 26 in 2 parts of either.  The choice is
+// within 4 % of the best of these.)
 void tile_plan(const CacheProblem& p, CachePlan* f) {
     const int64_t rows = (int64_t)p.group * p.sq, groups = (int64_t)p.batch * p.heads_kv;
     const double last = p.sk / 64.0;  // steps of the longest job, and of them all in the mean

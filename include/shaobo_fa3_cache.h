@@ -75,7 +75,8 @@ typedef struct ShaoboFa3Cache {
  * (bounds, where they are given, follow), and q_out = q turned likewise.
  * freqs NULL: nothing is turned.  positions NULL: one axis, a token's place;
  * otherwise as shaobo_fa3_rotary takes them.  Every row of q is turned,
- * padding too.  The turn is formed in fp64 and rounded once to dtype. */
+ * padding too.  The turn is formed in fp64 and becomes dtype by way of fp32, as a
+ * cast does. */
 typedef struct ShaoboFa3CacheAppendParams {
     uint32_t struct_size;
     int32_t seqlen;
@@ -164,8 +165,9 @@ size_t shaobo_fa3_cache_select_workspace_bytes(const ShaoboFa3CacheSelectParams*
 int shaobo_fa3_cache_select(const ShaoboFa3CacheSelectParams* params, void* stream);
 
 /* k and v [batch, num_heads_kv, seqlen, head_dim] in dtype: the first seqlen
- * places of every sequence as the cache holds them (4 bits: rounded to dtype
- * once), zeros at and behind kv_lens[b] and where there is no page. */
+ * places of every sequence as the cache holds them (4 bits: level times scale in
+ * fp32, rounded to dtype), zeros at and behind kv_lens[b] and where there is no
+ * page. */
 typedef struct ShaoboFa3CacheReadParams {
     uint32_t struct_size;
     int32_t seqlen;

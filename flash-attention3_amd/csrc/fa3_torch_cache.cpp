@@ -1,6 +1,7 @@
 // PyTorch operators of the paged cache: shaobo_fa3::cache_append (and
 // ::cache_append_into), ::cache_attn, ::cache_select and ::cache_read
-// (shaobo_fa3_torch.py adds their fake implementations).  Built into the attention layer's library.
+// (shaobo_fa3_torch.py adds their fake implementations).  Built into the
+// attention layer's library.
 #include "fa3_torch_common.h"
 #include "shaobo_fa3_cache.h"
 
@@ -38,10 +39,6 @@ const Tensor* given(const optional<Tensor>& t) { return t.has_value() ? &*t : nu
 void check_written(const Tensor& t, const char* name) {
     TORCH_CHECK_VALUE(at::has_internal_overlap(t) != at::MemOverlap::Yes, name,
                       ": written to, it must not overlap itself");
-}
-bool apart(const Tensor& a, const Tensor& b) {
-    const at::MemOverlapStatus s = at::get_overlap_status(a, b);
-    return s != at::MemOverlapStatus::Full && s != at::MemOverlapStatus::Partial;
 }
 
 // Counts a write as autograd does, so that a backward that saved t misses its
@@ -160,7 +157,9 @@ void append(const Tensor& k, const Tensor& v, const Tensor& k_pages, const Tenso
     p.cache = cache_of(k_pages, v_pages, page_table, kv_lens, new_lens, k.scalar_type(), k.size(3));
     check_written(k_pages, "k_pages");
     check_written(v_pages, "v_pages");
-    TORCH_CHECK_VALUE(apart(k_pages, v_pages), "k_pages and v_pages must not overlap");
+    // (that overlap in part may be one pool whose pages the table tells apart)
+    TORCH_CHECK_VALUE(at::get_overlap_status(k_pages, v_pages) != at::MemOverlapStatus::Full,
+                      "k_pages and v_pages must not overlap");
     const int64_t B = k.size(0), S = k.size(2);
     check_rows(k, k, page_table, "k");
     check_rows(v, k, page_table, "v");

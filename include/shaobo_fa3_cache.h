@@ -8,8 +8,8 @@
  * Pages.  Positions [n page_size, (n + 1) page_size) of sequence b are rows of
  * page page_table[b][n]; a number outside [0, pages) is no page: nothing is
  * written there, and its keys take no part.  A page belongs to one sequence
- * where it is written; sequences may share pages that are only read.  What is
- * written (pages of k and of v, q_out) must not overlap itself or the others.
+ * where it is written; sequences may share pages that are only read.  The rows
+ * that a call writes (of k, of v, of q_out) must not share memory.
  *
  * Lengths.  kv_lens[b] tokens are in the cache after the call's tokens are
  * (taken into 0 .. width page_size).  Of the seqlen rows of q, k and v the

@@ -678,8 +678,7 @@ def test_written_tensors_that_overlap_are_refused(T):
         s = step_state(T, bits, 2)
         w = dict(page_table=s["table"], kv_lens=s["lens"])
         kp, vp = s["kp"], s["vp"]
-        for k_pages, v_pages in ((kp[:1].expand(60, -1, -1, -1), vp), (kp, vp[:, :1].expand(-1, 2, -1, -1)), (kp, kp),
-                                 (kp[:50], kp[10:])):
+        for k_pages, v_pages in ((kp[:1].expand(60, -1, -1, -1), vp), (kp, vp[:, :1].expand(-1, 2, -1, -1)), (kp, kp)):
             refused("overlap", lambda: T.cache_append(s["k"], s["v"], k_pages, v_pages, **w))
             if k_pages.shape == v_pages.shape:
                 T.cache_attention(s["q"], k_pages, v_pages, **w)
@@ -690,6 +689,14 @@ def test_written_tensors_that_overlap_are_refused(T):
         for q, q_out in ((s["q"], s["q"][:1].expand(3, -1, -1, -1)), (room[1:4], room[:3]), (room[1:4], room[2:])):
             refused("overlap|apart", lambda: op(*a, q, None, s["fr"], False, None, q_out))
         op(*a, room[1:4], None, s["fr"], False, None, room[1:4])
+        # one pool, k's and v's pages in turn, beside pages of their own
+        pool = torch.zeros(61, *kp.shape[1:], dtype=kp.dtype, device="cuda")
+        even = dict(page_table=(2 * torch.randperm(30, generator=gen_of(1), device="cuda")).int().view(3, 10),
+                    kv_lens=i32([300, 64, 2]))
+        apart = [torch.zeros_like(kp), torch.zeros_like(vp)]
+        T.cache_append(s["k"], s["v"], *apart, **even)
+        T.cache_append(s["k"], s["v"], pool[:-1], pool[1:], **even)
+        assert torch.equal(pool[:-1][::2], apart[0][::2]) and torch.equal(pool[1:][::2], apart[1][::2])
     torch.cuda.synchronize()
 
 

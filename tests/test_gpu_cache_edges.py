@@ -734,3 +734,28 @@ def test_large_values(T, S, bits, dtype):
     assert float(O.rows_of(cache["v"], bits).abs().max()) > 0.99 * top
     out, _ = check_attn(T, cache, q, o)
     assert torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("bits", [16, 4])
+def test_an_append_takes_lengths_into_their_range(T, bits):
+    """Lengths below 0, more new tokens than rows or than the sequence has, fewer
+    than none: the same rows written as with lengths in range."""
+    gen = gen_of(2)
+    k, v, q = (rows(gen, 6, h, 9, 64, BF) for h in (2, 2, 4))
+    fr = T.rotary_freqs([32], device="cuda")
+    table = torch.randperm(24, generator=gen, device="cuda").int().view(6, 4)
+    got = []
+    for kv, new in (([-5, 100, 100, 3, 3, -2147483648], [4, 2147483647, -7, 2147483647, 5, -2147483648]),
+                    ([0, 100, 100, 3, 3, 0], [4, 9, 0, 9, 5, 0])):
+        kp, vp, bounds = T.cache_pages(24, 2, 32, 64, BF, bits=bits, bounds=True)
+        qt = T.cache_append(k, v, kp, vp, q=q, freqs=fr, bounds=bounds, page_table=table, kv_lens=i32(kv), new_lens=i32(new))
+        got.append((kp, vp, bounds, qt))
+    torch.cuda.synchronize()
+    for a, b in zip(*got):
+        assert torch.equal(a.view(torch.uint8), b.view(torch.uint8))
+    want = torch.zeros(24, 32, dtype=torch.bool, device="cuda")  # the rows that hold tokens
+    for b, places in ((1, range(91, 100)), (3, range(3)), (4, range(3))):
+        for p in places:
+            want[table[b, p // 32], p % 32] = True
+    written = kp != 0 if bits == 16 else O.parts(kp)[1][..., None] != 0
+    assert torch.equal(written.any(-1).any(1), want)

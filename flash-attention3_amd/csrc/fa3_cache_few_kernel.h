@@ -18,7 +18,7 @@
 // Two blocks' loads are out at a time; there is no barrier before the waves meet.
 //
 // Bound by HBM: 16 sequences of up to 8192 in 16 bits 62.6 us, 5.1 TB/s; 48 of up
-// to 16384 in 4 bits 108.6 us, 5.0 TB/s (the codes make 44 % of the SIMDs' cycles
+// to 16384 in 4 bits 108.6 us, 5.0 TB/s (the codes make 49 % of the SIMDs' cycles
 // vector instructions, matrix ones 14 %).  Where few keys are left to a wave,
 // its chain of loads, products and exponentials: 8 x 5 tokens over 6001 in 4
 // bits 16 us, one token over 129 6.1 (kernel trace; 4.7 a call in a captured graph).
